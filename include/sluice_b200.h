@@ -39,7 +39,8 @@ enum {
   SL_ERR_CUDA = 3,        /* CUDA runtime error */
   SL_ERR_UNSUPPORTED = 4, /* shape / dtype this build does not cover */
   SL_ERR_TIMEOUT = 5,     /* a bounded device wait ran out */
-  SL_ERR_NO_SCRATCH = 6   /* problem too large for sl_fused_experts_noalloc */
+  SL_ERR_NO_SCRATCH = 6,  /* problem too large for sl_fused_experts_noalloc */
+  SL_ERR_NO_BLOCKS = 7    /* sl_plan_kv_blocks: no free block, or no room in a table row */
 };
 
 /* Human-readable text for a status code. */
@@ -480,6 +481,93 @@ int sl_fused_experts_noalloc(const void* hidden, int T, int H, int I,
                              int n_shared, float routed_scaling_factor,
                              void* out, int32_t* status_out,
                              sl_stream_t stream);
+
+/* ------------------------------------------------------------ prompt pass
+ * Not part of the reference's MoE operator surface: what a decoder around
+ * the MoE layers needs to take whole prompts at once (the reference runs
+ * inside vLLM, whose block manager, rotary embedding and prefill attention
+ * these stand in for). */
+enum { SL_DTYPE_BF16 = 0, SL_DTYPE_FP16 = 1, SL_DTYPE_FP32 = 2 };
+
+/* Block tables and slot maps of a packed batch, from its requests' lengths,
+ * with no host round trip. Request r has context_lens[r] cached tokens and
+ * adds new_lens[r] (i32 [B]); its table row (i32, `table_width` wide, rows
+ * ld_table apart) holds ceil(context / block_size) blocks and is given the
+ * blocks that context + new tokens need, in request order, from the ring
+ * free_blocks (i32 [num_free_slots]), whose free entries are the positions
+ * [free_range[0], free_range[1]) modulo num_free_slots.
+ *   cu_new, cu_total  i32 [B + 1]: offsets of the new, and of all, tokens
+ *   positions, slots  i64 [T]: of each new token, its position in its
+ *                     sequence and its cache row block * block_size + offset
+ *   kv_slots          i64 [Tk]: the cache rows of all context + new tokens
+ *                     (Tk = 0: not wanted, may be NULL)
+ *   free_range_out    i64 [2]: the range with the taken blocks gone (may be
+ *                     free_range itself)
+ *   status            i32 [2]: status, blocks taken
+ * Rows behind the last request get position and slot -1. A request whose
+ * blocks the ring or its table row cannot hold takes none: its new tokens
+ * get slot -1, its table row stays as it was, and status becomes
+ * SL_ERR_NO_BLOCKS. Negative lengths count as 0, and more tokens than T or Tk
+ * are cut off (cu_new and cu_total stay within T and Tk): SL_ERR_INVALID.
+ * B in [1, 8192]. */
+int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new_lens, int B,
+                      int block_size, int32_t* block_table, int64_t ld_table, int table_width,
+                      const int32_t* free_blocks, int num_free_slots, const int64_t* free_range,
+                      int64_t* free_range_out, int64_t T, int64_t Tk, int32_t* cu_new,
+                      int32_t* cu_total, int64_t* positions, int64_t* slots, int64_t* kv_slots,
+                      int32_t* status, sl_stream_t stream);
+
+/* One tensor [T, heads, dim] of a rotary call: read from x, written to y
+ * (y = x with the same strides: in place). Strides in elements, the last
+ * dimension contiguous; columns [offset, offset + rot) are rotated. */
+typedef struct {
+  const void* x;
+  void* y;
+  int64_t x_token, x_head, y_token, y_head;
+  int heads, dim, offset;
+} sl_rotary_part;
+
+/* Rotary positions: row t at positions[t] (i64), pair j turned by
+ * 2 pi * positions[t] * turns[j] (f64 [rot / 2]) and scaled by `factor`, the
+ * angle reduced in 64 bits. interleaved: pairs (2j, 2j + 1); otherwise
+ * (j, j + rot / 2). Columns outside the rotated ones are copied. A row at a
+ * negative position (padding) is copied whole; in place it is left as it was.
+ * k may be NULL. rot even, at most 512; dim at most 4096; interleaved pairs
+ * start on a multiple of two elements. */
+int sl_rotary(const int64_t* positions, const double* turns, int T, int rot, int interleaved,
+              float factor, int dtype, const sl_rotary_part* q, const sl_rotary_part* k,
+              sl_stream_t stream);
+
+/* Causal attention over packed sequences. Sequence b's queries are rows
+ * [cu_q[b], cu_q[b+1]) of q and its keys and values rows
+ * [cu_k[b], cu_k[b+1]) of k and v (i32 [B + 1], offsets from 0); the queries
+ * are its last tokens: query i sees the keys 0 .. i + (keys - queries).
+ *   q   [Tq, heads, dim]; k [Tk, kv_heads, dim - shared_dim];
+ *   v   [Tk, kv_heads, v_dim]; out [Tq, heads, v_dim]
+ *   k_shared [Tk, shared_dim]: the last columns of every head's keys (NULL
+ *       with shared_dim = 0: k has all dim columns)
+ * out = softmax(scale * q k^T) v per head, head h reading key head
+ * h / (heads / kv_heads). A query that sees no key gets zeros; rows of q that
+ * belong to no sequence leave their output rows as they were; keys and
+ * values that no query may see do not reach the output, whatever they hold.
+ * Strides in elements, last dimension contiguous, multiples of 8; addresses
+ * 16-byte aligned. bf16 or fp16; (dim, v_dim) one of (64, 64), (128, 128),
+ * (192, 128); shared_dim 0 or, at dim 192, 64; at most 128 heads per key
+ * head. The workspace (sl_prompt_attention_workspace_bytes) starts with a
+ * status word: SL_OK, or SL_ERR_TIMEOUT when a bounded wait ran out. */
+typedef struct {
+  const void *q, *k, *v, *k_shared;
+  void* out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, k_shared_token, out_token, out_head;
+  const int32_t *cu_q, *cu_k;
+  int64_t Tq, Tk;
+  int B, heads, kv_heads, dim, v_dim, shared_dim, dtype;
+  float scale;
+} sl_attention_args;
+size_t sl_prompt_attention_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads,
+                                           int v_dim);
+int sl_prompt_attention(const sl_attention_args* args, void* workspace, size_t workspace_bytes,
+                        sl_stream_t stream);
 
 #ifdef __cplusplus
 }

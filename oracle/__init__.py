@@ -19,6 +19,9 @@ Contents (each function cites the reference file:line it restates):
   expert MLP, weighted top-k sum, shared experts, fp8 128x128 block-scale
   dequantisation), restated from vLLM's ``cpu_fused_moe_torch`` and
   ``fused_moe.py``. Pinned against vLLM's ``cpu_fused_moe_torch`` run here.
+* ``prompt`` — the prompt pass (block planner, rotary positions, causal
+  attention over packed sequences) from its definitions, in plain integers
+  and 64 bits; nothing of it is in the reference.
 
 Tie rule: the reference's ``torch.topk(sorted=False)`` leaves the order (and,
 at an exact tie on the k-th score, the choice) of the selected experts

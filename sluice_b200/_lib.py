@@ -23,6 +23,7 @@ SL_ERR_CUDA = 3
 SL_ERR_UNSUPPORTED = 4
 SL_ERR_TIMEOUT = 5
 SL_ERR_NO_SCRATCH = 6
+SL_ERR_NO_BLOCKS = 7
 
 SEG_FREE, SEG_PROBATION, SEG_PROTECTED, SEG_PINNED = 0, 1, 2, 3
 PLAN_FAST_HIT = 1
@@ -46,8 +47,10 @@ WAVE_NFIELDS = 5
 
 _c = ctypes
 _vp, _i, _sz, _f = _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_float
+_i64 = _c.c_int64
 
 WEIGHTS_BF16, WEIGHTS_FP8_BLOCK128 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 
 
 class ExpertWeights(ctypes.Structure):
@@ -57,6 +60,24 @@ class ExpertWeights(ctypes.Structure):
                 ("num_slots", _i), ("shared_w13", _vp), ("shared_w2", _vp),
                 ("shared_w13_scale", _vp), ("shared_w2_scale", _vp), ("n_shared", _i),
                 ("dtype", _i)]
+
+
+class RotaryPart(ctypes.Structure):
+    """``sl_rotary_part`` (include/sluice_b200.h)."""
+
+    _fields_ = [("x", _vp), ("y", _vp), ("x_token", _i64), ("x_head", _i64), ("y_token", _i64),
+                ("y_head", _i64), ("heads", _i), ("dim", _i), ("offset", _i)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """``sl_attention_args`` (include/sluice_b200.h)."""
+
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "k_shared", "out")] + \
+        [(n, _i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head",
+                             "k_shared_token", "out_token", "out_head")] + \
+        [("cu_q", _vp), ("cu_k", _vp), ("Tq", _i64), ("Tk", _i64)] + \
+        [(n, _i) for n in ("B", "heads", "kv_heads", "dim", "v_dim", "shared_dim", "dtype")] + \
+        [("scale", _f)]
 
 
 _SIGNATURES = {
@@ -105,6 +126,12 @@ _SIGNATURES = {
     "sl_linear_small": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp]),
     "sl_mla_decode": (_i, [_vp, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                            _i, _i, _f, _vp, _vp]),
+    "sl_plan_kv_blocks": (_i, [_vp, _vp, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _vp, _i64, _i64,
+                               _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sl_rotary": (_i, [_vp, _vp, _i, _i, _i, _f, _i, _c.POINTER(RotaryPart),
+                       _c.POINTER(RotaryPart), _vp]),
+    "sl_prompt_attention_workspace_bytes": (_sz, [_i, _i64, _i64, _i, _i, _i]),
+    "sl_prompt_attention": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp]),
 }
 
 _lock = threading.Lock()
@@ -154,7 +181,8 @@ def status_text(status: int) -> str:
     except Exception:  # library not loadable: plain text
         return {0: "ok", 1: "overflow", 2: "invalid argument", 3: "CUDA error",
                 4: "unsupported", 5: "timeout",
-                6: "problem too large for the no-alloc scratch"}.get(int(status), "unknown")
+                6: "problem too large for the no-alloc scratch",
+                7: "no free cache blocks"}.get(int(status), "unknown")
 
 
 def check(rc: int, what: str) -> None:

@@ -1,0 +1,534 @@
+// The prompt pass's small operators: the KV block planner (block tables and
+// slot maps from request lengths) and rotary positions.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace {
+
+// ------------------------------------------------------------ block planner
+// Request r holds held = ceil(context / bs) blocks and needs
+// need = ceil((context + new) / bs). With take = need - held and
+// off = the sum of take over the requests before it, its i-th new block is
+// free[(head + off + i) mod N]. Token i of the request sits at position
+// context + i, in slot block(position / bs) * bs + position mod bs.
+//
+// Every CTA makes the same scan over the requests in shared memory and then
+// fills its share of the tables and maps. A new block's id is read from the
+// free ring, not from the table, so no CTA waits for another's table writes;
+// the ring's range is read by all and written by none of a launch of several
+// CTAs that updates it in place (plan_range_kernel then writes it).
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxRequests = 8192;
+constexpr int kPlanChunk = 512;  // consecutive rows that a warp fills
+
+struct PlanArgs {
+  const int32_t* context;
+  const int32_t* fresh;
+  int B, bs, width, N;
+  int64_t T, Tk;
+  int32_t* table;
+  int64_t ld_table;
+  const int32_t* free_blocks;
+  const int64_t* range;
+  int64_t* range_out;
+  int32_t* cu_new;
+  int32_t* cu_total;
+  int64_t* positions;
+  int64_t* slots;
+  int64_t* kv_slots;
+  int32_t* status;
+  int write_range;
+};
+
+struct Lengths {
+  int context, fresh, held, take;
+  bool invalid, refused;
+};
+
+// One request's lengths, made safe: negative ones count as zero, and a
+// request that does not fit its table row takes nothing.
+__device__ __forceinline__ Lengths plan_lengths(const PlanArgs& a, int r) {
+  Lengths l;
+  l.context = a.context[r];
+  l.fresh = a.fresh[r];
+  l.invalid = l.context < 0 || l.fresh < 0;
+  l.context = max(l.context, 0);
+  l.fresh = max(l.fresh, 0);
+  const int64_t total = static_cast<int64_t>(l.context) + l.fresh;
+  const int64_t held = (static_cast<int64_t>(l.context) + a.bs - 1) / a.bs;
+  const int64_t need = (total + a.bs - 1) / a.bs;
+  l.refused = need > a.width;
+  l.invalid |= held > a.width;
+  l.held = static_cast<int>(held);
+  l.take = l.refused ? 0 : static_cast<int>(need - held);
+  return l;
+}
+
+__device__ __forceinline__ int saturated(int64_t v) {
+  return static_cast<int>(v < 0x7fffffff ? v : 0x7fffffff);
+}
+
+// Inclusive scan of three sums over the CTA (each warp by shuffles, then
+// the warps' totals); `tot` receives the CTA's sums.
+__device__ __forceinline__ void scan3(int64_t (&v)[3], int64_t (*warp_sum)[32], int64_t (&tot)[3]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v[k], o);
+      if (lane >= o) v[k] += u;
+    }
+    if (lane == 31) warp_sum[k][warp] = v[k];
+  }
+  __syncthreads();
+  if (warp < 3) {
+    int64_t s = lane < nw ? warp_sum[warp][lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    warp_sum[warp][lane] = s;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (warp > 0) v[k] += warp_sum[k][warp - 1];
+    tot[k] = warp_sum[k][nw - 1];
+  }
+  __syncthreads();
+}
+
+// The request that row t of a packed batch belongs to, known to lie in
+// [lo, hi]: the last r with cu[r] <= t.
+__device__ __forceinline__ int find_request(const int* cu, int t, int lo, int hi) {
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a) {
+  extern __shared__ int plan_sm[];
+  __shared__ int64_t warp_sum[3][32];
+  __shared__ int s_invalid, s_short, s_end;
+  int* cu_new = plan_sm;                 // [B + 1]
+  int* cu_total = cu_new + a.B + 1;      // [B + 1]
+  int* off = cu_total + a.B + 1;         // [B] blocks taken before, -1: refused
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid == 0) {
+    s_invalid = s_short = s_end = 0;
+    cu_new[0] = cu_total[0] = 0;
+  }
+  sl::pdl_wait();
+  sl::pdl_trigger();
+  int64_t head = a.range[0];
+  int64_t avail = a.range[1] - head;
+  const bool bad_range = avail < 0 || avail > a.N || head < 0;
+  if (bad_range) head = avail = 0;
+  __syncthreads();
+
+  // the scan: rows before each request and blocks taken before it
+  int64_t carry[3] = {0, 0, 0};
+  for (int r0 = 0; r0 < a.B; r0 += blockDim.x) {
+    const int r = r0 + tid;
+    Lengths l = {};
+    if (r < a.B) l = plan_lengths(a, r);
+    int64_t v[3] = {l.fresh, static_cast<int64_t>(l.context) + l.fresh, l.take}, tot[3];
+    scan3(v, warp_sum, tot);
+    if (r < a.B) {
+      const int64_t end = carry[2] + v[2];
+      // a request is served when its blocks end inside the free range, or
+      // when it needs none
+      const bool short_of = l.take > 0 && end > avail;
+      cu_new[r + 1] = saturated(carry[0] + v[0]);
+      cu_total[r + 1] = saturated(carry[1] + v[1]);
+      off[r] = l.refused || short_of ? -1 : saturated(end - l.take);
+      if (l.take > 0 && !short_of) atomicMax(&s_end, saturated(end));
+      if (l.invalid) s_invalid = 1;
+      if (l.refused || short_of) s_short = 1;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) carry[k] += tot[k];
+  }
+  __syncthreads();
+  // more rows than the outputs hold, or than 32-bit offsets count
+  const bool over = carry[0] > a.T || carry[1] > 0x7fffffff || (a.Tk > 0 && carry[1] > a.Tk);
+
+  const int gwarp = (blockIdx.x * blockDim.x + tid) >> 5, nwarps = (gridDim.x * blockDim.x) >> 5;
+  // the i-th free block: head and i are at most the ring's size
+  const int64_t ring_at = head % a.N;
+  auto new_block = [&](int i) -> int {
+    int64_t at = ring_at + i;
+    if (at >= a.N) at -= a.N;
+    return a.free_blocks[at];
+  };
+  auto block_of = [&](int r, int held, int o, int blk) -> int {
+    if (blk < held) return blk < a.width ? a.table[static_cast<int64_t>(r) * a.ld_table + blk] : -1;
+    if (o < 0) return -1;
+    return new_block(o + (blk - held));
+  };
+  auto slot_of = [&](int r, int context, int pos) -> int64_t {
+    const unsigned blk = static_cast<unsigned>(pos) / static_cast<unsigned>(a.bs);
+    const int held = static_cast<int>((static_cast<int64_t>(context) + a.bs - 1) / a.bs);
+    const int o = off[r];
+    // a refused request's new rows have no slot, even inside its last block
+    const int b = o < 0 && pos >= context ? -1 : block_of(r, held, o, static_cast<int>(blk));
+    return b < 0 ? -1 : static_cast<int64_t>(b) * a.bs + (pos - static_cast<int>(blk) * a.bs);
+  };
+  // rows of a packed batch, kPlanChunk consecutive ones per warp and turn
+  auto fill = [&](const int* cu, int64_t rows, bool all_rows) {
+    const int used = cu[a.B];
+    for (int64_t c0 = static_cast<int64_t>(gwarp) * kPlanChunk; c0 < rows;
+         c0 += static_cast<int64_t>(nwarps) * kPlanChunk) {
+      const int64_t c1 = min(rows, c0 + kPlanChunk);
+      int lo = 0, hi = 0;
+      if (c0 < used) {
+        lo = find_request(cu, static_cast<int>(c0), 0, a.B - 1);
+        hi = find_request(cu, static_cast<int>(min(c1, static_cast<int64_t>(used)) - 1), lo, a.B - 1);
+      }
+      for (int64_t t = c0 + lane; t < c1; t += 32) {
+        int64_t slot = -1, pos = -1;
+        if (t < used) {
+          const int r = find_request(cu, static_cast<int>(t), lo, hi);
+          const int context = (cu_total[r + 1] - cu_total[r]) - (cu_new[r + 1] - cu_new[r]);
+          const int p = static_cast<int>(t) - cu[r] + (all_rows ? 0 : context);
+          pos = p;
+          slot = slot_of(r, context, p);
+        }
+        if (all_rows) {
+          a.kv_slots[t] = slot;
+        } else {
+          a.positions[t] = pos;
+          a.slots[t] = slot;
+        }
+      }
+    }
+  };
+  fill(cu_new, a.T, false);
+  if (a.kv_slots != nullptr) fill(cu_total, a.Tk, true);
+
+  // the table rows of the requests that take blocks: a warp per request
+  for (int r = gwarp; r < a.B; r += nwarps) {
+    const int o = off[r];
+    const Lengths l = plan_lengths(a, r);
+    if (o < 0 || l.take == 0) continue;
+    int32_t* row = a.table + static_cast<int64_t>(r) * a.ld_table + l.held;
+    for (int i = lane; i < l.take; i += 32) row[i] = new_block(o + i);
+  }
+  if (blockIdx.x == 0) {
+    // offsets that a reader may follow: never past the rows that were filled
+    const int cap = saturated(a.T), cap_k = a.Tk > 0 ? saturated(a.Tk) : 0x7fffffff;
+    for (int r = tid; r <= a.B; r += blockDim.x) {
+      a.cu_new[r] = min(cu_new[r], cap);
+      a.cu_total[r] = min(cu_total[r], cap_k);
+    }
+    if (tid == 0) {
+      a.status[0] = s_invalid || bad_range || over ? SL_ERR_INVALID
+                    : s_short                      ? SL_ERR_NO_BLOCKS
+                                                   : SL_OK;
+      a.status[1] = s_end;
+      if (a.write_range) {
+        const int64_t first = a.range[0], tail = a.range[1];
+        a.range_out[0] = first + s_end;
+        a.range_out[1] = tail;
+      }
+    }
+  }
+}
+
+// The free range of a plan that several CTAs read, moved on in place.
+__global__ void plan_range_kernel(int64_t* range, const int32_t* status) {
+  sl::pdl_wait();
+  sl::pdl_trigger();
+  range[0] += status[1];
+}
+
+// ------------------------------------------------------------------- rotary
+// A pair (a, b) of a head at position p becomes (a cos t - b sin t,
+// b cos t + a sin t) times a factor, t = p * freq. The angle is formed in
+// turns, p * (freq / 2 pi), in 64 bits, whole turns taken off there, and only
+// the rest (at most half a turn) goes to 32 bits, so a position of a million
+// keeps as many bits of its phase as position one. Pairs are adjacent columns
+// (interleaved) or columns rot / 2 apart (half).
+constexpr int kRotThreads = 256;
+constexpr int kRotMaxPairs = 256;
+
+struct RotTensor {
+  const void* x;
+  void* y;
+  int64_t xs, xh, ys, yh;  // strides of a token and a head, in elements
+  int heads, offset;
+  int units;               // units of a head: its rotated ones, then the copied
+  uint32_t units_mul;      // index / units == (index * units_mul) >> 32
+};
+
+struct RotArgs {
+  const int64_t* positions;
+  const double* turns;  // [rot / 2] turns per position
+  float factor;
+  int T, rot, per_cta, rot_units;
+  RotTensor t[2];
+};
+
+template <typename E>
+__device__ __forceinline__ float to_f(E v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename E>
+__device__ __forceinline__ E from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+template <typename E, int V>
+struct alignas(sizeof(E) * V) RotVec {
+  E e[V];
+};
+
+// A unit is V adjacent columns of a head (interleaved: V / 2 pairs), or V
+// columns and the V columns rot / 2 further (half: V pairs). V elements are
+// one load: 16 bytes where the sizes, strides and addresses allow it.
+template <typename E, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
+  extern __shared__ float2 cs[];  // [per_cta][rot / 2] (cos, sin) * factor
+  __shared__ int s_skip[32];
+  using Vec = RotVec<E, V>;
+  sl::pdl_wait();
+  sl::pdl_trigger();
+  const int half = a.rot >> 1;
+  const int t0 = blockIdx.x * a.per_cta;
+  const int nt = min(a.per_cta, a.T - t0);
+  for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+    const int t = i / half, j = i - t * half;
+    const int64_t p = a.positions[t0 + t];
+    const double turns = static_cast<double>(p) * a.turns[j];
+    float s, c;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+    cs[i] = make_float2(c * a.factor, s * a.factor);
+    if (j == 0) s_skip[t] = p < 0;
+  }
+  __syncthreads();
+  const int nq = a.t[0].heads * a.t[0].units, n = nq + a.t[1].heads * a.t[1].units;
+  constexpr int U = 4;  // items in flight per thread
+  for (int i0 = threadIdx.x; i0 < nt * n; i0 += blockDim.x * U) {
+    Vec lo[U], hi[U];
+    E* dst[U];
+    int pair[U];  // first pair's place in cs, -1: copied
+    bool live[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * blockDim.x;
+      live[u] = i < nt * n;
+      if (!live[u]) continue;
+      const int t = i / n, w = i - t * n;
+      const RotTensor& x = w < nq ? a.t[0] : a.t[1];
+      const int idx = w < nq ? w : w - nq;
+      const int head = x.units == 1 ? idx
+                                    : static_cast<int>(__umulhi(static_cast<uint32_t>(idx), x.units_mul));
+      const int unit = idx - head * x.units;
+      int col;
+      if (unit < a.rot_units) {
+        col = x.offset + unit * V;
+        pair[u] = s_skip[t] ? -2 : t * half + (kInterleaved ? unit * (V / 2) : unit * V);
+      } else {
+        // columns that are not rotated: those before the rotated ones, then
+        // those behind them
+        const int c = (unit - a.rot_units) * V;
+        col = c < x.offset ? c : c + a.rot;
+        pair[u] = -1;
+      }
+      const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
+      dst[u] = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
+      lo[u] = *reinterpret_cast<const Vec*>(src);
+      if (!kInterleaved && unit < a.rot_units) hi[u] = *reinterpret_cast<const Vec*>(src + half);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!live[u]) continue;
+      if (pair[u] >= 0) {
+        if constexpr (kInterleaved) {
+#pragma unroll
+          for (int k = 0; k < V / 2; ++k) {
+            const float2 c = cs[pair[u] + k];
+            const float x0 = to_f(lo[u].e[2 * k]), x1 = to_f(lo[u].e[2 * k + 1]);
+            lo[u].e[2 * k] = from_f<E>(x0 * c.x - x1 * c.y);
+            lo[u].e[2 * k + 1] = from_f<E>(x1 * c.x + x0 * c.y);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float2 c = cs[pair[u] + k];
+            const float x0 = to_f(lo[u].e[k]), x1 = to_f(hi[u].e[k]);
+            lo[u].e[k] = from_f<E>(x0 * c.x - x1 * c.y);
+            hi[u].e[k] = from_f<E>(x1 * c.x + x0 * c.y);
+          }
+        }
+      }
+      *reinterpret_cast<Vec*>(dst[u]) = lo[u];
+      if (!kInterleaved && pair[u] != -1) *reinterpret_cast<Vec*>(dst[u] + half) = hi[u];
+    }
+  }
+}
+
+template <typename E, bool kInterleaved>
+cudaError_t launch_rotary(const RotArgs& a, int v, dim3 grid, size_t smem, cudaStream_t st) {
+  switch (v) {
+    case 8:
+      if constexpr (sizeof(E) == 2)
+        return sl::launch(rotary_kernel<E, 8, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
+      return cudaErrorInvalidValue;
+    case 4: return sl::launch(rotary_kernel<E, 4, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
+    case 2: return sl::launch(rotary_kernel<E, 2, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
+    default:
+      if constexpr (!kInterleaved)
+        return sl::launch(rotary_kernel<E, 1, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
+      return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new_lens, int B,
+                                 int block_size, int32_t* block_table, int64_t ld_table,
+                                 int table_width, const int32_t* free_blocks, int num_free_slots,
+                                 const int64_t* free_range, int64_t* free_range_out, int64_t T,
+                                 int64_t Tk, int32_t* cu_new, int32_t* cu_total,
+                                 int64_t* positions, int64_t* slots, int64_t* kv_slots,
+                                 int32_t* status, sl_stream_t stream) {
+  if (B <= 0 || block_size <= 0 || table_width <= 0 || ld_table < table_width ||
+      num_free_slots <= 0 || T < 0 || Tk < 0 || (Tk > 0 && !kv_slots))
+    return SL_ERR_INVALID;
+  if (B > kPlanMaxRequests) return SL_ERR_UNSUPPORTED;
+  if (!context_lens || !new_lens || !block_table || !free_blocks || !free_range ||
+      !free_range_out || !cu_new || !cu_total || !status || (T > 0 && (!positions || !slots)))
+    return SL_ERR_INVALID;
+  PlanArgs a = {context_lens, new_lens, B, block_size, table_width, num_free_slots, T, Tk,
+                block_table, ld_table, free_blocks, free_range, free_range_out, cu_new, cu_total,
+                positions, slots, Tk > 0 ? kv_slots : nullptr, status, 1};
+  // one CTA for what it fills in about two turns of its warps, else a CTA per
+  // as much, at most one per SM
+  const int64_t rows = T + Tk, per_cta = 2 * kPlanChunk * (kPlanThreads / 32);
+  int64_t grid = (rows + per_cta - 1) / per_cta;
+  const int sms = sl_device_sm_count();
+  if (sms <= 0) return SL_ERR_CUDA;
+  grid = grid < 1 ? 1 : (grid > sms ? sms : grid);
+  const bool in_place = free_range_out == free_range;
+  a.write_range = !(in_place && grid > 1);
+  const size_t smem = sizeof(int) * (3 * static_cast<size_t>(B) + 2);
+  static std::atomic<uint64_t> smem_set{0};
+  if (smem > 40 * 1024)
+    SL_CUDA_TRY(sl::ensure_smem_limit(plan_kv_blocks_kernel,
+                                      sizeof(int) * (3 * kPlanMaxRequests + 2), smem_set));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  SL_CUDA_TRY(sl::launch(plan_kv_blocks_kernel, dim3(static_cast<unsigned>(grid)),
+                         dim3(kPlanThreads), smem, st, a));
+  if (!a.write_range)
+    SL_CUDA_TRY(sl::launch(plan_range_kernel, dim3(1), dim3(1), 0, st, free_range_out,
+                           static_cast<const int32_t*>(status)));
+  return SL_OK;
+}
+
+extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, int rot,
+                         int interleaved, float factor, int dtype, const sl_rotary_part* q,
+                         const sl_rotary_part* k, sl_stream_t stream) {
+  if (T < 0 || rot <= 0 || rot % 2 || !q || dtype < SL_DTYPE_BF16 || dtype > SL_DTYPE_FP32)
+    return SL_ERR_INVALID;
+  if (rot > 2 * kRotMaxPairs) return SL_ERR_UNSUPPORTED;
+  const sl_rotary_part none = {};
+  const sl_rotary_part* parts[2] = {q, k ? k : &none};
+  if (q->heads <= 0) return SL_ERR_INVALID;
+  for (const sl_rotary_part* p : parts) {
+    if (p->heads < 0) return SL_ERR_INVALID;
+    if (p->heads == 0) continue;
+    if (p->dim < rot || p->offset < 0 || p->offset > p->dim - rot) return SL_ERR_INVALID;
+    if (T > 0 && (!p->x || !p->y)) return SL_ERR_INVALID;
+    // (the unit index times the units of a head stays below 2^32)
+    if (p->dim > 4096 || static_cast<int64_t>(p->heads) * p->dim >= (1 << 20))
+      return SL_ERR_UNSUPPORTED;
+  }
+  if (T == 0) return SL_OK;
+  if (!positions || !turns) return SL_ERR_INVALID;
+  const int size = dtype == SL_DTYPE_FP32 ? 4 : 2;
+  // the widest unit that divides every size, stride and address
+  auto fits = [&](int v) {
+    if ((interleaved ? rot : rot / 2) % v || (interleaved && v < 2)) return false;
+    for (const sl_rotary_part* p : parts) {
+      if (p->heads == 0) continue;
+      const int64_t all = static_cast<int64_t>(p->dim) | p->offset | p->x_token | p->x_head |
+                          p->y_token | p->y_head;
+      if (all % v || (reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->y)) %
+                         static_cast<uintptr_t>(v * size))
+        return false;
+    }
+    return true;
+  };
+  int v = 16 / size;
+  while (v > 1 && !fits(v)) v >>= 1;
+  // interleaved pairs sit in one unit: a tensor that starts in the middle of
+  // a pair's alignment is refused rather than split
+  if (!fits(v)) return SL_ERR_UNSUPPORTED;
+  RotArgs a = {};
+  a.positions = positions;
+  a.turns = turns;
+  a.factor = factor;
+  a.T = T;
+  a.rot = rot;
+  a.rot_units = (interleaved ? rot : rot / 2) / v;
+  int items = 0;
+  for (int i = 0; i < 2; ++i) {
+    const sl_rotary_part* p = parts[i];
+    RotTensor& t = a.t[i];
+    t.units = 1;
+    t.units_mul = 0;
+    if (p->heads == 0) continue;
+    const bool in_place = p->x == p->y && p->x_token == p->y_token && p->x_head == p->y_head;
+    t.x = p->x;
+    t.y = p->y;
+    t.xs = p->x_token;
+    t.xh = p->x_head;
+    t.ys = p->y_token;
+    t.yh = p->y_head;
+    t.heads = p->heads;
+    t.offset = p->offset;
+    // in place the columns that are not rotated are left alone
+    t.units = a.rot_units + (in_place ? 0 : (p->dim - rot) / v);
+    t.units_mul = t.units == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + t.units - 1) / t.units);
+    items += t.heads * t.units;
+  }
+  // tokens per CTA: about four units per thread, so that the angles' sines
+  // and cosines and the launch are spread over several rows
+  int per = 4 * kRotThreads / items;
+  per = per < 1 ? 1 : (per > 32 ? 32 : per);
+  const int sms = sl_device_sm_count();
+  if (sms <= 0) return SL_ERR_CUDA;
+  while (per > 1 && (T + per - 1) / per < 4 * sms) per >>= 1;
+  a.per_cta = per;
+  const dim3 grid((T + per - 1) / per);
+  const size_t smem = static_cast<size_t>(per) * (rot / 2) * sizeof(float2);
+  if (smem > 48 * 1024) return SL_ERR_UNSUPPORTED;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (dtype == SL_DTYPE_BF16)
+    e = interleaved ? launch_rotary<__nv_bfloat16, true>(a, v, grid, smem, st)
+                    : launch_rotary<__nv_bfloat16, false>(a, v, grid, smem, st);
+  else if (dtype == SL_DTYPE_FP16)
+    e = interleaved ? launch_rotary<__half, true>(a, v, grid, smem, st)
+                    : launch_rotary<__half, false>(a, v, grid, smem, st);
+  else
+    e = interleaved ? launch_rotary<float, true>(a, v, grid, smem, st)
+                    : launch_rotary<float, false>(a, v, grid, smem, st);
+  SL_CUDA_TRY(e);
+  return SL_OK;
+}
