@@ -39,8 +39,7 @@ enum {
   SL_ERR_CUDA = 3,        /* CUDA runtime error */
   SL_ERR_UNSUPPORTED = 4, /* shape / dtype this build does not cover */
   SL_ERR_TIMEOUT = 5,     /* a bounded device wait ran out */
-  SL_ERR_NO_SCRATCH = 6,  /* problem too large for sl_fused_experts_noalloc */
-  SL_ERR_NO_BLOCKS = 7    /* sl_plan_kv_blocks: no free block, or no room in a table row */
+  SL_ERR_NO_SCRATCH = 6   /* problem too large for sl_fused_experts_noalloc */
 };
 
 /* Human-readable text for a status code. */
@@ -488,6 +487,11 @@ int sl_fused_experts_noalloc(const void* hidden, int T, int H, int I,
  * inside vLLM, whose block manager, rotary embedding and prefill attention
  * these stand in for). */
 enum { SL_DTYPE_BF16 = 0, SL_DTYPE_FP16 = 1, SL_DTYPE_FP32 = 2 };
+enum {
+  SL_KV_PLAN_OK = 0,
+  SL_KV_PLAN_NO_BLOCKS = 1, /* the free blocks, or the room in a table row, ran out */
+  SL_KV_PLAN_BAD_INPUT = 2  /* lengths or a free range that cannot be */
+};
 
 /* Block tables and slot maps of a packed batch, from its requests' lengths,
  * with no host round trip. Request r has context_lens[r] cached tokens and
@@ -503,12 +507,13 @@ enum { SL_DTYPE_BF16 = 0, SL_DTYPE_FP16 = 1, SL_DTYPE_FP32 = 2 };
  *                     (Tk = 0: not wanted, may be NULL)
  *   free_range_out    i64 [2]: the range with the taken blocks gone (may be
  *                     free_range itself)
- *   status            i32 [2]: status, blocks taken
+ *   status            i32 [2]: SL_KV_PLAN_*, blocks taken
  * Rows behind the last request get position and slot -1. A request whose
  * blocks the ring or its table row cannot hold takes none: its new tokens
  * get slot -1, its table row stays as it was, and status becomes
- * SL_ERR_NO_BLOCKS. Negative lengths count as 0, and more tokens than T or Tk
- * are cut off (cu_new and cu_total stay within T and Tk): SL_ERR_INVALID.
+ * SL_KV_PLAN_NO_BLOCKS. Negative lengths count as 0, and more tokens than T
+ * or Tk are cut off (cu_new and cu_total stay within T and Tk):
+ * SL_KV_PLAN_BAD_INPUT.
  * B in [1, 8192]. */
 int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new_lens, int B,
                       int block_size, int32_t* block_table, int64_t ld_table, int table_width,

@@ -23,7 +23,6 @@ SL_ERR_CUDA = 3
 SL_ERR_UNSUPPORTED = 4
 SL_ERR_TIMEOUT = 5
 SL_ERR_NO_SCRATCH = 6
-SL_ERR_NO_BLOCKS = 7
 
 SEG_FREE, SEG_PROBATION, SEG_PROTECTED, SEG_PINNED = 0, 1, 2, 3
 PLAN_FAST_HIT = 1
@@ -51,6 +50,7 @@ _i64 = _c.c_int64
 
 WEIGHTS_BF16, WEIGHTS_FP8_BLOCK128 = 0, 1
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
+KV_PLAN_OK, KV_PLAN_NO_BLOCKS, KV_PLAN_BAD_INPUT = 0, 1, 2
 
 
 class ExpertWeights(ctypes.Structure):
@@ -181,8 +181,7 @@ def status_text(status: int) -> str:
     except Exception:  # library not loadable: plain text
         return {0: "ok", 1: "overflow", 2: "invalid argument", 3: "CUDA error",
                 4: "unsupported", 5: "timeout",
-                6: "problem too large for the no-alloc scratch",
-                7: "no free cache blocks"}.get(int(status), "unknown")
+                6: "problem too large for the no-alloc scratch"}.get(int(status), "unknown")
 
 
 def check(rc: int, what: str) -> None:

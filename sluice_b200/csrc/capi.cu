@@ -21,8 +21,6 @@ extern "C" const char* sl_status_string(int status) {
     case SL_ERR_NO_SCRATCH:
       return "problem needs more than the 32 MiB static scratch of sl_fused_experts_noalloc; "
              "use sl_fused_experts with a caller workspace";
-    case SL_ERR_NO_BLOCKS:
-      return "the free cache blocks, or the room in a block table row, ran out";
     default: return "unknown status";
   }
 }

@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
       a.cu_total[r] = min(cu_total[r], cap_k);
     }
     if (tid == 0) {
-      a.status[0] = s_invalid || bad_range || over ? SL_ERR_INVALID
-                    : s_short                      ? SL_ERR_NO_BLOCKS
-                                                   : SL_OK;
+      a.status[0] = s_invalid || bad_range || over ? SL_KV_PLAN_BAD_INPUT
+                    : s_short                      ? SL_KV_PLAN_NO_BLOCKS
+                                                   : SL_KV_PLAN_OK;
       a.status[1] = s_end;
       if (a.write_range) {
         const int64_t first = a.range[0], tail = a.range[1];

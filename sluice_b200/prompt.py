@@ -50,6 +50,17 @@ def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, length: int | None =
 
 
 # ------------------------------------------------------------ block planner
+class KvPlanError(_lib.SluiceError):
+    """The device found that a plan could not be made in full."""
+
+    def __init__(self, status: int):
+        RuntimeError.__init__(self, "plan_kv_blocks: " + (
+            "the free cache blocks, or the room in a block table row, ran out"
+            if status == _lib.KV_PLAN_NO_BLOCKS else
+            "lengths, token counts or a free range that cannot be"))
+        self.status = status
+
+
 class KvPlan(NamedTuple):
     """A packed batch, as ``plan_kv_blocks`` lays it out."""
 
@@ -58,12 +69,14 @@ class KvPlan(NamedTuple):
     positions: torch.Tensor         # int64 [num_tokens] position in its sequence
     slots: torch.Tensor             # int64 [num_tokens] cache row, -1: none
     kv_slots: torch.Tensor | None   # int64 [num_kv_tokens] cache rows of all tokens
-    status: torch.Tensor            # int32 [2] status, blocks taken
+    status: torch.Tensor            # int32 [2] KV_PLAN_*, blocks taken
 
     def check(self) -> None:
-        """Raise if the plan ran out of blocks or was given bad lengths
-        (synchronises)."""
-        check(int(self.status[0].item()), "plan_kv_blocks")
+        """Raise ``KvPlanError`` if the plan ran out of blocks or was given
+        bad lengths (synchronises)."""
+        status = int(self.status[0].item())
+        if status != _lib.KV_PLAN_OK:
+            raise KvPlanError(status)
 
 
 def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,

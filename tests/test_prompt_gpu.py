@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import prompt as oprompt
-from sluice_b200 import SluiceError, ops, prompt
+from sluice_b200 import _lib, ops, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -95,11 +95,11 @@ def test_plan_without_blocks_left():
     for in_place in (True, False):
         p, ref = _check_plan([0, 10, 15, 3, 16], [33, 6, 2, 2, 40], 16, extra=-3,
                              in_place=in_place)
-        assert ref[7] and p.status[0].item() == 7
-        with pytest.raises(SluiceError, match="free cache blocks"):
+        assert ref[7] and p.status[0].item() == _lib.KV_PLAN_NO_BLOCKS
+        with pytest.raises(prompt.KvPlanError, match="free cache blocks"):
             p.check()
     p, ref = _check_plan([0, 10, 40], [90, 6, 20], 16, width_extra=-2)
-    assert ref[7] and p.status[0].item() == 7
+    assert ref[7] and p.status[0].item() == _lib.KV_PLAN_NO_BLOCKS
 
 
 def test_plan_survives_bad_lengths_and_ranges():
@@ -108,18 +108,18 @@ def test_plan_survives_bad_lengths_and_ranges():
     table, ring, head, tail = _plan_case([0, 0], [20, 20], 16)
     guard = 64
     p, _, _ = _run_plan([-5, 0], [20, -1], table, ring, head, tail, 16, 20, 0)
-    assert p.status[0].item() == 2 and p.cu_new.tolist() == [0, 20, 20]
+    assert p.status[0].item() == _lib.KV_PLAN_BAD_INPUT and p.cu_new.tolist() == [0, 20, 20]
     p, _, _ = _run_plan([0, 0], [20, 20], table, ring, head, tail, 16, 30, 30)
-    assert p.status[0].item() == 2
+    assert p.status[0].item() == _lib.KV_PLAN_BAD_INPUT
     assert p.cu_new.tolist() == [0, 20, 30] and p.cu_total.tolist() == [0, 20, 30]
     width = len(table[0])
     p, _, _ = _run_plan([width * 16 + 1, 0], [1, 20], table, ring, head, tail, 16, 21, 0)
-    assert p.status[0].item() == 2 and p.slots[0].item() == -1 and p.slots[1].item() >= 0
+    assert p.status[0].item() == _lib.KV_PLAN_BAD_INPUT and p.slots[0].item() == -1 and p.slots[1].item() >= 0
     p, _, out = _run_plan([0, 0], [20, 20], table, ring, 0, len(ring) + 1, 16, 40, 0)
-    assert p.status[0].item() == 2 and p.slots.eq(-1).all() and out.tolist() == [0, len(ring) + 1]
+    assert p.status[0].item() == _lib.KV_PLAN_BAD_INPUT and p.slots.eq(-1).all() and out.tolist() == [0, len(ring) + 1]
     p, _, _ = _run_plan([2 ** 31 - 1, 2 ** 31 - 1], [2 ** 31 - 1, 5], table, ring, head, tail, 16,
                         guard, guard)
-    assert p.status[0].item() == 2 and p.slots.eq(-1).all() and p.cu_total.max().item() <= guard
+    assert p.status[0].item() == _lib.KV_PLAN_BAD_INPUT and p.slots.eq(-1).all() and p.cu_total.max().item() <= guard
 
 
 def test_plan_replays_in_a_graph_and_moves_its_range():
