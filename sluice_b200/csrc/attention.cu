@@ -1,110 +1,991 @@
-// Causal attention over packed sequences with grouped heads.
+// Causal attention over packed sequences with grouped heads, on the fifth
+// generation tensor cores.
+//
+//   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i . k_j - m_i),
+//   j <= i + keys - queries
+//
+// One pass over the keys with a running maximum m and sum (the sum of the
+// rounded-off weights is never formed again). An item is 2 x 128 rows of one
+// sequence and key head; its rows are (token, head of the group) pairs, so a
+// single token of a wide group fills rows that would otherwise be empty, and
+// a key tile is read once for all heads of its group. Per item and 128-key
+// tile: S = Q K^T (128 x 128 per 128 rows, fp32, in TMEM), the softmax
+// warpgroup of those rows reads a row per thread, writes the weights P over S
+// in the inputs' type, and O += P V takes P from TMEM. The two halves of an
+// item run half a step apart: while one half's weights are formed the tensor
+// core works for the other.
+//
+// Roles (12 warps): 0-3 and 4-7 softmax of the two halves (a row per thread)
+// and their output; 8 issues the MMAs; 9 the tile loads (TMA); 10, 11 clean
+// the value tiles that hold keys which some row may not see.
+//
+// Shared memory: the item's queries (2 x 128 rows) and a ring of 16 KB slots
+// that the key and value tiles pass through: 64 columns of 128 keys, or 64
+// values rows of 128 columns.
 #include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
 
 #include "common.cuh"
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 384;
+constexpr int kTile = 128;           // rows of a half and keys of a tile
+constexpr int kSlotBytes = 16384;
+constexpr int kCoarse = 256;         // entries of the work table
+constexpr int kMaxSlots = 12;
+constexpr float kLag = 8.f;          // how far (in powers of 2) the maximum may lag behind
+constexpr int kMarks = 16;           // items that the value guards may be ahead by
 
-template <typename E>
-__device__ __forceinline__ float val(E v);
-template <>
-__device__ __forceinline__ float val(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float val(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename E>
-__device__ __forceinline__ E rounded(float v);
-template <>
-__device__ __forceinline__ __half rounded(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 rounded(float v) { return __float2bfloat16_rn(v); }
+struct Params {
+  CUtensorMap q, k, v, ks;
+  void* out;
+  int64_t out_token, out_head;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const void* vraw;                  // values, for the rare repair of a column
+  int64_t v_token, v_head;
+  int B, Tq, Tk, heads, kv_heads, group, half_tokens;  // tokens of a half: 128 / group
+  int shared;                        // the last 64 key columns come from ks
+  int grid;                          // CTAs
+  int split;                         // 1: equal shares of all key tiles per CTA
+  int rows_cap;                      // rows of a partial result
+  float scale_log2;                  // scale / ln 2
+  float* part;                       // [2 * grid][rows_cap][v_dim]
+  float2* part_ml;                   // [2 * grid][rows_cap] (maximum, sum)
+  int32_t* status;
+};
 
-// A warp per (query, head): 32 keys at a time, a lane each for the scores,
-// then the lanes share out the value columns. The running maximum and sum of
-// the softmax make one pass over the keys.
-template <typename E, int kDim, int kVDim>
-__global__ void __launch_bounds__(kThreads) attention_simple_kernel(sl_attention_args a,
-                                                                    int32_t* status) {
-  __shared__ float q_sm[kThreads / 32][kDim];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  sl::pdl_wait();
-  sl::pdl_trigger();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = SL_OK;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp;
-  if (item >= a.Tq * a.heads) return;
-  const int64_t row = item / a.heads;
-  const int h = static_cast<int>(item % a.heads), hk = h / (a.heads / a.kv_heads);
-  // the sequence: the last one that begins at or before the row
-  int lo = 0, hi = a.B;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu_q[mid] <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  if (lo >= a.B || row < a.cu_q[0]) return;
-  const int64_t q0 = a.cu_q[lo], q1 = a.cu_q[lo + 1];
-  const int64_t k0 = max(a.cu_k[lo], 0), k1 = min(static_cast<int64_t>(a.cu_k[lo + 1]), a.Tk);
-  const int64_t seen = min(max(k1 - k0, static_cast<int64_t>(0)), row - q0 + 1 + (k1 - k0) - (q1 - q0));
-  const E* q = static_cast<const E*>(a.q) + row * a.q_token + h * a.q_head;
-  for (int d = lane; d < kDim; d += 32) q_sm[warp][d] = val(q[d]);
-  __syncwarp();
-  const int own = kDim - a.shared_dim;
-  float m = -INFINITY, l = 0.f, o[kVDim / 32] = {};
-  for (int64_t j0 = 0; j0 < seen; j0 += 32) {
-    const int64_t j = j0 + lane;
-    float s = -INFINITY;
-    if (j < seen) {
-      const E* k = static_cast<const E*>(a.k) + (k0 + j) * a.k_token + hk * a.k_head;
-      s = 0.f;
-      for (int d = 0; d < own; ++d) s = fmaf(q_sm[warp][d], val(k[d]), s);
-      if (a.shared_dim) {
-        const E* ks = static_cast<const E*>(a.k_shared) + (k0 + j) * a.k_shared_token;
-        for (int d = own; d < kDim; ++d) s = fmaf(q_sm[warp][d], val(ks[d - own]), s);
-      }
-      s *= a.scale;
-    }
-    float top = s;
+// ------------------------------------------------------------------ helpers
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(sl::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sl::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// D (+)= A B, A from TMEM (the weights), B from shared memory.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Shared-memory descriptor of an operand whose rows are the reduction index
+// (values: a row per key, 128-byte swizzled rows of 64 columns): 8-row groups
+// 1024 bytes apart, the next 64 columns `lbo` bytes on.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t lbo) {
+  uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int N, bool b_rows) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_rows ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_fence_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float m1 = fmaxf(m, top);
-    // (a row whose scores are all -inf so far keeps zero weights)
-    const float base = m1 == -INFINITY ? 0.f : m1;
-    const float corr = __expf(m - base), p = __expf(s - base);
-    float sum = p;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * corr + sum;
-    m = m1;
-#pragma unroll
-    for (int c = 0; c < kVDim / 32; ++c) o[c] *= corr;
-    const int n = static_cast<int>(min(static_cast<int64_t>(32), seen - j0));
-    for (int u = 0; u < n; ++u) {
-      const float pu = __shfl_sync(0xffffffffu, p, u);
-      const E* v = static_cast<const E*>(a.v) + (k0 + j0 + u) * a.v_token + hk * a.v_head;
-#pragma unroll
-      for (int c = 0; c < kVDim / 32; ++c) o[c] = fmaf(pu, val(v[lane + 32 * c]), o[c]);
-    }
-  }
-  E* out = static_cast<E*>(a.out) + row * a.out_token + h * a.out_head;
-#pragma unroll
-  for (int c = 0; c < kVDim / 32; ++c)
-    out[lane + 32 * c] = rounded<E>(seen > 0 ? o[c] / l : 0.f);
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// the largest of three; NaN if any is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t d;
+  if constexpr (kBf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
 }
 
-template <typename E>
-int run(const sl_attention_args& a, int32_t* status, cudaStream_t st) {
-  const int64_t ctas = (a.Tq * a.heads + kThreads / 32 - 1) / (kThreads / 32);
-  if (ctas > 0x7fffffff) return SL_ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(ctas));
-  cudaError_t e;
-  if (a.dim == 64)
-    e = sl::launch(attention_simple_kernel<E, 64, 64>, grid, dim3(kThreads), 0, st, a, status);
-  else if (a.dim == 128)
-    e = sl::launch(attention_simple_kernel<E, 128, 128>, grid, dim3(kThreads), 0, st, a, status);
-  else
-    e = sl::launch(attention_simple_kernel<E, 192, 128>, grid, dim3(kThreads), 0, st, a, status);
-  SL_CUDA_TRY(e);
+// A bounded wait whose outcome all lanes of the warp agree on.
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, sl::mbar_wait(bar, parity));
+}
+
+// --------------------------------------------------------------------- work
+// One stretch of an item's key tiles: [j0, j1) of n.
+struct Seg {
+  int seq, tile, head;
+  int q0, q_len, k0, k_len;   // the sequence's rows, clamped to the tensors
+  int tok;                    // first token of the item
+  int n, j0, j1;              // key tiles of the item, and this stretch
+  int nh[2];                  // key tiles that each half's last row reaches
+  int lim0;                   // keys that the item's first row sees
+};
+
+struct Seq {
+  int q0, q_len, k0, k_len;
+};
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return max(lo, min(v, hi)); }
+
+__device__ __forceinline__ Seq load_seq(const Params& p, int s) {
+  Seq r;
+  r.q0 = clampi(p.cu_q[s], 0, p.Tq);
+  r.q_len = clampi(p.cu_q[s + 1], r.q0, p.Tq) - r.q0;
+  r.k0 = clampi(p.cu_k[s], 0, p.Tk);
+  r.k_len = clampi(p.cu_k[s + 1], r.k0, p.Tk) - r.k0;
+  return r;
+}
+// keys that token `tok` of a sequence sees
+__device__ __forceinline__ int seen(const Seq& s, int tok) {
+  return clampi(tok + 1 + s.k_len - s.q_len, 0, s.k_len);
+}
+__device__ __forceinline__ int tiles_of(const Params& p, const Seq& s) {
+  return (s.q_len + 2 * p.half_tokens - 1) / (2 * p.half_tokens);
+}
+// key tiles of item `t` (at least one unit of work, to write its rows)
+__device__ __forceinline__ int reach(const Params& p, const Seq& s, int t) {
+  const int last = min(s.q_len, (t + 1) * 2 * p.half_tokens) - 1;
+  return (seen(s, last) + kTile - 1) / kTile;
+}
+__device__ __forceinline__ int64_t work_of(const Params& p, const Seq& s) {
+  const int nt = tiles_of(p, s);
+  if (!p.split) return nt;
+  int64_t w = 0;
+  for (int t = 0; t < nt; ++t) w += max(1, reach(p, s, t));
+  return w;
+}
+
+// cum[i]: work of the sequences before the i-th run of `per` ones (in items,
+// or in key tiles where items are split); all threads take part.
+__device__ __forceinline__ void build_table(const Params& p, int* cum, int* warp_sum, int per) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t w = 0;
+  if (tid < kCoarse)
+    for (int s = tid * per; s < min(p.B, (tid + 1) * per); ++s) w += work_of(p, load_seq(p, s));
+  int v = static_cast<int>(min(w, static_cast<int64_t>(1 << 22)));
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (tid < kCoarse && lane == 31) warp_sum[warp] = v;
+  __syncthreads();
+  if (tid < kCoarse) {
+    for (int i = 0; i < warp; ++i) v += warp_sum[i];
+    cum[tid + 1] = v;
+    if (tid == 0) cum[0] = 0;
+  }
+  __syncthreads();
+}
+
+// The sequence that unit u falls in, and u's place in it (warp-uniform).
+__device__ __forceinline__ Seq find_seq(const Params& p, const int* cum, int per, int u, int& seq,
+                                        int& rest) {
+  const int lane = threadIdx.x & 31;
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < kCoarse / 32; ++i) c += cum[lane * (kCoarse / 32) + i + 1] <= u;
+  const int run = __reduce_add_sync(0xffffffffu, c);
+  rest = u - cum[run];
+  const int end = min(p.B, (run + 1) * per);
+  seq = run * per;
+  if (per > 1) {
+    for (int s0 = seq;; s0 += 32) {
+      const int s = s0 + lane;
+      const int own = s < end ? static_cast<int>(work_of(p, load_seq(p, s))) : 0;
+      int v = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, v > rest);
+      if (hit || s0 + 32 >= end) {
+        const int l = hit ? __ffs(hit) - 1 : 0;
+        seq = s0 + l;
+        rest -= __shfl_sync(0xffffffffu, v - own, l);
+        break;
+      }
+      rest -= __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  return load_seq(p, seq);
+}
+
+__device__ __forceinline__ void fill_seg(const Params& p, const Seq& s, Seg& g) {
+  g.q0 = s.q0;
+  g.q_len = s.q_len;
+  g.k0 = s.k0;
+  g.k_len = s.k_len;
+  g.tok = g.tile * 2 * p.half_tokens;
+  g.lim0 = seen(s, g.tok);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int first = g.tok + h * p.half_tokens;
+    const int last = min(s.q_len, first + p.half_tokens) - 1;
+    g.nh[h] = first < s.q_len ? (seen(s, last) + kTile - 1) / kTile : 0;
+  }
+  g.n = max(g.nh[0], g.nh[1]);
+}
+
+// Walks a CTA's share of the work. Every role's warp walks it by itself.
+//   whole items: the longest first, dealt out in turns that go back and forth;
+//   split: an equal run of key tiles, item after item.
+struct Walk {
+  int total, at, end, round;
+
+  __device__ void start(const Params& p, const int* cum) {
+    total = units(p, cum);
+    round = 0;
+    if (p.split) {
+      at = share(p, total, blockIdx.x);
+      end = share(p, total, blockIdx.x + 1);
+    }
+  }
+  __device__ static int units(const Params& p, const int* cum) {
+    return static_cast<int>(min(static_cast<int64_t>(cum[kCoarse]) * p.kv_heads,
+                                static_cast<int64_t>(1 << 30)));
+  }
+  __device__ static int share(const Params& p, int total, int c) {
+    return static_cast<int>(static_cast<int64_t>(total) * c / p.grid);
+  }
+  __device__ bool next(const Params& p, const int* cum, int per, Seg& g) {
+    if (!p.split) {
+      const int G = p.grid;
+      const int c = blockIdx.x;
+      const int i = round * G + ((round & 1) ? G - 1 - c : c);
+      if (i >= total) return false;
+      ++round;
+      g.head = i % p.kv_heads;
+      int rest;
+      const Seq s = find_seq(p, cum, per, i / p.kv_heads, g.seq, rest);
+      g.tile = tiles_of(p, s) - 1 - rest;
+      fill_seg(p, s, g);
+      g.j0 = 0;
+      g.j1 = g.n;
+      return true;
+    }
+    if (at >= end) return false;
+    int j, n;
+    locate(p, cum, per, at, g, j, n);
+    g.j0 = j;
+    g.j1 = min(n, j + end - at);
+    at += g.j1 - j;
+    g.j1 = min(g.j1, g.n);  // (an item without keys is one empty unit)
+    return true;
+  }
+  // The item that unit u falls in: u is its key tile j of n units.
+  __device__ static void locate(const Params& p, const int* cum, int per, int u, Seg& g, int& j,
+                                int& n) {
+    const int lane = threadIdx.x & 31;
+    // units of a sequence count all heads: tile after tile, head after head
+    int rest;
+    const Seq s = find_seq(p, cum, per, u / p.kv_heads, g.seq, rest);
+    int r = rest * p.kv_heads + u % p.kv_heads;
+    const int nt = tiles_of(p, s);
+    for (int t0 = 0;; t0 += 32) {
+      const int t = t0 + lane;
+      const int own = t < nt ? max(1, reach(p, s, t)) * p.kv_heads : 0;
+      int v = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, v > r);
+      if (hit || t0 + 32 >= nt) {
+        const int l = hit ? __ffs(hit) - 1 : 0;
+        g.tile = t0 + l;
+        r -= __shfl_sync(0xffffffffu, v - own, l);
+        break;
+      }
+      r -= __shfl_sync(0xffffffffu, v, 31);
+    }
+    fill_seg(p, s, g);
+    n = max(1, g.n);
+    g.head = min(r / n, p.kv_heads - 1);
+    j = r - r / n * n;
+  }
+};
+
+// ------------------------------------------------------------------- kernel
+template <int kDim, int kVDim>
+struct Cfg {
+  static constexpr int kChunks = kDim / 64;                  // 64-column slots of a key tile
+  static constexpr int kVSlots = kVDim / 64;                 // slots of a value tile
+  static constexpr int kVRows = kTile / kVSlots;             // keys of a value slot
+  static constexpr int kQBytes = 2 * kChunks * kSlotBytes;
+  static constexpr int kSlots = (14 * kSlotBytes - kQBytes) / kSlotBytes;  // 8, 10, 12
+  static constexpr int kBufBytes = kQBytes + kSlots * kSlotBytes;          // 224 KB
+};
+
+struct Sync {
+  uint64_t full[kMaxSlots], empty[kMaxSlots], clean[kMaxSlots];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], o_free[2], drain;
+  uint32_t tmem;
+  int mark[kMarks];
+  int warp_sum[kCoarse / 32];
+  int cum[kCoarse + 1];
+};
+constexpr int kSmemBytes = 14 * kSlotBytes + 1024 + static_cast<int>(sizeof(Sync));
+static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+
+// A place in the ring and the parity of its current use.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  template <int N>
+  __device__ __forceinline__ void step() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+template <int kDim, int kVDim, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(
+    const __grid_constant__ Params p) {
+  using C = Cfg<kDim, kVDim>;
+  extern __shared__ uint8_t sm_raw[];
+  uint8_t* buf = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = buf + C::kQBytes;
+  Sync& sy = *reinterpret_cast<Sync*>(buf + C::kBufBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.B + kCoarse - 1) / kCoarse;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      sl::mbar_init(&sy.full[i], 1);
+      sl::mbar_init(&sy.empty[i], 1);
+      sl::mbar_init(&sy.clean[i], 2);
+    }
+    for (int h = 0; h < 2; ++h) {
+      sl::mbar_init(&sy.q_full[h], 1);
+      sl::mbar_init(&sy.q_empty[h], 1);
+      sl::mbar_init(&sy.s_full[h], 1);
+      sl::mbar_init(&sy.p_full[h], 4);
+      sl::mbar_init(&sy.pv_done[h], 1);
+      sl::mbar_init(&sy.o_free[h], 4);
+    }
+    sl::mbar_init(&sy.drain, 1);
+    for (int i = 0; i < kMarks; ++i) sy.mark[i] = -1;
+    sl::fence_barrier_init();
+  }
+  if (warp == 8) sl::tmem_alloc(&sy.tmem, 512);
+  if (tid == kThreads - 1) {
+    sl::tma_prefetch_desc(&p.q);
+    sl::tma_prefetch_desc(&p.k);
+    sl::tma_prefetch_desc(&p.v);
+  }
+  sl::pdl_wait();
+  sl::pdl_trigger();
+  if (blockIdx.x == 0 && tid == 0) *p.status = SL_OK;
+  build_table(p, sy.cum, sy.warp_sum, per);  // (its barriers publish the set-up above)
+  sl::tc_fence_before();
+  __syncthreads();
+  sl::tc_fence_after();
+  const uint32_t tmem = sy.tmem;
+  const uint32_t s_col[2] = {tmem, tmem + kTile};
+  const uint32_t o_col[2] = {tmem + 2 * kTile, tmem + 2 * kTile + kVDim};
+  bool ok = true;
+  Walk walk;
+  walk.start(p, sy.cum);
+  Seg g;
+
+  if (warp < 8) {
+    // ---------------------------------------------------------- softmax
+    const int h = warp >> 2;
+    const int row = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // (warp mod 4) * 32 lanes
+    const uint32_t s_at = s_col[h] + lanes, o_at = o_col[h] + lanes;
+    const int token = row / p.group, in_group = row - token * p.group;
+    const bool packed = token < p.half_tokens;
+    int n_s = 0, n_item = 0;  // key tiles so far; items with keys so far
+    while (ok && walk.next(p, sy.cum, per, g)) {
+      const int first = g.tok + h * p.half_tokens;
+      const int j1 = min(g.j1, g.nh[h]);
+      const bool has = g.j0 < g.j1;
+      const int mark = has ? n_item++ : -1;
+      if (first >= g.q_len) continue;
+      const int tok = first + token;
+      const bool live = packed && tok < g.q_len;
+      const int lim = live ? clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len) : 0;
+      const int lim_first = clampi(first + 1 + g.k_len - g.q_len, 0, g.k_len);
+      float m = -INFINITY, l = 0.f;
+      for (int j = g.j0; j < j1; ++j) {
+        if (!(ok = wait_all(&sy.s_full[h], n_s & 1))) break;
+        sl::tc_fence_after();
+        uint32_t r[kTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
+        if ((j + 1) * kTile > lim_first) {
+          const int left = lim - j * kTile;
+#pragma unroll
+          for (int c = 0; c < kTile; ++c)
+            if (c >= left) r[c] = 0xff800000u;  // -inf
+        }
+        auto s = [&](int c) { return __uint_as_float(r[c]); };
+        float top = max3(s(0), s(1), s(2)), top2 = max3(s(3), s(4), s(5));
+#pragma unroll
+        for (int c = 6; c < kTile - 2; c += 4) {
+          top = max3(top, s(c), s(c + 1));
+          top2 = max3(top2, s(c + 2), s(c + 3));
+        }
+        top = max3(top, s(kTile - 2), s(kTile - 1));
+        top = max2(top, top2);
+        // a score of +inf leaves no finite weights: the row is NaN, as
+        // inf - inf makes it
+        if (top == INFINITY) top = __int_as_float(0x7fffffff);
+        const float m1 = max2(m, top);
+        // the maximum may lag behind by a factor 2^kLag: the weights stay
+        // far inside the type's range, and the sums and outputs are rescaled
+        // only where it grows by more (also on NaN, and on the first tile)
+        const bool move = live && !((m1 - m) * p.scale_log2 <= kLag) && !(m1 == -INFINITY);
+        if (__any_sync(0xffffffffu, move)) {
+          const float corr = m1 == -INFINITY ? 1.f : ex2((m - m1) * p.scale_log2);
+          m = m1;
+          l *= corr;
+          if (j > g.j0) {
+            // the sums so far, once the products before this tile are in
+            if (!(ok = wait_all(&sy.pv_done[h], (n_s - 1) & 1))) break;
+            sl::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kVDim / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_at + 32 * c, o);
+              tmem_fence_ld(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st32(o_at + 32 * c, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+        float2 sum = make_float2(0.f, 0.f);
+        const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
+#pragma unroll
+        for (int c = 0; c < kTile / 2; ++c) {
+          float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
+          x.x = ex2(x.x);
+          x.y = ex2(x.y);
+          sum = __fadd2_rn(sum, x);
+          r[c] = pack2<kBf16>(x.x, x.y);
+        }
+        l += sum.x + sum.y;
+        tmem_st32(s_at, r);
+        tmem_st32(s_at + 32, r + 32);
+        tmem_wait_st();
+        sl::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sl::mbar_arrive(&sy.p_full[h]);
+        ++n_s;
+      }
+      if (!ok) break;
+      // ------------------------------------------------------- output
+      const bool whole = g.j0 == 0 && g.j1 == g.n;
+      const int out_row = g.q0 + tok, out_head = g.head * p.group + in_group;
+      const int prow = h * p.half_tokens * p.group + row;
+      const int pslot = 2 * blockIdx.x + (g.j0 > 0 ? 0 : 1);
+      float* part = p.part + (static_cast<int64_t>(pslot) * p.rows_cap + prow) * kVDim;
+      if (!whole && live) p.part_ml[static_cast<int64_t>(pslot) * p.rows_cap + prow] =
+          make_float2(m, l);
+      const bool ran = g.j0 < j1;
+      if (ran) {
+        if (!(ok = wait_all(&sy.pv_done[h], (n_s - 1) & 1))) break;
+        sl::tc_fence_after();
+      }
+      const bool repair = has && sy.mark[mark % kMarks] == mark;
+      // no key seen: zeros; only keys that score -inf: 0 / 0
+      const float inv = lim == 0 ? 0.f : 1.f / l;
+      uint16_t* dst = static_cast<uint16_t*>(p.out) +
+          static_cast<int64_t>(out_row) * p.out_token + static_cast<int64_t>(out_head) * p.out_head;
+#pragma unroll
+      for (int c = 0; c < kVDim / 32; ++c) {
+        uint32_t o[32];
+        if (ran) {
+          tmem_ld32(o_at + 32 * c, o);
+          tmem_fence_ld(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (repair && live) {
+          // values that are not finite were taken out of the tiles that not
+          // all rows see; a row that does see one gets it back: its weight
+          // is positive, so only its sign and kind count
+          const int ja = max(g.lim0, g.j0 * kTile), jb = min(lim, g.j1 * kTile);
+          for (int j = ja; j < jb; ++j) {
+            const uint16_t* v = static_cast<const uint16_t*>(p.vraw) +
+                static_cast<int64_t>(g.k0 + j) * p.v_token + static_cast<int64_t>(g.head) * p.v_head +
+                32 * c;
+            constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const uint32_t b = v[i];
+              if ((b & kExp) == kExp) {
+                const bool nan = b & (kExp == 0x7f80u ? 0x7fu : 0x3ffu);
+                const float bad = nan ? __int_as_float(0x7fffffff)
+                                      : (b & 0x8000u) ? -INFINITY : INFINITY;
+                o[i] = __float_as_uint(__uint_as_float(o[i]) + bad);
+              }
+            }
+          }
+        }
+        if (live && whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 w;
+            uint32_t* e = &w.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              e[k] = pack2<kBf16>(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                  __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = w;
+          }
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(part + 32 * c + 4 * i) =
+                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        __syncwarp();
+      }
+      if (ran) {
+        sl::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sl::mbar_arrive(&sy.o_free[h]);
+      }
+    }
+  } else if (warp == 8) {
+    // -------------------------------------------------------------- MMA
+    constexpr uint32_t idesc_s = idesc_f16(kBf16, kTile, false);
+    constexpr uint32_t idesc_o = idesc_f16(kBf16, kVDim, true);
+    const uint32_t q_sm = sl::smem_u32(buf), ring_sm = sl::smem_u32(ring);
+    Ring kv;                       // next slot to take up
+    int n_s[2] = {0, 0}, n_o[2] = {0, 0}, n_q[2] = {0, 0};
+    uint32_t clean_phase = 0;
+    while (ok && walk.next(p, sy.cum, per, g)) {
+      if (g.j0 >= g.j1) continue;
+      const int j1[2] = {min(g.j1, g.nh[0]), min(g.j1, g.nh[1])};
+      int k_slot[C::kChunks], v_slot[C::kVSlots];
+      // S of one half against the key tile in k_slot
+      auto scores = [&](int h) {
+        if (sl::elect_one()) {
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              sl::umma_bf16(s_col[h],
+                            sl::umma_desc_sw128(q_sm + (h * C::kChunks + c) * kSlotBytes + 32 * k),
+                            sl::umma_desc_sw128(ring_sm + k_slot[c] * kSlotBytes + 32 * k),
+                            idesc_s, c + k > 0);
+          sl::umma_commit(&sy.s_full[h]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](const int* slot, int n) {
+        if (sl::elect_one())
+          for (int i = 0; i < n; ++i) sl::umma_commit(&sy.empty[slot[i]]);
+        __syncwarp();
+      };
+      auto take = [&](int* slot, int n) {
+        for (int i = 0; i < n && ok; ++i) {
+          slot[i] = kv.slot;
+          ok = wait_all(&sy.full[kv.slot], kv.phase);
+          kv.step<C::kSlots>();
+        }
+        sl::tc_fence_after();
+      };
+      take(k_slot, C::kChunks);
+      for (int h = 0; h < 2 && ok; ++h) {
+        if (g.j0 >= j1[h]) continue;
+        if (!(ok = wait_all(&sy.q_full[h], n_q[h] & 1))) break;
+        ++n_q[h];
+        scores(h);
+      }
+      if (!ok) break;
+      release(k_slot, C::kChunks);
+      for (int j = g.j0; j < g.j1 && ok; ++j) {
+        take(v_slot, C::kVSlots);
+        if (!ok) break;
+        if ((j + 1) * kTile > g.lim0) {
+          // cleaned by the guards first
+#pragma unroll
+          for (int i = 0; i < C::kVSlots; ++i) {
+            if (!ok) break;
+            ok = wait_all(&sy.clean[v_slot[i]], (clean_phase >> v_slot[i]) & 1);
+            clean_phase ^= 1u << v_slot[i];
+          }
+          if (!ok) break;
+        }
+        bool next_key = false;
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (j >= j1[h]) continue;
+          if (j == g.j0 && n_o[h] > 0 &&
+              !(ok = wait_all(&sy.o_free[h], (n_o[h] - 1) & 1)))
+            break;
+          if (!(ok = wait_all(&sy.p_full[h], n_s[h] & 1))) break;
+          ++n_s[h];
+          sl::tc_fence_after();
+          if (sl::elect_one()) {
+#pragma unroll
+            for (int i = 0; i < C::kVSlots; ++i)
+#pragma unroll
+              for (int k = 0; k < C::kVRows / 16; ++k)
+                umma_ts(o_col[h], s_col[h] + (i * (C::kVRows / 16) + k) * 8,
+                        desc_rows(ring_sm + v_slot[i] * kSlotBytes + 2048 * k, C::kVRows * 128),
+                        idesc_o, j > g.j0 || i + k > 0);
+            sl::umma_commit(&sy.pv_done[h]);
+          }
+          __syncwarp();
+          if (j + 1 < j1[h]) {
+            if (!next_key) {
+              take(k_slot, C::kChunks);
+              next_key = true;
+              if (!ok) break;
+            }
+            scores(h);
+          }
+        }
+        if (!ok) break;
+        release(v_slot, C::kVSlots);
+        // (a half may end earlier: the key tile is taken up by the other)
+        if (next_key) release(k_slot, C::kChunks);
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (g.j0 < j1[h]) {
+          ++n_o[h];
+          if (sl::elect_one()) sl::umma_commit(&sy.q_empty[h]);
+          __syncwarp();
+        }
+    }
+    // everything issued is in before TMEM and the barriers go
+    if (sl::elect_one()) sl::umma_commit(&sy.drain);
+    __syncwarp();
+    ok = wait_all(&sy.drain, 0) && ok;
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ loads
+    Ring kv;
+    int n_q[2] = {0, 0}, turns = 0;
+    const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.half_tokens) * 128;
+    while (ok && walk.next(p, sy.cum, per, g)) {
+      if (g.j0 >= g.j1) continue;
+      const int j1[2] = {min(g.j1, g.nh[0]), min(g.j1, g.nh[1])};
+      auto claim = [&](uint32_t bytes) -> bool {
+        if (turns > 0 && !wait_all(&sy.empty[kv.slot], kv.phase ^ 1)) return false;
+        if (lane == 0) sl::mbar_arrive_expect_tx(&sy.full[kv.slot], bytes);
+        return true;
+      };
+      auto advance = [&]() {
+        kv.step<C::kSlots>();
+        if (kv.slot == 0) turns = 1;
+      };
+      auto load_q = [&](int h) {
+        if (g.j0 >= j1[h]) return true;
+        if (n_q[h] > 0 && !wait_all(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
+        ++n_q[h];
+        if (lane == 0) {
+          sl::mbar_arrive_expect_tx(&sy.q_full[h], q_bytes * C::kChunks);
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            tma_load_3d(buf + (h * C::kChunks + c) * kSlotBytes, &p.q, &sy.q_full[h], 64 * c,
+                        g.head * p.group, g.q0 + g.tok + h * p.half_tokens);
+        }
+        return true;
+      };
+      auto load_k = [&](int j) {
+#pragma unroll
+        for (int c = 0; c < C::kChunks; ++c) {
+          if (!claim(kSlotBytes)) return false;
+          if (lane == 0) {
+            uint8_t* dst = ring + kv.slot * kSlotBytes;
+            // the last columns may be one row that all heads share
+            const bool own = !(kDim == 192 && c == 2 && p.shared);
+            tma_load_3d(dst, own ? &p.k : &p.ks, &sy.full[kv.slot], own ? 64 * c : 0,
+                        own ? g.head : 0, g.k0 + j * kTile);
+          }
+          advance();
+        }
+        return true;
+      };
+      auto load_v = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < C::kVSlots; ++i) {
+          if (!claim(kSlotBytes)) return false;
+          if (lane == 0)
+#pragma unroll
+            for (int c = 0; c < kVDim / 64; ++c)
+              tma_load_3d(ring + kv.slot * kSlotBytes + c * C::kVRows * 128, &p.v,
+                          &sy.full[kv.slot], 64 * c, g.head, g.k0 + j * kTile + i * C::kVRows);
+          advance();
+        }
+        return true;
+      };
+      ok = load_q(0) && load_k(g.j0) && load_q(1);
+      for (int j = g.j0; j < g.j1 && ok; ++j) {
+        ok = load_v(j);
+        if (ok && j + 1 < g.j1) ok = load_k(j + 1);
+      }
+    }
+    if (!ok) {
+      // what was asked for lands before the buffers go
+      const int last = turns > 0 ? C::kSlots : kv.slot;
+      for (int i = 0; i < last; ++i)
+        (void)wait_all(&sy.full[i], i < kv.slot ? kv.phase : kv.phase ^ 1);
+      for (int h = 0; h < 2; ++h)
+        if (n_q[h] > 0) (void)wait_all(&sy.q_full[h], (n_q[h] - 1) & 1);
+    }
+  } else {
+    // ------------------------------------------------------ value guards
+    // In a tile that reaches past what the item's first row sees, rows of
+    // other sequences are zeroed (a weight of zero times what they hold could
+    // be NaN), and so are values that are not finite; those that some row
+    // does see are marked for the output to put back.
+    const int t = tid - 10 * 32;
+    Ring kv;
+    int n_item = 0;
+    while (ok && walk.next(p, sy.cum, per, g)) {
+      if (g.j0 >= g.j1) continue;
+      const int mark = n_item++;
+      for (int j = g.j0; j < g.j1 && ok; ++j) {
+        // every use of a slot is waited for, cleaned or not: a wait names a use
+        // by its parity alone
+        for (int c = 0; c < C::kChunks && ok; ++c) {
+          ok = wait_all(&sy.full[kv.slot], kv.phase);
+          kv.step<C::kSlots>();
+        }
+        const bool guard = (j + 1) * kTile > g.lim0;
+        for (int i = 0; i < C::kVSlots && ok; ++i) {
+          if (!(ok = wait_all(&sy.full[kv.slot], kv.phase))) break;
+          if (guard) {
+            const int key0 = j * kTile + i * C::kVRows;
+            const int lo = clampi(g.lim0 - key0, 0, C::kVRows);     // rows that all see
+            const int hi = clampi(g.k_len - key0, 0, C::kVRows);    // rows of the sequence
+            uint8_t* base = ring + kv.slot * kSlotBytes;
+            bool found = false;
+            for (int x = t; x < 1024; x += 64) {
+              const int r = (x >> 3) & (C::kVRows - 1);
+              if (r < lo) continue;
+              uint4* at = reinterpret_cast<uint4*>(base + x * 16);
+              if (r >= hi) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 w = *at;
+              uint32_t* e = &w.x;
+              bool bad = false;
+              constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((e[k] & kExp) == kExp) {
+                  e[k] &= 0xffff0000u;
+                  bad = true;
+                }
+                if ((e[k] & (kExp << 16)) == kExp << 16) {
+                  e[k] &= 0xffffu;
+                  bad = true;
+                }
+              }
+              if (bad) {
+                *at = w;
+                found = true;
+              }
+            }
+            if (found) sy.mark[mark % kMarks] = mark;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) sl::mbar_arrive(&sy.clean[kv.slot]);
+          }
+          kv.step<C::kSlots>();
+        }
+      }
+    }
+  }
+  if (!ok && lane == 0) atomicMax(p.status, SL_ERR_TIMEOUT);
+  sl::tc_fence_before();
+  __syncthreads();
+  sl::tc_fence_after();
+  if (warp == 8) sl::tmem_dealloc(tmem, 512);
+}
+
+// Joins the partial results of an item that several CTAs share. Block c looks
+// at the boundary between CTAs c and c + 1: the first boundary inside an item
+// joins all of the item's stretches, in order.
+constexpr int kJoinThreads = 256;
+
+template <int kVDim, bool kBf16>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(
+    const __grid_constant__ Params p) {
+  __shared__ int cum[kCoarse + 1], warp_sum[kCoarse / 32];
+  sl::pdl_wait();
+  sl::pdl_trigger();
+  const int per = (p.B + kCoarse - 1) / kCoarse;
+  build_table(p, cum, warp_sum, per);
+  const int total = Walk::units(p, cum);
+  const int c = blockIdx.x;
+  const int u = Walk::share(p, total, c + 1);
+  if (u >= total) return;
+  Seg g;
+  int j, n;
+  Walk::locate(p, cum, per, u, g, j, n);
+  const int u0 = u - j;  // the item's first unit
+  // whole on this side, or joined by an earlier boundary (the same boundary,
+  // too, where a CTA's share is empty)
+  if (j == 0 || Walk::share(p, total, c) > u0 || Walk::share(p, total, c) == u) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = 2 * p.half_tokens * p.group;
+  constexpr int kCols = kVDim / 32;
+  for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows;
+       r += gridDim.y * (kJoinThreads / 32)) {
+    const int token = r / p.group, tok = g.tok + token;
+    if (tok >= g.q_len) break;
+    const int lim = clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len);
+    float m = -INFINITY, l = 0.f, o[kCols] = {};
+    for (int s = c; s < p.grid && Walk::share(p, total, s) < u0 + n; ++s) {
+      if (Walk::share(p, total, s) == Walk::share(p, total, s + 1)) continue;
+      const int slot = 2 * s + (s == c && Walk::share(p, total, s) <= u0 ? 1 : 0);
+      const int64_t at = static_cast<int64_t>(slot) * p.rows_cap + r;
+      const float2 ml = p.part_ml[at];
+      const float m1 = max2(m, ml.x);
+      const float base = m1 == -INFINITY ? 0.f : m1;
+      const float a = ex2((m - base) * p.scale_log2), b = ex2((ml.x - base) * p.scale_log2);
+      const float* src = p.part + at * kVDim + lane * kCols;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] = o[i] * a + src[i] * b;
+      l = l * a + ml.y * b;
+      m = m1;
+    }
+    const float inv = lim == 0 ? 0.f : 1.f / l;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) +
+        static_cast<int64_t>(g.q0 + tok) * p.out_token +
+        static_cast<int64_t>(g.head * p.group + r - token * p.group) * p.out_head + lane * kCols;
+#pragma unroll
+    for (int i = 0; i < kCols; i += 2)
+      *reinterpret_cast<uint32_t*>(dst + i) = pack2<kBf16>(o[i] * inv, o[i + 1] * inv);
+  }
+}
+
+// --------------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// [tokens, heads, columns] with strides in elements, in boxes of 64 columns
+// (one 128-byte swizzled row each), box_heads heads and box_tokens tokens.
+bool make_map(CUtensorMap* m, const void* base, bool bf16, int64_t columns, int64_t heads,
+              int64_t tokens, int64_t head_stride, int64_t token_stride, int box_heads,
+              int box_tokens) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2,
+                           static_cast<cuuint64_t>(token_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t step[3] = {1, 1, 1};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int64_t kHeaderBytes = 256;
+constexpr int64_t kMostUnits = 1 << 22;
+
+struct Shape {
+  int64_t items, units;  // at most so many items, and key tiles of all items
+  int64_t grid;
+  bool split;
+  int rows_cap;
+};
+
+Shape shape_of(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads, int sms) {
+  Shape r;
+  const int group = heads / kv_heads;
+  const int64_t tokens = 2 * (kTile / group);
+  const int64_t items = (Tq + B * (tokens - 1)) / tokens;
+  r.items = (items < Tq ? items : Tq) * kv_heads;
+  r.units = r.items * (Tk / kTile + 2);
+  // few items with long key ranges: share out the key tiles instead
+  r.split = r.items < sms && Tk / B >= 8 * kTile && r.units < kMostUnits;
+  r.grid = r.split ? (r.units < sms ? r.units : sms) : (r.items < sms ? r.items : sms);
+  const int64_t rows = Tq * group;
+  r.rows_cap = static_cast<int>(rows < 2 * kTile ? rows : 2 * kTile);
+  return r;
+}
+
+template <int kDim, int kVDim, bool kBf16>
+int launch_all(const Params& p, cudaStream_t st) {
+  auto kern = attention_kernel<kDim, kVDim, kBf16>;
+  static std::atomic<uint64_t> smem_set{0};
+  SL_CUDA_TRY(sl::ensure_smem_limit(kern, kSmemBytes, smem_set));
+  SL_CUDA_TRY(sl::launch(kern, dim3(p.grid), dim3(kThreads), kSmemBytes, st, p));
+  if (p.split && p.grid > 1)
+    SL_CUDA_TRY(sl::launch(attention_join_kernel<kVDim, kBf16>,
+                           dim3(p.grid - 1, p.rows_cap > 64 ? 4 : 1), dim3(kJoinThreads), 0, st,
+                           p));
   return SL_OK;
 }
 
@@ -112,8 +993,14 @@ int run(const sl_attention_args& a, int32_t* status, cudaStream_t st) {
 
 extern "C" size_t sl_prompt_attention_workspace_bytes(int B, int64_t Tq, int64_t Tk, int heads,
                                                       int kv_heads, int v_dim) {
-  if (B <= 0 || Tq < 0 || Tk < 0 || heads <= 0 || kv_heads <= 0 || v_dim <= 0) return 0;
-  return 256;
+  if (B <= 0 || Tq < 0 || Tk < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
+      heads / kv_heads > kTile || v_dim <= 0)
+    return 0;
+  const int sms = sl_device_sm_count();
+  // (without a device: the size for this part's 148)
+  const Shape r = shape_of(B, Tq, Tk, heads, kv_heads, sms > 0 ? sms : 148);
+  if (!r.split) return kHeaderBytes;
+  return static_cast<size_t>(kHeaderBytes + 2 * r.grid * r.rows_cap * (4 * (int64_t)v_dim + 8));
 }
 
 extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspace,
@@ -126,7 +1013,7 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   const bool dims = (a.dim == 64 && a.v_dim == 64) || (a.dim == 128 && a.v_dim == 128) ||
                     (a.dim == 192 && a.v_dim == 128);
   if (!dims || (a.shared_dim != 0 && !(a.shared_dim == 64 && a.dim == 192)) ||
-      (a.dtype != SL_DTYPE_BF16 && a.dtype != SL_DTYPE_FP16) || a.heads / a.kv_heads > 128 ||
+      (a.dtype != SL_DTYPE_BF16 && a.dtype != SL_DTYPE_FP16) || a.heads / a.kv_heads > kTile ||
       a.Tq > 0x7fffffff || a.Tk > 0x7fffffff)
     return SL_ERR_UNSUPPORTED;
   if (a.Tq == 0) return SL_OK;
@@ -144,7 +1031,50 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   if ((a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.k_shared_token |
        a.out_token | a.out_head) & 7)
     return SL_ERR_INVALID;
+  const int sms = sl_device_sm_count();
+  if (sms <= 0) return SL_ERR_CUDA;
+  const Shape r = shape_of(a.B, a.Tq, a.Tk, a.heads, a.kv_heads, sms);
+  if (r.items >= kMostUnits) return SL_ERR_UNSUPPORTED;
+  const bool bf16 = a.dtype == SL_DTYPE_BF16;
+  Params p = {};
+  p.group = a.heads / a.kv_heads;
+  p.half_tokens = kTile / p.group;
+  bool ok = make_map(&p.q, a.q, bf16, a.dim, a.heads, a.Tq, a.q_head, a.q_token, p.group,
+                     p.half_tokens);
+  if (keys) {
+    ok = ok && make_map(&p.k, a.k, bf16, a.dim - a.shared_dim, a.kv_heads, a.Tk, a.k_head,
+                        a.k_token, 1, kTile);
+    ok = ok && make_map(&p.v, a.v, bf16, a.v_dim, a.kv_heads, a.Tk, a.v_head, a.v_token, 1,
+                        a.v_dim == 128 ? kTile / 2 : kTile);
+    if (a.shared_dim)
+      ok = ok && make_map(&p.ks, a.k_shared, bf16, a.shared_dim, 1, a.Tk, a.shared_dim,
+                          a.k_shared_token, 1, kTile);
+  }
+  if (!ok) return SL_ERR_INVALID;
+  p.out = a.out;
+  p.out_token = a.out_token;
+  p.out_head = a.out_head;
+  p.cu_q = a.cu_q;
+  p.cu_k = a.cu_k;
+  p.vraw = a.v;
+  p.v_token = a.v_token;
+  p.v_head = a.v_head;
+  p.B = a.B;
+  p.Tq = static_cast<int>(a.Tq);
+  p.Tk = static_cast<int>(a.Tk);
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.shared = a.shared_dim != 0;
+  p.grid = static_cast<int>(r.grid);
+  p.split = r.split;
+  p.rows_cap = r.rows_cap;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = static_cast<int32_t*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
+  p.part_ml = reinterpret_cast<float2*>(p.part + 2 * r.grid * r.rows_cap * a.v_dim);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  int32_t* status = static_cast<int32_t*>(workspace);
-  return a.dtype == SL_DTYPE_BF16 ? run<__nv_bfloat16>(a, status, st) : run<__half>(a, status, st);
+  if (a.dim == 64) return bf16 ? launch_all<64, 64, true>(p, st) : launch_all<64, 64, false>(p, st);
+  if (a.dim == 128)
+    return bf16 ? launch_all<128, 128, true>(p, st) : launch_all<128, 128, false>(p, st);
+  return bf16 ? launch_all<192, 128, true>(p, st) : launch_all<192, 128, false>(p, st);
 }
