@@ -37,6 +37,9 @@ constexpr int kSlotBytes = 16384;
 constexpr int kCoarse = 256;         // entries of the work table
 constexpr int kMaxSlots = 12;
 constexpr float kLag = 8.f;          // how far (in powers of 2) the maximum may lag behind
+// registers a thread: 168 at launch, then shared out between the softmax warps
+// and the others (256 x 208 + 128 x 88 = 384 x 168)
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kMarks = 16;           // items that the value guards may be ahead by
 
 struct Params {
@@ -121,6 +124,27 @@ __device__ __forceinline__ void tmem_fence_ld(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+// Eight columns of this thread's row times f.
+__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
+                   taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -442,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
 
   if (warp < 8) {
     // ---------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int h = warp >> 2;
     const int row = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // (warp mod 4) * 32 lanes
@@ -499,15 +524,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
             // the sums so far, once the products before this tile are in
             if (!(ok = wait_all(&sy.pv_done[h], (n_s - 1) & 1))) break;
             sl::tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < kVDim / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_at + 32 * c, o);
-              tmem_fence_ld(o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-              tmem_st32(o_at + 32 * c, o);
-            }
+            // (rare: eight columns at a time, the scores keep their registers)
+#pragma unroll 1
+            for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
           }
         }
         const float base = m == -INFINITY ? 0.f : -m * p.scale_log2;
@@ -606,7 +625,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         if (lane == 0) sl::mbar_arrive(&sy.o_free[h]);
       }
     }
-  } else if (warp == 8) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  }
+  if (warp == 8) {
     // -------------------------------------------------------------- MMA
     constexpr uint32_t idesc_s = idesc_f16(kBf16, kTile, false);
     constexpr uint32_t idesc_o = idesc_f16(kBf16, kVDim, true);
@@ -787,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       for (int h = 0; h < 2; ++h)
         if (n_q[h] > 0) (void)wait_all(&sy.q_full[h], (n_q[h] - 1) & 1);
     }
-  } else {
+  } else if (warp > 9) {
     // ------------------------------------------------------ value guards
     // In a tile that reaches past what the item's first row sees, rows of
     // other sequences are zeroed (a weight of zero times what they hold could
