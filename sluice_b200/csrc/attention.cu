@@ -16,8 +16,8 @@
 // core works for the other.
 //
 // Roles (12 warps): 0-3 and 4-7 softmax of the two halves (a row per thread)
-// and their output; 8 issues the MMAs; 9 the tile loads (TMA); 10, 11 clean
-// the value tiles that hold keys which some row may not see.
+// and their output; 8 and 11 issue the MMAs of a half each; 9 the tile loads
+// (TMA); 10 cleans the value tiles that hold keys which some row may not see.
 //
 // Shared memory: the item's queries (2 x 128 rows) and a ring of 16 KB slots
 // that the key and value tiles pass through: 64 columns of 128 keys, or 64
@@ -26,6 +26,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -35,8 +36,10 @@ constexpr int kThreads = 384;
 constexpr int kTile = 128;           // rows of a half and keys of a tile
 constexpr int kSlotBytes = 16384;
 constexpr int kCoarse = 256;         // entries of the work table
-constexpr int kMaxSlots = 12;
-constexpr float kLag = 8.f;          // how far (in powers of 2) the maximum may lag behind
+constexpr int kBars = 16;            // barriers of tiles in flight
+// How far (in powers of 2) a row's maximum may lag behind its scores: bf16
+// weights have the exponents of the 32-bit sums, fp16 ones end at 2^16.
+constexpr float kLagBf16 = 32.f, kLagF16 = 8.f;
 // registers a thread: 168 at launch, then shared out between the softmax warps
 // and the others (256 x 208 + 128 x 88 = 384 x 168)
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
@@ -56,6 +59,7 @@ struct Params {
   int split;                         // 1: equal shares of all key tiles per CTA
   int rows_cap;                      // rows of a partial result
   float scale_log2;                  // scale / ln 2
+  float lag;                         // how far the maximum may lag behind, in scores
   float* part;                       // [2 * grid][rows_cap][v_dim]
   float2* part_ml;                   // [2 * grid][rows_cap] (maximum, sum)
   int32_t* status;
@@ -70,26 +74,39 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(sl::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-// D (+)= A B, A from TMEM (the weights), B from shared memory.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+// Shared-memory matrix descriptors of 128-byte swizzled tiles: 8-row groups
+// 1024 bytes apart (high word, with the version and the swizzle); the low word
+// is the address / 16 and the step between 64-column groups / 16. An operand
+// whose rows hold the reduction index's values (queries, keys) has one group
+// per row; one whose rows are the reduction index (values: a row per key) has
+// the next 64 columns a group of rows further.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kKMajorLo = 1u << 16;
+template <int kRows>
+constexpr uint32_t kRowMajorLo = static_cast<uint32_t>(kRows * 128 >> 4) << 16;
+
+// D (+)= A B, both from shared memory.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)
       : "memory");
 }
-// Shared-memory descriptor of an operand whose rows are the reduction index
-// (values: a row per key, 128-byte swizzled rows of 64 columns): 8-row groups
-// 1024 bytes apart, the next 64 columns `lbo` bytes on.
-__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t lbo) {
-  uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(lbo >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
+// D (+)= A B, A from TMEM (the weights).
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)
+      : "memory");
 }
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int N, bool b_rows) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_rows ? 1u << 16 : 0u) |
@@ -175,9 +192,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return d;
 }
 
-// A bounded wait whose outcome all lanes of the warp agree on.
-__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, sl::mbar_wait(bar, parity));
+// A bounded wait of a whole warp: its lanes run the same instructions on the
+// same word, so they agree on the outcome.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  const bool done = sl::mbar_wait(bar, parity);
+  __syncwarp();
+  return done;
 }
 
 // --------------------------------------------------------------------- work
@@ -298,6 +318,22 @@ __device__ __forceinline__ void fill_seg(const Params& p, const Seq& s, Seg& g) 
   g.n = max(g.nh[0], g.nh[1]);
 }
 
+// The parts of a stretch that steer the issuing warps, as values that the
+// compiler knows to be the same in all lanes.
+__device__ __forceinline__ void uniform(Seg& g) {
+  constexpr unsigned kAll = 0xffffffffu;
+  g.head = __shfl_sync(kAll, g.head, 0);
+  g.q0 = __shfl_sync(kAll, g.q0, 0);
+  g.k0 = __shfl_sync(kAll, g.k0, 0);
+  g.k_len = __shfl_sync(kAll, g.k_len, 0);
+  g.tok = __shfl_sync(kAll, g.tok, 0);
+  g.j0 = __shfl_sync(kAll, g.j0, 0);
+  g.j1 = __shfl_sync(kAll, g.j1, 0);
+  g.nh[0] = __shfl_sync(kAll, g.nh[0], 0);
+  g.nh[1] = __shfl_sync(kAll, g.nh[1], 0);
+  g.lim0 = __shfl_sync(kAll, g.lim0, 0);
+}
+
 // Walks a CTA's share of the work. Every role's warp walks it by itself.
 //   whole items: the longest first, dealt out in turns that go back and forth;
 //   split: an equal run of key tiles, item after item.
@@ -390,8 +426,8 @@ struct Cfg {
 };
 
 struct Sync {
-  uint64_t full[kMaxSlots], empty[kMaxSlots], clean[kMaxSlots];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], o_free[2], drain;
+  uint64_t full[kBars], empty[kBars], clean[kBars];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2], o_free[2], drain[2], turn[2][4];
   uint32_t tmem;
   int mark[kMarks];
   int warp_sum[kCoarse / 32];
@@ -400,18 +436,58 @@ struct Sync {
 constexpr int kSmemBytes = 14 * kSlotBytes + 1024 + static_cast<int>(sizeof(Sync));
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
-// A place in the ring and the parity of its current use.
-struct Ring {
+// A role's place in the sequence of tiles (keys, values, keys, ...): the
+// tile's number, which names its barriers and their parity, and its first slot.
+// At most kSlots tiles are in flight, fewer than there are barriers.
+struct Tiles {
+  uint32_t n = 0;
   int slot = 0;
-  uint32_t phase = 0;
+  __device__ __forceinline__ int bar() const { return n % kBars; }
+  __device__ __forceinline__ uint32_t phase() const { return (n / kBars) & 1; }
   template <int N>
-  __device__ __forceinline__ void step() {
-    if (++slot == N) {
-      slot = 0;
-      phase ^= 1;
-    }
+  __device__ __forceinline__ int place(int i) const {
+    return slot + i < N ? slot + i : slot + i - N;
+  }
+  template <int N>
+  __device__ __forceinline__ void step(int slots) {
+    slot = place<N>(slots);
+    ++n;
   }
 };
+
+// Rows [lo, rows) of a value group (128-byte rows in shared memory, any
+// swizzle): those from hi on are zeroed, and values that are not finite in
+// the others. Whether there were any.
+template <bool kBf16>
+__device__ __forceinline__ bool clean_rows(uint8_t* base, int lo, int hi, int rows, int lane) {
+  constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+  bool found = false;
+#pragma unroll 4
+  for (int x = lo * 8 + lane; x < hi * 8; x += 32) {
+    uint4* at = reinterpret_cast<uint4*>(base + x * 16);
+    uint4 w = *at;
+    uint32_t* e = &w.x;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if ((e[k] & kExp) == kExp) {
+        e[k] &= 0xffff0000u;
+        bad = true;
+      }
+      if ((e[k] & (kExp << 16)) == kExp << 16) {
+        e[k] &= 0xffffu;
+        bad = true;
+      }
+    }
+    if (bad) {
+      *at = w;
+      found = true;
+    }
+  }
+  for (int x = max(lo, hi) * 8 + lane; x < rows * 8; x += 32)
+    *reinterpret_cast<uint4*>(base + x * 16) = make_uint4(0, 0, 0, 0);
+  return found;
+}
 
 template <int kDim, int kVDim, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
@@ -422,24 +498,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       (reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = buf + C::kQBytes;
   Sync& sy = *reinterpret_cast<Sync*>(buf + C::kBufBytes);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int per = (p.B + kCoarse - 1) / kCoarse;
 
   if (tid == 0) {
-    for (int i = 0; i < C::kSlots; ++i) {
+    for (int i = 0; i < kBars; ++i) {
       sl::mbar_init(&sy.full[i], 1);
-      sl::mbar_init(&sy.empty[i], 1);
-      sl::mbar_init(&sy.clean[i], 2);
+      sl::mbar_init(&sy.empty[i], 2);
+      sl::mbar_init(&sy.clean[i], 1);
     }
     for (int h = 0; h < 2; ++h) {
       sl::mbar_init(&sy.q_full[h], 1);
       sl::mbar_init(&sy.q_empty[h], 1);
       sl::mbar_init(&sy.s_full[h], 1);
-      sl::mbar_init(&sy.p_full[h], 4);
+      sl::mbar_init(&sy.p_full[h][0], 4);
+      sl::mbar_init(&sy.p_full[h][1], 4);
       sl::mbar_init(&sy.pv_done[h], 1);
       sl::mbar_init(&sy.o_free[h], 4);
+      sl::mbar_init(&sy.drain[h], 1);
+      for (int i = 0; i < 4; ++i) sl::mbar_init(&sy.turn[h][i], 1);
     }
-    sl::mbar_init(&sy.drain, 1);
     for (int i = 0; i < kMarks; ++i) sy.mark[i] = -1;
     sl::fence_barrier_init();
   }
@@ -474,80 +552,135 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     const int token = row / p.group, in_group = row - token * p.group;
     const bool packed = token < p.half_tokens;
     int n_s = 0, n_item = 0;  // key tiles so far; items with keys so far
+    // The warps of the two halves that share a scheduler take turns at the
+    // exponentials, so that one half's run while the other's products do.
+    int n_turn = h - 1;
+    auto take_turn = [&]() -> bool {
+      const int t = n_turn++;
+      return t < 0 || wait(&sy.turn[h][warp & 3], t & 1);
+    };
+    auto pass_turn = [&]() {
+      if (lane == 0) sl::mbar_arrive(&sy.turn[h ^ 1][warp & 3]);
+    };
     while (ok && walk.next(p, sy.cum, per, g)) {
       const int first = g.tok + h * p.half_tokens;
       const int j1 = min(g.j1, g.nh[h]);
       const bool has = g.j0 < g.j1;
       const int mark = has ? n_item++ : -1;
-      if (first >= g.q_len) continue;
+      if (first >= g.q_len) {
+        for (int j = g.j0; j < g.j1 && ok; ++j) {
+          ok = take_turn();
+          pass_turn();
+        }
+        continue;
+      }
       const int tok = first + token;
       const bool live = packed && tok < g.q_len;
       const int lim = live ? clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len) : 0;
       const int lim_first = clampi(first + 1 + g.k_len - g.q_len, 0, g.k_len);
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, base = 0.f;  // base: -m in powers of 2
       for (int j = g.j0; j < j1; ++j) {
-        if (!(ok = wait_all(&sy.s_full[h], n_s & 1))) break;
+        if (!(ok = wait(&sy.s_full[h], n_s & 1))) break;
         sl::tc_fence_after();
         uint32_t r[kTile];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
-        if ((j + 1) * kTile > lim_first) {
-          const int left = lim - j * kTile;
-#pragma unroll
-          for (int c = 0; c < kTile; ++c)
-            if (c >= left) r[c] = 0xff800000u;  // -inf
-        }
         auto s = [&](int c) { return __uint_as_float(r[c]); };
-        float top = max3(s(0), s(1), s(2)), top2 = max3(s(3), s(4), s(5));
+        auto load_scores = [&]() {
 #pragma unroll
-        for (int c = 6; c < kTile - 2; c += 4) {
-          top = max3(top, s(c), s(c + 1));
-          top2 = max3(top2, s(c + 2), s(c + 3));
-        }
-        top = max3(top, s(kTile - 2), s(kTile - 1));
-        top = max2(top, top2);
-        // a score of +inf leaves no finite weights: the row is NaN, as
-        // inf - inf makes it
-        if (top == INFINITY) top = __int_as_float(0x7fffffff);
-        const float m1 = max2(m, top);
-        // the maximum may lag behind by a factor 2^kLag: the weights stay
-        // far inside the type's range, and the sums and outputs are rescaled
-        // only where it grows by more (also on NaN, and on the first tile)
-        const bool move = live && !((m1 - m) * p.scale_log2 <= kLag) && !(m1 == -INFINITY);
-        if (__any_sync(0xffffffffu, move)) {
-          const float corr = m1 == -INFINITY ? 1.f : ex2((m - m1) * p.scale_log2);
-          m = m1;
-          l *= corr;
-          if (j > g.j0) {
-            // the sums so far, once the products before this tile are in
-            if (!(ok = wait_all(&sy.pv_done[h], (n_s - 1) & 1))) break;
-            sl::tc_fence_after();
-            // (rare: eight columns at a time, the scores keep their registers)
-#pragma unroll 1
-            for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
+          for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
+        };
+        float2 sum = make_float2(0.f, 0.f);
+        // Scores [c0, c0 + 64) as weights, in place and packed.
+        auto weights = [&](int c0) {
+          const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
+#pragma unroll
+          for (int c = c0 / 2; c < c0 / 2 + 32; ++c) {
+            float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum = __fadd2_rn(sum, x);
+            r[c] = pack2<kBf16>(x.x, x.y);
+          }
+        };
+        // Handed over in halves: the product with the first 64 values runs
+        // while the weights of the others are formed.
+        auto hand_over = [&](int c0) {
+          tmem_st32(s_at + c0 / 2, r + c0 / 2);
+          if (c0 != 0) pass_turn();
+          tmem_wait_st();
+          sl::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) sl::mbar_arrive(&sy.p_full[h][c0 != 0]);
+        };
+        auto row_max = [&]() {
+          float t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = max3(s(32 * i), s(32 * i + 1), s(32 * i + 2));
+#pragma unroll
+          for (int c = 3; c < 31; c += 2)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = max3(t[i], s(32 * i + c), s(32 * i + c + 1));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = max2(t[i], s(32 * i + 31));
+          return max2(max3(t[0], t[1], t[2]), t[3]);
+        };
+        load_scores();
+        if (!(ok = take_turn())) break;
+        const bool hides = (j + 1) * kTile > lim_first;
+        bool go_on = false;
+        if (j > g.j0 && !hides) {
+          // Most tiles: weights against the maximum so far, which may lag
+          // behind this tile's by a factor 2^kLag (the sums and the weights'
+          // type hold that). The tile's own maximum is found meanwhile, and
+          // only where it is beyond that (or NaN) is the work done again.
+          const float top = row_max();
+          weights(0);
+          go_on = !__any_sync(0xffffffffu, live && !(top <= m + p.lag));
+          if (!go_on) {
+            load_scores();
+            sum = make_float2(0.f, 0.f);
           }
         }
-        const float base = m == -INFINITY ? 0.f : -m * p.scale_log2;
-        float2 sum = make_float2(0.f, 0.f);
-        const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
+        if (!go_on) {
+          if (hides) {
+            const int left = lim - j * kTile;
 #pragma unroll
-        for (int c = 0; c < kTile / 2; ++c) {
-          float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          sum = __fadd2_rn(sum, x);
-          r[c] = pack2<kBf16>(x.x, x.y);
+            for (int c = 0; c < kTile; ++c)
+              if (c >= left) r[c] = 0xff800000u;  // -inf
+          }
+          float top = row_max();
+          // a score of +inf leaves no finite weights: the row is NaN, as
+          // inf - inf makes it
+          if (top == INFINITY) top = __int_as_float(0x7fffffff);
+          const float m1 = max2(m, top);
+          const bool move = live && !(m1 <= m + p.lag);
+          if (__any_sync(0xffffffffu, move)) {
+            const float corr = move ? ex2((m - m1) * p.scale_log2) : 1.f;
+            if (move) m = m1;
+            base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+            l *= corr;
+            if (j > g.j0) {
+              // the sums so far, once the products before this tile are in
+              if (!(ok = wait(&sy.pv_done[h], (n_s - 1) & 1))) break;
+              sl::tc_fence_after();
+              // (rare: eight columns at a time, the scores keep their registers)
+#pragma unroll 1
+              for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
+            }
+          }
+          weights(0);
         }
+        hand_over(0);
+        weights(64);
+        hand_over(64);
         l += sum.x + sum.y;
-        tmem_st32(s_at, r);
-        tmem_st32(s_at + 32, r + 32);
-        tmem_wait_st();
-        sl::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) sl::mbar_arrive(&sy.p_full[h]);
         ++n_s;
+      }
+      // (the other half may have more tiles)
+      for (int j = max(g.j0, j1); j < g.j1 && ok; ++j) {
+        ok = take_turn();
+        pass_turn();
       }
       if (!ok) break;
       // ------------------------------------------------------- output
@@ -560,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           make_float2(m, l);
       const bool ran = g.j0 < j1;
       if (ran) {
-        if (!(ok = wait_all(&sy.pv_done[h], (n_s - 1) & 1))) break;
+        if (!(ok = wait(&sy.pv_done[h], (n_s - 1) & 1))) break;
         sl::tc_fence_after();
       }
       const bool repair = has && sy.mark[mark % kMarks] == mark;
@@ -628,135 +761,129 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   }
-  if (warp == 8) {
-    // -------------------------------------------------------------- MMA
+  if (warp == 8 || warp == 11) {
+    // ------------------------------------------------- MMAs of one half
+    const int h = warp == 8 ? 0 : 1;
     constexpr uint32_t idesc_s = idesc_f16(kBf16, kTile, false);
     constexpr uint32_t idesc_o = idesc_f16(kBf16, kVDim, true);
-    const uint32_t q_sm = sl::smem_u32(buf), ring_sm = sl::smem_u32(ring);
-    Ring kv;                       // next slot to take up
-    int n_s[2] = {0, 0}, n_o[2] = {0, 0}, n_q[2] = {0, 0};
+    const uint32_t q_lo = kKMajorLo + ((sl::smem_u32(buf) + h * C::kChunks * kSlotBytes) >> 4);
+    const uint32_t ring_lo = sl::smem_u32(ring) >> 4;
+    const uint32_t s_d = s_col[h], o_d = o_col[h];
+    const bool leader = sl::elect_one();
+    Tiles at;
+    int n_s = 0, n_o = 0;
     uint32_t clean_phase = 0;
-    while (ok && walk.next(p, sy.cum, per, g)) {
-      if (g.j0 >= g.j1) continue;
-      const int j1[2] = {min(g.j1, g.nh[0]), min(g.j1, g.nh[1])};
-      int k_slot[C::kChunks], v_slot[C::kVSlots];
-      // S of one half against the key tile in k_slot
-      auto scores = [&](int h) {
-        if (sl::elect_one()) {
+    // S = Q K^T with the key tile at `at`, or (this half sees none of it) let
+    // it go
+    auto key_tile = [&](bool mine) {
+      if (leader) {
+        if (mine) {
 #pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
+          for (int c = 0; c < C::kChunks; ++c) {
+            const uint32_t k_lo = kKMajorLo + ring_lo + at.place<C::kSlots>(c) * (kSlotBytes >> 4);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              sl::umma_bf16(s_col[h],
-                            sl::umma_desc_sw128(q_sm + (h * C::kChunks + c) * kSlotBytes + 32 * k),
-                            sl::umma_desc_sw128(ring_sm + k_slot[c] * kSlotBytes + 32 * k),
-                            idesc_s, c + k > 0);
+              umma_ss(s_d, q_lo + c * (kSlotBytes >> 4) + 2 * k, k_lo + 2 * k, idesc_s, c + k > 0);
+          }
           sl::umma_commit(&sy.s_full[h]);
+          sl::umma_commit(&sy.empty[at.bar()]);
+        } else {
+          sl::mbar_arrive(&sy.empty[at.bar()]);
         }
-        __syncwarp();
-      };
-      auto release = [&](const int* slot, int n) {
-        if (sl::elect_one())
-          for (int i = 0; i < n; ++i) sl::umma_commit(&sy.empty[slot[i]]);
-        __syncwarp();
-      };
-      auto take = [&](int* slot, int n) {
-        for (int i = 0; i < n && ok; ++i) {
-          slot[i] = kv.slot;
-          ok = wait_all(&sy.full[kv.slot], kv.phase);
-          kv.step<C::kSlots>();
-        }
-        sl::tc_fence_after();
-      };
-      take(k_slot, C::kChunks);
-      for (int h = 0; h < 2 && ok; ++h) {
-        if (g.j0 >= j1[h]) continue;
-        if (!(ok = wait_all(&sy.q_full[h], n_q[h] & 1))) break;
-        ++n_q[h];
-        scores(h);
       }
-      if (!ok) break;
-      release(k_slot, C::kChunks);
-      for (int j = g.j0; j < g.j1 && ok; ++j) {
-        take(v_slot, C::kVSlots);
-        if (!ok) break;
+      __syncwarp();
+      at.step<C::kSlots>(C::kChunks);
+    };
+    while (ok && walk.next(p, sy.cum, per, g)) {
+      uniform(g);
+      if (g.j0 >= g.j1) continue;
+      const int j1 = min(g.j1, g.nh[h]);
+      const bool any = g.j0 < j1;
+      if (any && !(ok = wait(&sy.q_full[h], n_o & 1))) break;
+      if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+      sl::tc_fence_after();
+      key_tile(any);
+      for (int j = g.j0; j < g.j1; ++j) {
+        const bool mine = j < j1;
+        // this tile's values and the next one's keys are here, as a rule, long
+        // before the weights
+        if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        const int v_bar = at.bar();
         if ((j + 1) * kTile > g.lim0) {
-          // cleaned by the guards first
+          // cleaned by the guard first
+          if (!(ok = wait(&sy.clean[v_bar], (clean_phase >> v_bar) & 1))) break;
+          clean_phase ^= 1u << v_bar;
+        }
+        const int v_slot0 = at.place<C::kSlots>(0), v_slot1 = at.place<C::kSlots>(1);
+        at.step<C::kSlots>(C::kVSlots);
+        const bool next = j + 1 < g.j1;
+        if (next && !(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        if (mine) {
+          if (j == g.j0 && n_o > 0 && !(ok = wait(&sy.o_free[h], (n_o - 1) & 1))) break;
+          // O += P V in two halves of 64 keys, as the weights come in
 #pragma unroll
-          for (int i = 0; i < C::kVSlots; ++i) {
-            if (!ok) break;
-            ok = wait_all(&sy.clean[v_slot[i]], (clean_phase >> v_slot[i]) & 1);
-            clean_phase ^= 1u << v_slot[i];
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = wait(&sy.p_full[h][half], n_s & 1))) break;
+            sl::tc_fence_after();
+            if (leader) {
+              const uint32_t v_lo = kRowMajorLo<C::kVRows> + ring_lo +
+                  (C::kVSlots == 2 ? (half ? v_slot1 : v_slot0) * (kSlotBytes >> 4)
+                                   : v_slot0 * (kSlotBytes >> 4) + half * 512);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_ts(o_d, s_d + 32 * half + 8 * k, v_lo + 128 * k, idesc_o,
+                        j > g.j0 || half + k > 0);
+            }
           }
           if (!ok) break;
-        }
-        bool next_key = false;
-        for (int h = 0; h < 2 && ok; ++h) {
-          if (j >= j1[h]) continue;
-          if (j == g.j0 && n_o[h] > 0 &&
-              !(ok = wait_all(&sy.o_free[h], (n_o[h] - 1) & 1)))
-            break;
-          if (!(ok = wait_all(&sy.p_full[h], n_s[h] & 1))) break;
-          ++n_s[h];
-          sl::tc_fence_after();
-          if (sl::elect_one()) {
-#pragma unroll
-            for (int i = 0; i < C::kVSlots; ++i)
-#pragma unroll
-              for (int k = 0; k < C::kVRows / 16; ++k)
-                umma_ts(o_col[h], s_col[h] + (i * (C::kVRows / 16) + k) * 8,
-                        desc_rows(ring_sm + v_slot[i] * kSlotBytes + 2048 * k, C::kVRows * 128),
-                        idesc_o, j > g.j0 || i + k > 0);
+          ++n_s;
+          if (leader) {
+            sl::umma_commit(&sy.empty[v_bar]);
             sl::umma_commit(&sy.pv_done[h]);
           }
-          __syncwarp();
-          if (j + 1 < j1[h]) {
-            if (!next_key) {
-              take(k_slot, C::kChunks);
-              next_key = true;
-              if (!ok) break;
-            }
-            scores(h);
-          }
+        } else if (leader) {
+          sl::mbar_arrive(&sy.empty[v_bar]);
         }
-        if (!ok) break;
-        release(v_slot, C::kVSlots);
-        // (a half may end earlier: the key tile is taken up by the other)
-        if (next_key) release(k_slot, C::kChunks);
+        __syncwarp();
+        if (next) key_tile(j + 1 < j1);
       }
       if (!ok) break;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (g.j0 < j1[h]) {
-          ++n_o[h];
-          if (sl::elect_one()) sl::umma_commit(&sy.q_empty[h]);
-          __syncwarp();
-        }
+      if (any) {
+        ++n_o;
+        if (leader) sl::umma_commit(&sy.q_empty[h]);
+        __syncwarp();
+      }
     }
     // everything issued is in before TMEM and the barriers go
-    if (sl::elect_one()) sl::umma_commit(&sy.drain);
+    if (leader) sl::umma_commit(&sy.drain[h]);
     __syncwarp();
-    ok = wait_all(&sy.drain, 0) && ok;
+    ok = wait(&sy.drain[h], 0) && ok;
   } else if (warp == 9) {
     // ------------------------------------------------------------ loads
-    Ring kv;
-    int n_q[2] = {0, 0}, turns = 0;
+    Tiles at;
+    // the oldest tile that still holds slots, whether it is one of values,
+    // and the slots that are free
+    uint32_t oldest = 0;
+    bool oldest_v = false;
+    int room = C::kSlots, n_q[2] = {0, 0};
     const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.half_tokens) * 128;
+    auto claim = [&](int slots) -> bool {
+      while (room < slots) {
+        if (!wait(&sy.empty[oldest % kBars], (oldest / kBars) & 1)) return false;
+        room += oldest_v ? C::kVSlots : C::kChunks;
+        oldest_v = !oldest_v;
+        ++oldest;
+      }
+      room -= slots;
+      if (lane == 0) sl::mbar_arrive_expect_tx(&sy.full[at.bar()], slots * kSlotBytes);
+      return true;
+    };
     while (ok && walk.next(p, sy.cum, per, g)) {
+      uniform(g);
       if (g.j0 >= g.j1) continue;
-      const int j1[2] = {min(g.j1, g.nh[0]), min(g.j1, g.nh[1])};
-      auto claim = [&](uint32_t bytes) -> bool {
-        if (turns > 0 && !wait_all(&sy.empty[kv.slot], kv.phase ^ 1)) return false;
-        if (lane == 0) sl::mbar_arrive_expect_tx(&sy.full[kv.slot], bytes);
-        return true;
-      };
-      auto advance = [&]() {
-        kv.step<C::kSlots>();
-        if (kv.slot == 0) turns = 1;
-      };
-      auto load_q = [&](int h) {
-        if (g.j0 >= j1[h]) return true;
-        if (n_q[h] > 0 && !wait_all(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
+      auto load_q = [&](int h) -> bool {
+        if (g.j0 >= min(g.j1, g.nh[h])) return true;
+        if (n_q[h] > 0 && !wait(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
         ++n_q[h];
         if (lane == 0) {
           sl::mbar_arrive_expect_tx(&sy.q_full[h], q_bytes * C::kChunks);
@@ -767,111 +894,80 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         }
         return true;
       };
-      auto load_k = [&](int j) {
+      auto load_k = [&](int j) -> bool {
+        if (!claim(C::kChunks)) return false;
+        if (lane == 0) {
 #pragma unroll
-        for (int c = 0; c < C::kChunks; ++c) {
-          if (!claim(kSlotBytes)) return false;
-          if (lane == 0) {
-            uint8_t* dst = ring + kv.slot * kSlotBytes;
+          for (int c = 0; c < C::kChunks; ++c) {
             // the last columns may be one row that all heads share
             const bool own = !(kDim == 192 && c == 2 && p.shared);
-            tma_load_3d(dst, own ? &p.k : &p.ks, &sy.full[kv.slot], own ? 64 * c : 0,
-                        own ? g.head : 0, g.k0 + j * kTile);
+            tma_load_3d(ring + at.place<C::kSlots>(c) * kSlotBytes, own ? &p.k : &p.ks,
+                        &sy.full[at.bar()], own ? 64 * c : 0, own ? g.head : 0,
+                        g.k0 + j * kTile);
           }
-          advance();
         }
+        at.step<C::kSlots>(C::kChunks);
         return true;
       };
-      auto load_v = [&](int j) {
+      auto load_v = [&](int j) -> bool {
+        if (!claim(C::kVSlots)) return false;
+        if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < C::kVSlots; ++i) {
-          if (!claim(kSlotBytes)) return false;
-          if (lane == 0)
+          for (int i = 0; i < C::kVSlots; ++i)
 #pragma unroll
             for (int c = 0; c < kVDim / 64; ++c)
-              tma_load_3d(ring + kv.slot * kSlotBytes + c * C::kVRows * 128, &p.v,
-                          &sy.full[kv.slot], 64 * c, g.head, g.k0 + j * kTile + i * C::kVRows);
-          advance();
+              tma_load_3d(ring + at.place<C::kSlots>(i) * kSlotBytes + c * C::kVRows * 128, &p.v,
+                          &sy.full[at.bar()], 64 * c, g.head, g.k0 + j * kTile + i * C::kVRows);
         }
+        at.step<C::kSlots>(C::kVSlots);
         return true;
       };
       ok = load_q(0) && load_k(g.j0) && load_q(1);
-      for (int j = g.j0; j < g.j1 && ok; ++j) {
-        ok = load_v(j);
-        if (ok && j + 1 < g.j1) ok = load_k(j + 1);
-      }
+      for (int j = g.j0; j < g.j1 && ok; ++j)
+        ok = load_v(j) && (j + 1 >= g.j1 || load_k(j + 1));
     }
     if (!ok) {
       // what was asked for lands before the buffers go
-      const int last = turns > 0 ? C::kSlots : kv.slot;
-      for (int i = 0; i < last; ++i)
-        (void)wait_all(&sy.full[i], i < kv.slot ? kv.phase : kv.phase ^ 1);
+      for (; oldest < at.n; ++oldest)
+        (void)wait(&sy.full[oldest % kBars], (oldest / kBars) & 1);
       for (int h = 0; h < 2; ++h)
-        if (n_q[h] > 0) (void)wait_all(&sy.q_full[h], (n_q[h] - 1) & 1);
+        if (n_q[h] > 0) (void)wait(&sy.q_full[h], (n_q[h] - 1) & 1);
     }
-  } else if (warp > 9) {
-    // ------------------------------------------------------ value guards
+  } else if (warp == 10) {
+    // ------------------------------------------------------- value guard
     // In a tile that reaches past what the item's first row sees, rows of
     // other sequences are zeroed (a weight of zero times what they hold could
     // be NaN), and so are values that are not finite; those that some row
     // does see are marked for the output to put back.
-    const int t = tid - 10 * 32;
-    Ring kv;
+    Tiles at;
     int n_item = 0;
     while (ok && walk.next(p, sy.cum, per, g)) {
+      uniform(g);
       if (g.j0 >= g.j1) continue;
       const int mark = n_item++;
-      for (int j = g.j0; j < g.j1 && ok; ++j) {
-        // every use of a slot is waited for, cleaned or not: a wait names a use
-        // by its parity alone
-        for (int c = 0; c < C::kChunks && ok; ++c) {
-          ok = wait_all(&sy.full[kv.slot], kv.phase);
-          kv.step<C::kSlots>();
-        }
-        const bool guard = (j + 1) * kTile > g.lim0;
-        for (int i = 0; i < C::kVSlots && ok; ++i) {
-          if (!(ok = wait_all(&sy.full[kv.slot], kv.phase))) break;
-          if (guard) {
+      for (int j = g.j0; j < g.j1; ++j) {
+        at.step<C::kSlots>(C::kChunks);
+        // every value tile is waited for, cleaned or not: a wait names a use
+        // of its barrier by the parity alone
+        if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        if ((j + 1) * kTile > g.lim0) {
+          bool found = false;
+          for (int i = 0; i < C::kVSlots; ++i) {
             const int key0 = j * kTile + i * C::kVRows;
             const int lo = clampi(g.lim0 - key0, 0, C::kVRows);     // rows that all see
             const int hi = clampi(g.k_len - key0, 0, C::kVRows);    // rows of the sequence
-            uint8_t* base = ring + kv.slot * kSlotBytes;
-            bool found = false;
-            for (int x = t; x < 1024; x += 64) {
-              const int r = (x >> 3) & (C::kVRows - 1);
-              if (r < lo) continue;
-              uint4* at = reinterpret_cast<uint4*>(base + x * 16);
-              if (r >= hi) {
-                *at = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              uint4 w = *at;
-              uint32_t* e = &w.x;
-              bool bad = false;
-              constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+            uint8_t* base = ring + at.place<C::kSlots>(i) * kSlotBytes;
+            // (the slot's 64-column groups, one after the other)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((e[k] & kExp) == kExp) {
-                  e[k] &= 0xffff0000u;
-                  bad = true;
-                }
-                if ((e[k] & (kExp << 16)) == kExp << 16) {
-                  e[k] &= 0xffffu;
-                  bad = true;
-                }
-              }
-              if (bad) {
-                *at = w;
-                found = true;
-              }
-            }
-            if (found) sy.mark[mark % kMarks] = mark;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) sl::mbar_arrive(&sy.clean[kv.slot]);
+            for (int c = 0; c < kVDim / 64; ++c)
+              found |= clean_rows<kBf16>(base + c * C::kVRows * 128, lo, hi, C::kVRows, lane);
           }
-          kv.step<C::kSlots>();
+          if (found) sy.mark[mark % kMarks] = mark;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) sl::mbar_arrive(&sy.clean[at.bar()]);
         }
+        at.step<C::kSlots>(C::kVSlots);
       }
     }
   }
@@ -1091,6 +1187,7 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   p.split = r.split;
   p.rows_cap = r.rows_cap;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.lag = (bf16 ? kLagBf16 : kLagF16) / p.scale_log2;
   p.status = static_cast<int32_t*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
   p.part_ml = reinterpret_cast<float2*>(p.part + 2 * r.grid * r.rows_cap * a.v_dim);
