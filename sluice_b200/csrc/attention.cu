@@ -457,35 +457,42 @@ struct Tiles {
 
 // Rows [lo, rows) of a value group (128-byte rows in shared memory, any
 // swizzle): those from hi on are zeroed, and values that are not finite in
-// the others. Whether there were any.
+// the others. Whether there were any. One warp; the look is cheap and its
+// loads run ahead (an exponent of all ones carries into the sign's place when
+// one is added to it), the repair is rare.
 template <bool kBf16>
 __device__ __forceinline__ bool clean_rows(uint8_t* base, int lo, int hi, int rows, int lane) {
-  constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
-  bool found = false;
-#pragma unroll 4
-  for (int x = lo * 8 + lane; x < hi * 8; x += 32) {
-    uint4* at = reinterpret_cast<uint4*>(base + x * 16);
-    uint4 w = *at;
-    uint32_t* e = &w.x;
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if ((e[k] & kExp) == kExp) {
-        e[k] &= 0xffff0000u;
-        bad = true;
-      }
-      if ((e[k] & (kExp << 16)) == kExp << 16) {
-        e[k] &= 0xffffu;
-        bad = true;
-      }
-    }
-    if (bad) {
-      *at = w;
-      found = true;
-    }
-  }
+  constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t kOne = kBf16 ? 0x00800080u : 0x04000400u;
   for (int x = max(lo, hi) * 8 + lane; x < rows * 8; x += 32)
     *reinterpret_cast<uint4*>(base + x * 16) = make_uint4(0, 0, 0, 0);
+  bool found = false;
+  // 32 rows a turn, eight loads of a lane in flight
+  for (int x0 = lo * 8; x0 < hi * 8; x0 += 256) {
+    uint4 w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = x0 + 32 * i + lane;
+      // (past the last row: row lo once more)
+      w[i] = *reinterpret_cast<const uint4*>(base + (x < hi * 8 ? x : lo * 8 + (lane & 7)) * 16);
+    }
+    uint32_t carry = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      carry |= ((w[i].x & kExp) + kOne) | ((w[i].y & kExp) + kOne) | ((w[i].z & kExp) + kOne) |
+               ((w[i].w & kExp) + kOne);
+    if (!__any_sync(0xffffffffu, carry & 0x80008000u)) continue;
+    found = true;
+    for (int x = x0 + lane; x < min(hi * 8, x0 + 256); x += 32) {
+      uint32_t* e = reinterpret_cast<uint32_t*>(base + x * 16);
+      for (int k = 0; k < 4; ++k) {
+        uint32_t v = e[k];
+        if ((v & kExp & 0xffffu) == (kExp & 0xffffu)) v &= 0xffff0000u;
+        if ((v & kExp & 0xffff0000u) == (kExp & 0xffff0000u)) v &= 0xffffu;
+        e[k] = v;
+      }
+    }
+  }
   return found;
 }
 
