@@ -20,12 +20,12 @@ namespace {
 // CTAs that updates it in place (plan_range_kernel then writes it).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxRequests = 8192;
-constexpr int kPlanChunk = 512;  // consecutive rows that a warp fills
+constexpr int kPlanChunk = 128;  // consecutive rows that a warp fills in a turn, four a lane
 
 struct PlanArgs {
   const int32_t* context;
   const int32_t* fresh;
-  int B, bs, width, N;
+  int B, bs, shift, width, N;  // shift: log2 of bs, -1 where it is no power of two
   int64_t T, Tk;
   int32_t* table;
   int64_t ld_table;
@@ -46,6 +46,16 @@ struct Lengths {
   bool invalid, refused;
 };
 
+// x / block size of x >= 0, and the blocks that x rows take
+__device__ __forceinline__ int block_index(const PlanArgs& a, int x) {
+  return a.shift >= 0 ? x >> a.shift
+                      : static_cast<int>(static_cast<unsigned>(x) / static_cast<unsigned>(a.bs));
+}
+__device__ __forceinline__ int blocks_of(const PlanArgs& a, int x) {
+  const unsigned up = static_cast<unsigned>(x) + static_cast<unsigned>(a.bs) - 1u;
+  return static_cast<int>(a.shift >= 0 ? up >> a.shift : up / static_cast<unsigned>(a.bs));
+}
+
 // One request's lengths, made safe: negative ones count as zero, and a
 // request that does not fit its table row takes nothing.
 __device__ __forceinline__ Lengths plan_lengths(const PlanArgs& a, int r) {
@@ -56,12 +66,15 @@ __device__ __forceinline__ Lengths plan_lengths(const PlanArgs& a, int r) {
   l.context = max(l.context, 0);
   l.fresh = max(l.fresh, 0);
   const int64_t total = static_cast<int64_t>(l.context) + l.fresh;
-  const int64_t held = (static_cast<int64_t>(l.context) + a.bs - 1) / a.bs;
-  const int64_t need = (total + a.bs - 1) / a.bs;
-  l.refused = need > a.width;
-  l.invalid |= held > a.width;
-  l.held = static_cast<int>(held);
-  l.take = l.refused ? 0 : static_cast<int>(need - held);
+  // (a total past 31 bits fits no table row: more blocks than it has entries,
+  // or entries past its memory)
+  const bool huge = total > 0x7fffffff;
+  const int held = blocks_of(a, l.context);
+  const int need = huge ? held : blocks_of(a, static_cast<int>(total));
+  l.refused = need > a.width || huge;
+  l.invalid |= held > a.width || huge;
+  l.held = held;
+  l.take = l.refused ? 0 : need - held;
   return l;
 }
 
@@ -162,48 +175,55 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   const int gwarp = (blockIdx.x * blockDim.x + tid) >> 5, nwarps = (gridDim.x * blockDim.x) >> 5;
   // the i-th free block: head and i are at most the ring's size
   const int64_t ring_at = head % a.N;
-  auto new_block = [&](int i) -> int {
+  auto new_block = [&](int i) -> const int32_t* {
     int64_t at = ring_at + i;
     if (at >= a.N) at -= a.N;
-    return a.free_blocks[at];
+    return a.free_blocks + at;
   };
-  auto block_of = [&](int r, int held, int o, int blk) -> int {
-    if (blk < held) return blk < a.width ? a.table[static_cast<int64_t>(r) * a.ld_table + blk] : -1;
-    if (o < 0) return -1;
+  // where the cache block of a row is found (nullptr: the row has none)
+  auto block_at = [&](int r, int context, int pos) -> const int32_t* {
+    const int blk = block_index(a, pos), held = blocks_of(a, context), o = off[r];
+    // a refused request's new rows have no slot, even inside its last block
+    if (o < 0 && pos >= context) return nullptr;
+    if (blk < held) return blk < a.width ? a.table + r * a.ld_table + blk : nullptr;
     return new_block(o + (blk - held));
   };
-  auto slot_of = [&](int r, int context, int pos) -> int64_t {
-    const unsigned blk = static_cast<unsigned>(pos) / static_cast<unsigned>(a.bs);
-    const int held = static_cast<int>((static_cast<int64_t>(context) + a.bs - 1) / a.bs);
-    const int o = off[r];
-    // a refused request's new rows have no slot, even inside its last block
-    const int b = o < 0 && pos >= context ? -1 : block_of(r, held, o, static_cast<int>(blk));
-    return b < 0 ? -1 : static_cast<int64_t>(b) * a.bs + (pos - static_cast<int>(blk) * a.bs);
-  };
-  // rows of a packed batch, kPlanChunk consecutive ones per warp and turn
+  // rows of a packed batch, kPlanChunk consecutive ones per warp and turn: a
+  // lane's four are looked up together, so that their loads overlap
   auto fill = [&](const int* cu, int64_t rows, bool all_rows) {
     const int used = cu[a.B];
     for (int64_t c0 = static_cast<int64_t>(gwarp) * kPlanChunk; c0 < rows;
          c0 += static_cast<int64_t>(nwarps) * kPlanChunk) {
-      const int64_t c1 = min(rows, c0 + kPlanChunk);
       int lo = 0, hi = 0;
       if (c0 < used) {
         lo = find_request(cu, static_cast<int>(c0), 0, a.B - 1);
-        hi = find_request(cu, static_cast<int>(min(c1, static_cast<int64_t>(used)) - 1), lo, a.B - 1);
+        const int64_t last = min(c0 + kPlanChunk, min(rows, static_cast<int64_t>(used))) - 1;
+        hi = find_request(cu, static_cast<int>(last), lo, a.B - 1);
       }
-      for (int64_t t = c0 + lane; t < c1; t += 32) {
-        int64_t slot = -1, pos = -1;
-        if (t < used) {
+      constexpr int kEach = kPlanChunk / 32;
+      int pos[kEach], block[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int64_t t = c0 + lane + 32 * i;
+        pos[i] = block[i] = -1;
+        if (t < rows && t < used) {
           const int r = find_request(cu, static_cast<int>(t), lo, hi);
           const int context = (cu_total[r + 1] - cu_total[r]) - (cu_new[r + 1] - cu_new[r]);
-          const int p = static_cast<int>(t) - cu[r] + (all_rows ? 0 : context);
-          pos = p;
-          slot = slot_of(r, context, p);
+          pos[i] = static_cast<int>(t) - cu[r] + (all_rows ? 0 : context);
+          const int32_t* at = block_at(r, context, pos[i]);
+          if (at != nullptr) block[i] = *at;
         }
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int64_t t = c0 + lane + 32 * i;
+        if (t >= rows) continue;
+        const int64_t slot = block[i] < 0 ? -1
+            : static_cast<int64_t>(block[i]) * a.bs + (pos[i] - block_index(a, pos[i]) * a.bs);
         if (all_rows) {
           a.kv_slots[t] = slot;
         } else {
-          a.positions[t] = pos;
+          a.positions[t] = pos[i];
           a.slots[t] = slot;
         }
       }
@@ -218,7 +238,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
     const Lengths l = plan_lengths(a, r);
     if (o < 0 || l.take == 0) continue;
     int32_t* row = a.table + static_cast<int64_t>(r) * a.ld_table + l.held;
-    for (int i = lane; i < l.take; i += 32) row[i] = new_block(o + i);
+    for (int i = lane; i < l.take; i += 32) row[i] = *new_block(o + i);
   }
   if (blockIdx.x == 0) {
     // offsets that a reader may follow: never past the rows that were filled
@@ -272,6 +292,7 @@ struct RotArgs {
   const double* turns;  // [rot / 2] turns per position
   float factor;
   int T, rot, per_cta, rot_units;
+  float inv_items;      // 1 / units of a token, of all its heads
   RotTensor t[2];
 };
 
@@ -301,8 +322,11 @@ struct alignas(sizeof(E) * V) RotVec {
 // columns and the V columns rot / 2 further (half: V pairs). V elements are
 // one load: 16 bytes where the sizes, strides and addresses allow it.
 template <typename E, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
-  extern __shared__ float2 cs[];  // [per_cta][rot / 2] (cos, sin) * factor
+__global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(RotArgs a) {
+  // (cos, sin) * factor of each token, [pair within a unit][unit]: lanes of
+  // neighbouring units read neighbouring words
+  extern __shared__ float2 cs[];
+  constexpr int kPairs = kInterleaved ? V / 2 : V;  // of a unit
   __shared__ int s_skip[32];
   using Vec = RotVec<E, V>;
   sl::pdl_wait();
@@ -310,29 +334,21 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
   const int half = a.rot >> 1;
   const int t0 = blockIdx.x * a.per_cta;
   const int nt = min(a.per_cta, a.T - t0);
-  for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
-    const int t = i / half, j = i - t * half;
-    const int64_t p = a.positions[t0 + t];
-    const double turns = static_cast<double>(p) * a.turns[j];
-    float s, c;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c * a.factor, s * a.factor);
-    if (j == 0) s_skip[t] = p < 0;
-  }
-  __syncthreads();
   const int nq = a.t[0].heads * a.t[0].units, n = nq + a.t[1].heads * a.t[1].units;
-  constexpr int U = 4;  // items in flight per thread
-  for (int i0 = threadIdx.x; i0 < nt * n; i0 += blockDim.x * U) {
-    Vec lo[U], hi[U];
-    E* dst[U];
-    int pair[U];  // first pair's place in cs, -1: copied
-    bool live[U];
+  constexpr int U = kInterleaved ? 4 : 2;  // items in flight per thread
+  Vec lo[U], hi[U];
+  E* dst[U];
+  int pair[U];   // first pair's place in cs, -1: not rotated
+  int token[U];  // -1: no item
+  auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * blockDim.x;
-      live[u] = i < nt * n;
-      if (!live[u]) continue;
-      const int t = i / n, w = i - t * n;
+      const int i = i0 + u * kRotThreads;
+      token[u] = -1;
+      if (i >= nt * n) continue;
+      // i / n (exact: a CTA of several tokens has at most 2^12 items)
+      const int t = a.per_cta == 1 ? 0 : static_cast<int>((i + 0.5f) * a.inv_items);
+      const int w = i - t * n;
       const RotTensor& x = w < nq ? a.t[0] : a.t[1];
       const int idx = w < nq ? w : w - nq;
       const int head = x.units == 1 ? idx
@@ -341,7 +357,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
       int col;
       if (unit < a.rot_units) {
         col = x.offset + unit * V;
-        pair[u] = s_skip[t] ? -2 : t * half + (kInterleaved ? unit * (V / 2) : unit * V);
+        pair[u] = t * half + unit;
       } else {
         // columns that are not rotated: those before the rotated ones, then
         // those behind them
@@ -349,19 +365,34 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
         col = c < x.offset ? c : c + a.rot;
         pair[u] = -1;
       }
+      token[u] = t;
       const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
       dst[u] = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
       lo[u] = *reinterpret_cast<const Vec*>(src);
-      if (!kInterleaved && unit < a.rot_units) hi[u] = *reinterpret_cast<const Vec*>(src + half);
+      if (!kInterleaved && pair[u] >= 0) hi[u] = *reinterpret_cast<const Vec*>(src + half);
     }
+  };
+  // the first rows are on their way while the angles are formed
+  load(threadIdx.x);
+  for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
+    const int t = i / half, j = i - t * half;
+    const int64_t p = a.positions[t0 + t];
+    const double turns = static_cast<double>(p) * a.turns[j];
+    float s, c;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+    cs[t * half + j % kPairs * a.rot_units + j / kPairs] = make_float2(c * a.factor, s * a.factor);
+    if (j == 0) s_skip[t] = p < 0;
+  }
+  __syncthreads();
+  for (int i0 = threadIdx.x;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!live[u]) continue;
-      if (pair[u] >= 0) {
+      if (token[u] < 0) continue;
+      if (pair[u] >= 0 && !s_skip[token[u]]) {
         if constexpr (kInterleaved) {
 #pragma unroll
           for (int k = 0; k < V / 2; ++k) {
-            const float2 c = cs[pair[u] + k];
+            const float2 c = cs[pair[u] + k * a.rot_units];
             const float x0 = to_f(lo[u].e[2 * k]), x1 = to_f(lo[u].e[2 * k + 1]);
             lo[u].e[2 * k] = from_f<E>(x0 * c.x - x1 * c.y);
             lo[u].e[2 * k + 1] = from_f<E>(x1 * c.x + x0 * c.y);
@@ -369,7 +400,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            const float2 c = cs[pair[u] + k];
+            const float2 c = cs[pair[u] + k * a.rot_units];
             const float x0 = to_f(lo[u].e[k]), x1 = to_f(hi[u].e[k]);
             lo[u].e[k] = from_f<E>(x0 * c.x - x1 * c.y);
             hi[u].e[k] = from_f<E>(x1 * c.x + x0 * c.y);
@@ -377,8 +408,11 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotArgs a) {
         }
       }
       *reinterpret_cast<Vec*>(dst[u]) = lo[u];
-      if (!kInterleaved && pair[u] != -1) *reinterpret_cast<Vec*>(dst[u] + half) = hi[u];
+      if (!kInterleaved && pair[u] >= 0) *reinterpret_cast<Vec*>(dst[u] + half) = hi[u];
     }
+    i0 += U * kRotThreads;
+    if (i0 >= nt * n) break;
+    load(i0);
   }
 }
 
@@ -414,12 +448,17 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
   if (!context_lens || !new_lens || !block_table || !free_blocks || !free_range ||
       !free_range_out || !cu_new || !cu_total || !status || (T > 0 && (!positions || !slots)))
     return SL_ERR_INVALID;
-  PlanArgs a = {context_lens, new_lens, B, block_size, table_width, num_free_slots, T, Tk,
+  int shift = -1;
+  if ((block_size & (block_size - 1)) == 0)
+    for (shift = 0; (1 << shift) < block_size;) ++shift;
+  PlanArgs a = {context_lens, new_lens, B, block_size, shift, table_width, num_free_slots, T, Tk,
                 block_table, ld_table, free_blocks, free_range, free_range_out, cu_new, cu_total,
                 positions, slots, Tk > 0 ? kv_slots : nullptr, status, 1};
-  // one CTA for what it fills in about two turns of its warps, else a CTA per
-  // as much, at most one per SM
-  const int64_t rows = T + Tk, per_cta = 2 * kPlanChunk * (kPlanThreads / 32);
+  // a CTA per turn of its warps, at most one per SM; a small batch in a small
+  // CTA, whose scan has fewer warps to wait for
+  const int64_t rows = T + Tk;
+  const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;
+  const int64_t per_cta = kPlanChunk * (threads / 32);
   int64_t grid = (rows + per_cta - 1) / per_cta;
   const int sms = sl_device_sm_count();
   if (sms <= 0) return SL_ERR_CUDA;
@@ -433,7 +472,7 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
                                       sizeof(int) * (3 * kPlanMaxRequests + 2), smem_set));
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   SL_CUDA_TRY(sl::launch(plan_kv_blocks_kernel, dim3(static_cast<unsigned>(grid)),
-                         dim3(kPlanThreads), smem, st, a));
+                         dim3(threads), smem, st, a));
   if (!a.write_range)
     SL_CUDA_TRY(sl::launch(plan_range_kernel, dim3(1), dim3(1), 0, st, free_range_out,
                            static_cast<const int32_t*>(status)));
@@ -515,6 +554,7 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
   if (sms <= 0) return SL_ERR_CUDA;
   while (per > 1 && (T + per - 1) / per < 4 * sms) per >>= 1;
   a.per_cta = per;
+  a.inv_items = 1.f / static_cast<float>(items);
   const dim3 grid((T + per - 1) / per);
   const size_t smem = static_cast<size_t>(per) * (rot / 2) * sizeof(float2);
   if (smem > 48 * 1024) return SL_ERR_UNSUPPORTED;

@@ -16,6 +16,7 @@ never synchronise, so they can be captured in a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -24,22 +25,35 @@ import torch
 from . import _lib
 from ._lib import check, lib, ptr
 
+# the current stream's handle without the object around it (a few microseconds
+# a call; the same value as torch.cuda.current_stream(device).cuda_stream)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16,
            torch.float32: _lib.DTYPE_FP32}
 
 
-def _same_device(first: torch.Tensor, **others) -> torch.device:
-    """The CUDA device of ``first``, which every other tensor is on too."""
+def _device_index(first: torch.Tensor, *others) -> int:
+    """The index of the CUDA device of ``first``, which every other tensor is
+    on too."""
     if not first.is_cuda:
         raise ValueError("sluice_b200 ops take CUDA tensors")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
-    return first.device
+    dev = first.get_device()
+    for t in others:
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise ValueError(f"a tensor is on {t.device}, expected {first.device}")
+    return dev
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(dev: int, name: str, *args) -> None:
+    """``name`` of the library with ``args`` and the current stream of device
+    ``dev``, which is made the current one where it is not."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == dev:
+        check(fn(*args, _raw_stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _raw_stream(dev)), name)
 
 
 def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, length: int | None = None) -> None:
@@ -105,32 +119,32 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     _vector("new_lens", new_lens, torch.int32, B)
     _vector("free_blocks", free_blocks, torch.int32)
     _vector("free_range", free_range, torch.int64, 2)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 \
-            or block_table.shape[0] != B:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+            block_table.stride(1) != 1 or block_table.shape[0] != B:
         raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows")
-    if B > 1 and block_table.stride(0) < block_table.shape[1]:
+    width = block_table.shape[1]
+    ld = block_table.stride(0) if B > 1 else width
+    if ld < width:
         raise ValueError("block_table's rows overlap")
     if free_range_out is None:
         free_range_out = free_range
-    _vector("free_range_out", free_range_out, torch.int64, 2)
+    else:
+        _vector("free_range_out", free_range_out, torch.int64, 2)
     if num_tokens < 0 or num_kv_tokens < 0:
         raise ValueError("num_tokens and num_kv_tokens are counts")
-    dev = _same_device(context_lens, new_lens=new_lens, block_table=block_table,
-                       free_blocks=free_blocks, free_range=free_range,
-                       free_range_out=free_range_out)
-    with torch.cuda.device(dev):
-        # (the two vectors of a size from one allocation)
-        cu = torch.empty(2, B + 1, dtype=torch.int32, device=dev)
-        rows = torch.empty(2, num_tokens, dtype=torch.int64, device=dev)
-        kv = torch.empty(num_kv_tokens, dtype=torch.int64, device=dev) if num_kv_tokens else None
-        status = torch.empty(2, dtype=torch.int32, device=dev)
-        check(lib().sl_plan_kv_blocks(
-            ptr(context_lens), ptr(new_lens), B, int(block_size), ptr(block_table),
-            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
-            ptr(free_blocks), free_blocks.numel(), ptr(free_range), ptr(free_range_out),
-            num_tokens, num_kv_tokens, ptr(cu[0]), ptr(cu[1]), ptr(rows[0]), ptr(rows[1]),
-            ptr(kv), ptr(status), _stream(dev)), "sl_plan_kv_blocks")
-    return KvPlan(cu[0], cu[1], rows[0], rows[1], kv, status)
+    dev = _device_index(context_lens, new_lens, block_table, free_blocks, free_range,
+                        free_range_out)
+    # one allocation for the 64-bit outputs, one for the others
+    rows = context_lens.new_empty(2 * num_tokens + num_kv_tokens, dtype=torch.int64)
+    small = context_lens.new_empty(2 * B + 4)
+    r, c = rows.data_ptr(), small.data_ptr()
+    _call(dev, "sl_plan_kv_blocks", ptr(context_lens), ptr(new_lens), B, int(block_size),
+          ptr(block_table), ld, width, ptr(free_blocks), free_blocks.numel(), ptr(free_range),
+          ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
+          r + 8 * num_tokens, r + 16 * num_tokens if num_kv_tokens else None, c + 8 * (B + 1))
+    positions, slots, kv = rows.split_with_sizes([num_tokens, num_tokens, num_kv_tokens])
+    cu_new, cu_total, status = small.split_with_sizes([B + 1, B + 1, 2])
+    return KvPlan(cu_new, cu_total, positions, slots, kv if num_kv_tokens else None, status)
 
 
 # ------------------------------------------------------------------- rotary
@@ -210,22 +224,18 @@ class Rotary:
         self.turns = (freqs / (2 * math.pi)).to(device)
 
     def _part(self, name: str, x: torch.Tensor, out: torch.Tensor | None, offset: int, T: int):
-        if x.dim() != 3 or x.shape[0] != T:
-            raise ValueError(f"{name} must be [{T}, heads, dim], got {tuple(x.shape)}")
-        if not 0 <= offset <= x.shape[2] - self.rotary_dim:
-            raise ValueError(f"{name}'s columns [{offset}, {offset + self.rotary_dim}) are not "
-                             f"within its {x.shape[2]}")
+        """(the call's description of one tensor, its output, its input)."""
         in_place = out is x
-        # pairs are read as two elements at once, so they start on even ones
-        odd = self.interleaved and any(s % 2 for s, n in zip(x.stride()[:2], x.shape) if n > 1) \
-            or self.interleaved and x.data_ptr() % (2 * x.element_size())
-        if x.shape[2] > 1 and x.stride(2) != 1 or odd:
+        copied, x_strides = _rotary_input(name, x.shape, x.stride(), offset, T, self.rotary_dim,
+                                          self.interleaved)
+        if copied or (self.interleaved and x.data_ptr() % (2 * x.element_size())):
             if in_place:
                 raise ValueError(f"{name} cannot be rotated in place: its columns must be "
                                  "contiguous and its pairs aligned")
-            x = x.contiguous().clone() if x.is_contiguous() else x.contiguous()
+            x = x.clone(memory_format=torch.contiguous_format)
+            x_strides = x.stride()
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = x.new_empty(x.shape)
         elif not in_place:
             if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
                 raise ValueError(f"out_{name} must match {name}'s shape, type and device")
@@ -235,12 +245,12 @@ class Rotary:
             if not same and _ranges_meet(x, out):
                 raise ValueError(f"out_{name} overlaps {name}; pass {name} itself to rotate it "
                                  "in place")
-        if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        y_strides = out.stride()
+        if 0 in y_strides and any(s == 0 and n > 1 for s, n in zip(y_strides, out.shape)):
             raise ValueError(f"out_{name} has rows that share memory")
-        part = _lib.RotaryPart(ptr(x), ptr(out), x.stride(0), x.stride(1), out.stride(0),
-                               out.stride(1), x.shape[1], x.shape[2], offset)
-        # (x: a copy made above has to outlive the launch)
-        return part, out, x
+        _, heads, dim = x.shape
+        return _lib.RotaryPart(x.data_ptr(), out.data_ptr(), x_strides[0], x_strides[1],
+                               y_strides[0], y_strides[1], heads, dim, offset), out, x
 
     def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None,
                  *, q_offset: int = 0, k_offset: int = 0, out_q: torch.Tensor | None = None,
@@ -251,24 +261,34 @@ class Rotary:
         without ``k``), new tensors or ``out_q`` / ``out_k``; passing ``q``
         itself as ``out_q`` rotates in place. Rows at negative positions
         (padding) keep their values."""
-        if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+        dtype = _DTYPES.get(q.dtype)
+        if dtype is None or (k is not None and k.dtype != q.dtype):
             raise ValueError("q and k must share one of bfloat16, float16, float32")
         T = positions.numel()
         _vector("positions", positions, torch.int64)
         if k is None and out_k is not None:
             raise ValueError("out_k without k")
-        pq, out_q, _keep_q = self._part("q", q, out_q, q_offset, T)
-        pk, _keep_k = None, None
+        pq, out_q, q = self._part("q", q, out_q, q_offset, T)
+        pk = None
         if k is not None:
-            pk, out_k, _keep_k = self._part("k", k, out_k, k_offset, T)
-        dev = _same_device(q, positions=positions, k=k, out_q=out_q, out_k=out_k,
-                           turns=self.turns)
-        with torch.cuda.device(dev):
-            check(lib().sl_rotary(ptr(positions), ptr(self.turns), T, self.rotary_dim,
-                                  int(self.interleaved), float(self.factor), _DTYPES[q.dtype],
-                                  ctypes.byref(pq), ctypes.byref(pk) if pk is not None else None,
-                                  _stream(dev)), "sl_rotary")
+            pk, out_k, k = self._part("k", k, out_k, k_offset, T)
+        _call(_device_index(q, positions, k, self.turns), "sl_rotary", ptr(positions),
+              ptr(self.turns), T, self.rotary_dim, self.interleaved, self.factor, dtype,
+              ctypes.byref(pq), None if pk is None else ctypes.byref(pk))
         return out_q if k is None else (out_q, out_k)
+
+
+@functools.lru_cache(maxsize=512)
+def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int, interleaved: bool):
+    """(whether the input has to be copied first, its strides), by its layout."""
+    if len(shape) != 3 or shape[0] != T:
+        raise ValueError(f"{name} must be [{T}, heads, dim], got {tuple(shape)}")
+    if not 0 <= offset <= shape[2] - rot:
+        raise ValueError(f"{name}'s columns [{offset}, {offset + rot}) are not within its "
+                         f"{shape[2]}")
+    # pairs are read as two elements at once, so they start on even ones
+    odd = interleaved and any(s % 2 for s, n in zip(strides[:2], shape) if n > 1)
+    return (shape[2] > 1 and strides[2] != 1) or odd, strides
 
 
 def _ranges_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -285,22 +305,76 @@ def _ranges_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _tiled(t: torch.Tensor) -> torch.Tensor:
     """``t`` in a layout the kernel's tile loads take: contiguous columns,
     strides in multiples of 16 bytes, a 16-byte aligned address."""
-    ok = t.data_ptr() % 16 == 0 and (t.shape[-1] == 1 or t.stride(-1) == 1) and \
-        all(s % 8 == 0 and s > 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
-    if ok:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 or not _tile_strides(t.shape, t.stride()):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
-def _strides(t: torch.Tensor) -> list[int]:
+@functools.lru_cache(maxsize=512)
+def _tile_strides(shape, strides) -> bool:
+    return (shape[-1] <= 1 or strides[-1] == 1) and \
+        all(s % 8 == 0 and s > 0 for s, n in zip(strides[:-1], shape) if n > 1)
+
+
+def _strides(shape, strides) -> list[int]:
     """Strides of all but the last dimension; a dimension of one entry is
     given the extent of what is inside it."""
     s = []
-    inner = t.shape[-1]
-    for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    inner = shape[-1]
+    for n, st in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         s.append(st if n > 1 else inner)
         inner = max(inner, s[-1] * n)
     return s[::-1]
+
+
+@functools.lru_cache(maxsize=512)
+def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
+    """The call's description by its tensors' layouts, each (shape, strides)
+    (``k_shared`` None; ``out`` None: a new one), without the addresses."""
+    if len(q[0]) != 3 or len(k[0]) != 3 or len(v[0]) != 3:
+        raise ValueError("q, k and v are [tokens, heads, dim]")
+    Tq, heads, dim = q[0]
+    Tk, kv_heads, own = k[0]
+    v_dim = v[0][2]
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"prompt_attention takes bfloat16 or float16, got {dtype}")
+    if v[0][:2] != k[0][:2]:
+        raise ValueError(f"k {tuple(k[0])} and v {tuple(v[0])} differ in tokens or heads")
+    shared = 0
+    if k_shared is not None:
+        if len(k_shared[0]) != 2 or k_shared[0][0] != Tk:
+            raise ValueError(f"k_shared must be [{Tk}, columns], got {tuple(k_shared[0])}")
+        shared = k_shared[0][1]
+    if own + shared != dim:
+        raise ValueError(f"q has {dim} columns per head, k {own} + {shared}")
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
+    if nq < 1 or nk != nq:
+        raise ValueError(f"cu_q has {nq} entries and cu_k {nk}: both have one per sequence and "
+                         "one more")
+    if out is None:
+        out = ((Tq, heads, v_dim), (heads * v_dim, v_dim, 1))
+    elif tuple(out[0]) != (Tq, heads, v_dim):
+        raise ValueError(f"out must be [{Tq}, {heads}, {v_dim}], got {tuple(out[0])}")
+    elif out[1][2] != 1 or any(s % 8 or s <= 0 for s, n in zip(out[1][:2], out[0]) if n > 1):
+        raise ValueError("out needs contiguous columns and strides in multiples of 8 elements")
+    a = _lib.AttentionArgs()
+    a.q_token, a.q_head = _strides(*q)
+    a.k_token, a.k_head = _strides(*k)
+    a.v_token, a.v_head = _strides(*v)
+    a.out_token, a.out_head = _strides(*out)
+    if shared:
+        a.k_shared_token, = _strides(*k_shared)
+    a.Tq, a.Tk, a.B = Tq, Tk, nq - 1
+    a.heads, a.kv_heads, a.dim, a.v_dim, a.shared_dim = heads, kv_heads, dim, v_dim, shared
+    a.dtype = _DTYPES[dtype]
+    a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    return a
+
+
+def _workspace_bytes(a) -> int:
+    return max(256, lib().sl_prompt_attention_workspace_bytes(a.B, a.Tq, a.Tk, a.heads,
+                                                              a.kv_heads, a.v_dim))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -321,66 +395,40 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     that sees no key gets zeros; rows of ``q`` outside every sequence leave
     ``out`` as it was there (a new ``out`` is not initialised).
     """
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
-        raise ValueError("q, k and v are [tokens, heads, dim]")
-    Tq, heads, dim = q.shape
-    Tk, kv_heads, own = k.shape
-    v_dim = v.shape[2]
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"prompt_attention takes bfloat16 or float16, got {q.dtype}")
     for name, t in (("k", k), ("v", v), ("k_shared", k_shared), ("out", out)):
         if t is not None and t.dtype != q.dtype:
             raise ValueError(f"{name} is {t.dtype}, q is {q.dtype}")
-    if v.shape[:2] != k.shape[:2]:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ in tokens or heads")
-    shared = 0
+    q, k, v = _tiled(q), _tiled(k), _tiled(v)
     if k_shared is not None:
-        if k_shared.dim() != 2 or k_shared.shape[0] != Tk:
-            raise ValueError(f"k_shared must be [{Tk}, columns], got {tuple(k_shared.shape)}")
-        shared = k_shared.shape[1]
-    if own + shared != dim:
-        raise ValueError(f"q has {dim} columns per head, k {own} + {shared}")
-    if heads == 0 or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
-    B = cu_q.numel() - 1
+        k_shared = _tiled(k_shared)
     _vector("cu_q", cu_q, torch.int32)
-    _vector("cu_k", cu_k, torch.int32, B + 1)
-    if B < 0:
-        raise ValueError("cu_q needs at least one entry")
+    _vector("cu_k", cu_k, torch.int32)
+    a = _lib.AttentionArgs.from_buffer_copy(_attention_layout(
+        (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),
+        None if k_shared is None else (k_shared.shape, k_shared.stride()),
+        None if out is None else (out.shape, out.stride()), q.dtype, cu_q.numel(), cu_k.numel(),
+        scale))
     if out is None:
-        out = torch.empty(Tq, heads, v_dim, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (Tq, heads, v_dim):
-        raise ValueError(f"out must be [{Tq}, {heads}, {v_dim}], got {tuple(out.shape)}")
-    elif out.data_ptr() % 16 or out.stride(2) != 1 or any(
-            s % 8 or s <= 0 for s, n in zip(out.stride()[:2], out.shape) if n > 1):
-        raise ValueError("out needs contiguous columns, strides in multiples of 8 elements and "
-                         "a 16-byte aligned address")
+        out = q.new_empty(a.Tq, a.heads, a.v_dim)
+    elif out.data_ptr() % 16:
+        raise ValueError("out needs a 16-byte aligned address")
     elif any(_ranges_meet(out, t) for t in (q, k, v, k_shared) if t is not None):
         raise ValueError("out overlaps an input")
-    dev = _same_device(q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, k_shared=k_shared, out=out)
-    if B == 0 or Tq == 0:
+    dev = _device_index(q, k, v, cu_q, cu_k, k_shared, out)
+    if a.B == 0 or a.Tq == 0:
         return out
-    with torch.cuda.device(dev):
-        q, k, v = _tiled(q), _tiled(k), _tiled(v)
-        a = _lib.AttentionArgs()
-        a.q, a.k, a.v, a.out = ptr(q), ptr(k), ptr(v), ptr(out)
-        a.q_token, a.q_head = _strides(q)
-        a.k_token, a.k_head = _strides(k)
-        a.v_token, a.v_head = _strides(v)
-        a.out_token, a.out_head = _strides(out)
-        if shared:
-            k_shared = _tiled(k_shared)
-            a.k_shared = ptr(k_shared)
-            a.k_shared_token, = _strides(k_shared)
-        a.cu_q, a.cu_k = ptr(cu_q), ptr(cu_k)
-        a.Tq, a.Tk, a.B = Tq, Tk, B
-        a.heads, a.kv_heads, a.dim, a.v_dim, a.shared_dim = heads, kv_heads, dim, v_dim, shared
-        a.dtype = _DTYPES[q.dtype]
-        a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-        n = lib().sl_prompt_attention_workspace_bytes(B, Tq, Tk, heads, kv_heads, v_dim)
-        workspace = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
-        check(lib().sl_prompt_attention(ctypes.byref(a), ptr(workspace), workspace.numel(),
-                                        _stream(dev)), "sl_prompt_attention")
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    if a.shared_dim:
+        a.k_shared = k_shared.data_ptr()
+    # (the size goes by the device's SMs: asked for with it current)
+    if torch.cuda.current_device() == dev:
+        n = _workspace_bytes(a)
+    else:
+        with torch.cuda.device(dev):
+            n = _workspace_bytes(a)
+    workspace = q.new_empty(n, dtype=torch.uint8)
+    _call(dev, "sl_prompt_attention", ctypes.byref(a), workspace.data_ptr(), n)
     prompt_attention.last_workspace = workspace
     return out
 
