@@ -558,8 +558,8 @@ int sl_rotary(const int64_t* positions, const double* turns, int T, int rot, int
  * Strides in elements, last dimension contiguous, multiples of 8; addresses
  * 16-byte aligned. bf16 or fp16; (dim, v_dim) one of (64, 64), (128, 128),
  * (192, 128); shared_dim 0 or, at dim 192, 64; at most 128 heads per key
- * head. The workspace (sl_prompt_attention_workspace_bytes) starts with a
- * status word: SL_OK, or SL_ERR_TIMEOUT when a bounded wait ran out. */
+ * head. The workspace (sl_prompt_attention_workspace_bytes, 32-byte aligned)
+ * starts with a status word: SL_OK, or SL_ERR_TIMEOUT when a bounded wait ran out. */
 typedef struct {
   const void *q, *k, *v, *k_shared;
   void* out;

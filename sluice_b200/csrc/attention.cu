@@ -39,10 +39,11 @@ constexpr int kCoarse = 256;         // entries of the work table
 constexpr int kBars = 16;            // barriers of tiles in flight
 // How far (in powers of 2) a row's maximum may lag behind its scores: bf16
 // weights have the exponents of the 32-bit sums, fp16 ones end at 2^16.
-constexpr float kLagBf16 = 32.f, kLagF16 = 8.f;
+constexpr float kLagBf16 = 32.f, kLagF16 = 12.f;
 // registers a thread: 168 at launch, then shared out between the softmax warps
 // and the others (256 x 208 + 128 x 88 = 384 x 168)
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kCubic = 0;             // pairs of each 8 whose exponential is the cubic
 constexpr int kMarks = 16;           // items that the value guards may be ahead by
 
 struct Params {
@@ -55,6 +56,7 @@ struct Params {
   int64_t v_token, v_head;
   int B, Tq, Tk, heads, kv_heads, group, half_tokens;  // tokens of a half: 128 / group
   int shared;                        // the last 64 key columns come from ks
+  int wide;                          // the output's rows are 32-byte aligned
   int grid;                          // CTAs
   int split;                         // 1: equal shares of all key tiles per CTA
   int rows_cap;                      // rows of a partial result
@@ -170,6 +172,34 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of a pair without the special-function unit, for x from -125 (below: as
+// -125) to 127: x = n + f, n the nearest whole number (found by adding and
+// taking off 1.5 * 2^23, whose low mantissa bits then hold n), a cubic in f
+// that is nowhere off by more than 7.5e-5 of 2^f on [-1/2, 1/2] (the minimax
+// one in the relative error, by Remez' exchange), and n added to its exponent.
+// 7.5e-5 is a fifty-second of a bf16 half step, a sixth of an fp16 one. What
+// should be zero is 2^-125 against weights of 2^-32 at least in their sum.
+__device__ __forceinline__ float2 ex2_cubic(float2 x) {
+  const float2 big = make_float2(12582912.f, 12582912.f);
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 t = __fadd2_rn(x, big);
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 y = __ffma2_rn(f, make_float2(0.05517167f, 0.05517167f),
+                        make_float2(0.24261113f, 0.24261113f));
+  y = __ffma2_rn(y, f, make_float2(0.69326097f, 0.69326097f));
+  y = __ffma2_rn(y, f, make_float2(0.99992806f, 0.99992806f));
+  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
+  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
+  return y;
+}
+// 32 bytes to a 32-byte aligned address
+__device__ __forceinline__ void store32(void* to, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // the largest of three; NaN if any is
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -591,21 +621,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         sl::tc_fence_after();
         uint32_t r[kTile];
         auto s = [&](int c) { return __uint_as_float(r[c]); };
-        auto load_scores = [&]() {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
-        };
-        float2 sum = make_float2(0.f, 0.f);
+        float2 sum;
         // Scores [c0, c0 + 64) as weights, in place and packed.
         auto weights = [&](int c0) {
           const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
 #pragma unroll
           for (int c = c0 / 2; c < c0 / 2 + 32; ++c) {
             float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
-            x.x = ex2(x.x);
-            x.y = ex2(x.y);
+            if (c % 8 < kCubic) {
+              x = ex2_cubic(x);
+            } else {
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
+            }
             sum = __fadd2_rn(sum, x);
             r[c] = pack2<kBf16>(x.x, x.y);
           }
@@ -632,52 +660,50 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           for (int i = 0; i < 4; ++i) t[i] = max2(t[i], s(32 * i + 31));
           return max2(max3(t[0], t[1], t[2]), t[3]);
         };
-        load_scores();
-        if (!(ok = take_turn())) break;
-        const bool hides = (j + 1) * kTile > lim_first;
-        bool go_on = false;
-        if (j > g.j0 && !hides) {
-          // Most tiles: weights against the maximum so far, which may lag
-          // behind this tile's by a factor 2^kLag (the sums and the weights'
-          // type hold that). The tile's own maximum is found meanwhile, and
-          // only where it is beyond that (or NaN) is the work done again.
-          const float top = row_max();
-          weights(0);
-          go_on = !__any_sync(0xffffffffu, live && !(top <= m + p.lag));
-          if (!go_on) {
-            load_scores();
-            sum = make_float2(0.f, 0.f);
-          }
-        }
-        if (!go_on) {
-          if (hides) {
+        // The weights are formed against the maximum so far, which may lag behind this tile's by a factor
+        // 2^kLag: the sums and the weights' type hold that. The tile's own
+        // maximum is found meanwhile; only where it is beyond that (or NaN)
+        // the rows move to it and the work is done again.
+        // (a score of +inf leaves no finite weights: the row is NaN, as inf - inf
+        // makes it)
+        auto no_inf = [](float x) { return x == INFINITY ? __int_as_float(0x7fffffff) : x; };
+        float top = 0.f;
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
+          if ((j + 1) * kTile > lim_first) {
             const int left = lim - j * kTile;
 #pragma unroll
             for (int c = 0; c < kTile; ++c)
               if (c >= left) r[c] = 0xff800000u;  // -inf
           }
-          float top = row_max();
-          // a score of +inf leaves no finite weights: the row is NaN, as
-          // inf - inf makes it
-          if (top == INFINITY) top = __int_as_float(0x7fffffff);
-          const float m1 = max2(m, top);
-          const bool move = live && !(m1 <= m + p.lag);
-          if (__any_sync(0xffffffffu, move)) {
-            const float corr = move ? ex2((m - m1) * p.scale_log2) : 1.f;
-            if (move) m = m1;
-            base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+          if (again) {
+            top = no_inf(top);
+            const bool move = live && !(top <= m + p.lag);
+            const float corr = move ? ex2((m - top) * p.scale_log2) : 1.f;
+            if (move) m = top;
             l *= corr;
             if (j > g.j0) {
               // the sums so far, once the products before this tile are in
               if (!(ok = wait(&sy.pv_done[h], (n_s - 1) & 1))) break;
               sl::tc_fence_after();
-              // (rare: eight columns at a time, the scores keep their registers)
 #pragma unroll 1
               for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
             }
+          } else {
+            if (j == g.j0 && live) m = no_inf(row_max());
+            if (!(ok = take_turn())) break;
           }
+          base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+          sum = make_float2(0.f, 0.f);
+          top = row_max();
           weights(0);
+          if (again || !__any_sync(0xffffffffu, live && !(top <= m + p.lag))) break;
         }
+        if (!ok) break;
         hand_over(0);
         weights(64);
         hand_over(64);
@@ -705,14 +731,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       }
       const bool repair = has && sy.mark[mark % kMarks] == mark;
       // no key seen: zeros; only keys that score -inf: 0 / 0
-      const float inv = lim == 0 ? 0.f : 1.f / l;
+      const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
       uint16_t* dst = static_cast<uint16_t*>(p.out) +
           static_cast<int64_t>(out_row) * p.out_token + static_cast<int64_t>(out_head) * p.out_head;
-#pragma unroll
-      for (int c = 0; c < kVDim / 32; ++c) {
+#pragma unroll 1
+      for (int c = 0; c < kVDim; c += 32) {
         uint32_t o[32];
         if (ran) {
-          tmem_ld32(o_at + 32 * c, o);
+          tmem_ld32(o_at + c, o);
           tmem_fence_ld(o);
         } else {
 #pragma unroll
@@ -726,36 +752,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           for (int j = ja; j < jb; ++j) {
             const uint16_t* v = static_cast<const uint16_t*>(p.vraw) +
                 static_cast<int64_t>(g.k0 + j) * p.v_token + static_cast<int64_t>(g.head) * p.v_head +
-                32 * c;
-            constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+                c;
+            constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u, kFrac = kBf16 ? 0x7fu : 0x3ffu;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const uint32_t b = v[i];
               if ((b & kExp) == kExp) {
-                const bool nan = b & (kExp == 0x7f80u ? 0x7fu : 0x3ffu);
-                const float bad = nan ? __int_as_float(0x7fffffff)
-                                      : (b & 0x8000u) ? -INFINITY : INFINITY;
+                const float bad = b & kFrac ? __int_as_float(0x7fffffff)
+                                            : (b & 0x8000u) ? -INFINITY : INFINITY;
                 o[i] = __float_as_uint(__uint_as_float(o[i]) + bad);
               }
             }
           }
         }
         if (live && whole) {
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 w;
-            uint32_t* e = &w.x;
+          for (int i = 0; i < 16; ++i)
+            w[i] = pack2<kBf16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          if (p.wide) {
+            store32(dst + c, w);
+            store32(dst + c + 16, w + 8);
+          } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              e[k] = pack2<kBf16>(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                  __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-            *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = w;
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(dst + c + 8 * i) =
+                  make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           }
         } else if (live) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(part + 32 * c + 4 * i) =
-                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) store32(part + c + 8 * i, o + 8 * i);
         }
         __syncwarp();
       }
@@ -959,13 +985,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
         if ((j + 1) * kTile > g.lim0) {
           bool found = false;
+#pragma unroll 1
           for (int i = 0; i < C::kVSlots; ++i) {
             const int key0 = j * kTile + i * C::kVRows;
             const int lo = clampi(g.lim0 - key0, 0, C::kVRows);     // rows that all see
             const int hi = clampi(g.k_len - key0, 0, C::kVRows);    // rows of the sequence
             uint8_t* base = ring + at.place<C::kSlots>(i) * kSlotBytes;
             // (the slot's 64-column groups, one after the other)
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < kVDim / 64; ++c)
               found |= clean_rows<kBf16>(base + c * C::kVRows * 128, lo, hi, C::kVRows, lane);
           }
@@ -1032,7 +1059,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(
       l = l * a + ml.y * b;
       m = m1;
     }
-    const float inv = lim == 0 ? 0.f : 1.f / l;
+    const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
     uint16_t* dst = static_cast<uint16_t*>(p.out) +
         static_cast<int64_t>(g.q0 + tok) * p.out_token +
         static_cast<int64_t>(g.head * p.group + r - token * p.group) * p.out_head + lane * kCols;
@@ -1151,7 +1178,7 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
     return SL_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
        reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.k_shared) |
-       reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+       reinterpret_cast<uintptr_t>(a.out)) & 15 || (reinterpret_cast<uintptr_t>(workspace) & 31))
     return SL_ERR_INVALID;
   if ((a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.k_shared_token |
        a.out_token | a.out_head) & 7)
@@ -1190,6 +1217,7 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
   p.shared = a.shared_dim != 0;
+  p.wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && ((a.out_token | a.out_head) & 15) == 0;
   p.grid = static_cast<int>(r.grid);
   p.split = r.split;
   p.rows_cap = r.rows_cap;
