@@ -222,13 +222,48 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return d;
 }
 
-// A bounded wait of a whole warp: its lanes run the same instructions on the
-// same word, so they agree on the outcome.
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-  const bool done = sl::mbar_wait(bar, parity);
-  __syncwarp();
-  return done;
+// A role's outlook: once a bounded wait has run out, it waits for nothing more
+// and issues nothing more, but walks its work to the end, so that the named
+// barriers, which have no limit of their own, still meet all their warps.
+struct Outlook {
+  bool ok = true;
+  // A bounded wait of a whole warp: its lanes run the same instructions on the
+  // same word, so they agree on the outcome. (Without the suspend-time hint of
+  // sl::mbar_wait: a signal takes 108 cycles instead of 137, a wait that is
+  // over already 14 instead of 49.)
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+    if (ok && !try_wait(bar, parity)) {
+      const uint64_t t0 = sl::globaltimer();
+      for (uint32_t i = 1; ok; ++i) {
+        if (try_wait(bar, parity)) break;
+        if ((i & 15u) == 0 && sl::globaltimer() - t0 > sl::kWaitLimitNs) ok = false;
+      }
+    }
+    __syncwarp();
+    return ok;
+  }
+  static __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(sl::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+  }
+};
+// Named barriers (a signal between warps takes a tenth of an mbarrier's): `n`
+// threads in all, those that wait and those that only arrive.
+__device__ __forceinline__ void bar_wait(int id, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
 }
+__device__ __forceinline__ void bar_arrive(int id, int n) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+constexpr int kBarTurn = 1;     // + 4 * half + quad: this half's turn; 64 threads
+constexpr int kBarWeights = 9;  // + 2 * half + part: weights are there; 160 threads
 
 // --------------------------------------------------------------------- work
 // One stretch of an item's key tiles: [j0, j1) of n.
@@ -457,7 +492,7 @@ struct Cfg {
 
 struct Sync {
   uint64_t full[kBars], empty[kBars], clean[kBars];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2], o_free[2], drain[2], turn[2][4];
+  uint64_t q_full[2], q_empty[2], s_full[2], pv_done[2], o_free[2], drain[2];
   uint32_t tmem;
   int mark[kMarks];
   int warp_sum[kCoarse / 32];
@@ -548,12 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       sl::mbar_init(&sy.q_full[h], 1);
       sl::mbar_init(&sy.q_empty[h], 1);
       sl::mbar_init(&sy.s_full[h], 1);
-      sl::mbar_init(&sy.p_full[h][0], 4);
-      sl::mbar_init(&sy.p_full[h][1], 4);
       sl::mbar_init(&sy.pv_done[h], 1);
       sl::mbar_init(&sy.o_free[h], 4);
       sl::mbar_init(&sy.drain[h], 1);
-      for (int i = 0; i < 4; ++i) sl::mbar_init(&sy.turn[h][i], 1);
     }
     for (int i = 0; i < kMarks; ++i) sy.mark[i] = -1;
     sl::fence_barrier_init();
@@ -574,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
   const uint32_t tmem = sy.tmem;
   const uint32_t s_col[2] = {tmem, tmem + kTile};
   const uint32_t o_col[2] = {tmem + 2 * kTile, tmem + 2 * kTile + kVDim};
-  bool ok = true;
+  Outlook out;
   Walk walk;
   walk.start(p, sy.cum);
   Seg g;
@@ -591,22 +623,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     int n_s = 0, n_item = 0;  // key tiles so far; items with keys so far
     // The warps of the two halves that share a scheduler take turns at the
     // exponentials, so that one half's run while the other's products do.
-    int n_turn = h - 1;
-    auto take_turn = [&]() -> bool {
-      const int t = n_turn++;
-      return t < 0 || wait(&sy.turn[h][warp & 3], t & 1);
+    const int quad = warp & 3;
+    bool free_turn = h == 0;
+    auto take_turn = [&]() {
+      if (!free_turn) bar_wait(kBarTurn + 4 * h + quad, 64);
+      free_turn = false;
     };
     auto pass_turn = [&]() {
-      if (lane == 0) sl::mbar_arrive(&sy.turn[h ^ 1][warp & 3]);
+      __syncwarp();
+      bar_arrive(kBarTurn + 4 * (h ^ 1) + quad, 64);
     };
-    while (ok && walk.next(p, sy.cum, per, g)) {
+    while (walk.next(p, sy.cum, per, g)) {
       const int first = g.tok + h * p.half_tokens;
       const int j1 = min(g.j1, g.nh[h]);
       const bool has = g.j0 < g.j1;
       const int mark = has ? n_item++ : -1;
       if (first >= g.q_len) {
-        for (int j = g.j0; j < g.j1 && ok; ++j) {
-          ok = take_turn();
+        for (int j = g.j0; j < g.j1; ++j) {
+          take_turn();
           pass_turn();
         }
         continue;
@@ -617,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       const int lim_first = clampi(first + 1 + g.k_len - g.q_len, 0, g.k_len);
       float m = -INFINITY, l = 0.f, base = 0.f;  // base: -m in powers of 2
       for (int j = g.j0; j < j1; ++j) {
-        if (!(ok = wait(&sy.s_full[h], n_s & 1))) break;
+        out.wait(&sy.s_full[h], n_s & 1);
         sl::tc_fence_after();
         uint32_t r[kTile];
         auto s = [&](int c) { return __uint_as_float(r[c]); };
@@ -646,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           tmem_wait_st();
           sl::tc_fence_before();
           __syncwarp();
-          if (lane == 0) sl::mbar_arrive(&sy.p_full[h][c0 != 0]);
+          bar_arrive(kBarWeights + 2 * h + (c0 != 0), 160);
         };
         auto row_max = [&]() {
           float t[4];
@@ -688,14 +722,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
             l *= corr;
             if (j > g.j0) {
               // the sums so far, once the products before this tile are in
-              if (!(ok = wait(&sy.pv_done[h], (n_s - 1) & 1))) break;
+              out.wait(&sy.pv_done[h], (n_s - 1) & 1);
               sl::tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
             }
           } else {
             if (j == g.j0 && live) m = no_inf(row_max());
-            if (!(ok = take_turn())) break;
+            take_turn();
           }
           base = m == -INFINITY ? 0.f : -m * p.scale_log2;
           sum = make_float2(0.f, 0.f);
@@ -703,7 +737,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           weights(0);
           if (again || !__any_sync(0xffffffffu, live && !(top <= m + p.lag))) break;
         }
-        if (!ok) break;
         hand_over(0);
         weights(64);
         hand_over(64);
@@ -711,11 +744,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         ++n_s;
       }
       // (the other half may have more tiles)
-      for (int j = max(g.j0, j1); j < g.j1 && ok; ++j) {
-        ok = take_turn();
+      for (int j = max(g.j0, j1); j < g.j1; ++j) {
+        take_turn();
         pass_turn();
       }
-      if (!ok) break;
       // ------------------------------------------------------- output
       const bool whole = g.j0 == 0 && g.j1 == g.n;
       const int out_row = g.q0 + tok, out_head = g.head * p.group + in_group;
@@ -726,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           make_float2(m, l);
       const bool ran = g.j0 < j1;
       if (ran) {
-        if (!(ok = wait(&sy.pv_done[h], (n_s - 1) & 1))) break;
+        out.wait(&sy.pv_done[h], (n_s - 1) & 1);
         sl::tc_fence_after();
       }
       const bool repair = has && sy.mark[mark % kMarks] == mark;
@@ -791,6 +823,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         if (lane == 0) sl::mbar_arrive(&sy.o_free[h]);
       }
     }
+    // (the last turn that half 1 passed on)
+    if (h == 0) take_turn();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   }
@@ -804,12 +838,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     const uint32_t s_d = s_col[h], o_d = o_col[h];
     const bool leader = sl::elect_one();
     Tiles at;
-    int n_s = 0, n_o = 0;
+    int n_o = 0;
     uint32_t clean_phase = 0;
     // S = Q K^T with the key tile at `at`, or (this half sees none of it) let
     // it go
     auto key_tile = [&](bool mine) {
-      if (leader) {
+      if (leader && out.ok) {
         if (mine) {
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c) {
@@ -827,38 +861,38 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       __syncwarp();
       at.step<C::kSlots>(C::kChunks);
     };
-    while (ok && walk.next(p, sy.cum, per, g)) {
+    while (walk.next(p, sy.cum, per, g)) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const int j1 = min(g.j1, g.nh[h]);
       const bool any = g.j0 < j1;
-      if (any && !(ok = wait(&sy.q_full[h], n_o & 1))) break;
-      if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+      if (any) out.wait(&sy.q_full[h], n_o & 1);
+      out.wait(&sy.full[at.bar()], at.phase());
       sl::tc_fence_after();
       key_tile(any);
       for (int j = g.j0; j < g.j1; ++j) {
         const bool mine = j < j1;
         // this tile's values and the next one's keys are here, as a rule, long
         // before the weights
-        if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        out.wait(&sy.full[at.bar()], at.phase());
         const int v_bar = at.bar();
         if ((j + 1) * kTile > g.lim0) {
           // cleaned by the guard first
-          if (!(ok = wait(&sy.clean[v_bar], (clean_phase >> v_bar) & 1))) break;
+          out.wait(&sy.clean[v_bar], (clean_phase >> v_bar) & 1);
           clean_phase ^= 1u << v_bar;
         }
         const int v_slot0 = at.place<C::kSlots>(0), v_slot1 = at.place<C::kSlots>(1);
         at.step<C::kSlots>(C::kVSlots);
         const bool next = j + 1 < g.j1;
-        if (next && !(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        if (next) out.wait(&sy.full[at.bar()], at.phase());
         if (mine) {
-          if (j == g.j0 && n_o > 0 && !(ok = wait(&sy.o_free[h], (n_o - 1) & 1))) break;
+          if (j == g.j0 && n_o > 0) out.wait(&sy.o_free[h], (n_o - 1) & 1);
           // O += P V in two halves of 64 keys, as the weights come in
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (!(ok = wait(&sy.p_full[h][half], n_s & 1))) break;
+            bar_wait(kBarWeights + 2 * h + half, 160);
             sl::tc_fence_after();
-            if (leader) {
+            if (leader && out.ok) {
               const uint32_t v_lo = kRowMajorLo<C::kVRows> + ring_lo +
                   (C::kVSlots == 2 ? (half ? v_slot1 : v_slot0) * (kSlotBytes >> 4)
                                    : v_slot0 * (kSlotBytes >> 4) + half * 512);
@@ -868,29 +902,27 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
                         j > g.j0 || half + k > 0);
             }
           }
-          if (!ok) break;
-          ++n_s;
-          if (leader) {
+          if (leader && out.ok) {
             sl::umma_commit(&sy.empty[v_bar]);
             sl::umma_commit(&sy.pv_done[h]);
           }
-        } else if (leader) {
+        } else if (leader && out.ok) {
           sl::mbar_arrive(&sy.empty[v_bar]);
         }
         __syncwarp();
         if (next) key_tile(j + 1 < j1);
       }
-      if (!ok) break;
       if (any) {
         ++n_o;
-        if (leader) sl::umma_commit(&sy.q_empty[h]);
+        if (leader && out.ok) sl::umma_commit(&sy.q_empty[h]);
         __syncwarp();
       }
     }
     // everything issued is in before TMEM and the barriers go
     if (leader) sl::umma_commit(&sy.drain[h]);
     __syncwarp();
-    ok = wait(&sy.drain[h], 0) && ok;
+    Outlook last;
+    out.ok &= last.wait(&sy.drain[h], 0);
   } else if (warp == 9) {
     // ------------------------------------------------------------ loads
     Tiles at;
@@ -902,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.half_tokens) * 128;
     auto claim = [&](int slots) -> bool {
       while (room < slots) {
-        if (!wait(&sy.empty[oldest % kBars], (oldest / kBars) & 1)) return false;
+        if (!out.wait(&sy.empty[oldest % kBars], (oldest / kBars) & 1)) return false;
         room += oldest_v ? C::kVSlots : C::kChunks;
         oldest_v = !oldest_v;
         ++oldest;
@@ -911,12 +943,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       if (lane == 0) sl::mbar_arrive_expect_tx(&sy.full[at.bar()], slots * kSlotBytes);
       return true;
     };
-    while (ok && walk.next(p, sy.cum, per, g)) {
+    while (walk.next(p, sy.cum, per, g)) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
       auto load_q = [&](int h) -> bool {
         if (g.j0 >= min(g.j1, g.nh[h])) return true;
-        if (n_q[h] > 0 && !wait(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
+        if (n_q[h] > 0 && !out.wait(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
         ++n_q[h];
         if (lane == 0) {
           sl::mbar_arrive_expect_tx(&sy.q_full[h], q_bytes * C::kChunks);
@@ -955,16 +987,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         at.step<C::kSlots>(C::kVSlots);
         return true;
       };
-      ok = load_q(0) && load_k(g.j0) && load_q(1);
-      for (int j = g.j0; j < g.j1 && ok; ++j)
-        ok = load_v(j) && (j + 1 >= g.j1 || load_k(j + 1));
+      bool go = load_q(0) && load_k(g.j0) && load_q(1);
+      for (int j = g.j0; j < g.j1 && go; ++j)
+        go = load_v(j) && (j + 1 >= g.j1 || load_k(j + 1));
+      if (!go) break;
     }
-    if (!ok) {
+    if (!out.ok) {
+      Outlook last;
       // what was asked for lands before the buffers go
       for (; oldest < at.n; ++oldest)
-        (void)wait(&sy.full[oldest % kBars], (oldest / kBars) & 1);
+        last.wait(&sy.full[oldest % kBars], (oldest / kBars) & 1);
       for (int h = 0; h < 2; ++h)
-        if (n_q[h] > 0) (void)wait(&sy.q_full[h], (n_q[h] - 1) & 1);
+        if (n_q[h] > 0) last.wait(&sy.q_full[h], (n_q[h] - 1) & 1);
     }
   } else if (warp == 10) {
     // ------------------------------------------------------- value guard
@@ -974,7 +1008,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     // does see are marked for the output to put back.
     Tiles at;
     int n_item = 0;
-    while (ok && walk.next(p, sy.cum, per, g)) {
+    while (walk.next(p, sy.cum, per, g)) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const int mark = n_item++;
@@ -982,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         at.step<C::kSlots>(C::kChunks);
         // every value tile is waited for, cleaned or not: a wait names a use
         // of its barrier by the parity alone
-        if (!(ok = wait(&sy.full[at.bar()], at.phase()))) break;
+        if (!out.wait(&sy.full[at.bar()], at.phase())) break;
         if ((j + 1) * kTile > g.lim0) {
           bool found = false;
 #pragma unroll 1
@@ -1003,9 +1037,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         }
         at.step<C::kSlots>(C::kVSlots);
       }
+      if (!out.ok) break;
     }
   }
-  if (!ok && lane == 0) atomicMax(p.status, SL_ERR_TIMEOUT);
+  if (!out.ok && lane == 0) atomicMax(p.status, SL_ERR_TIMEOUT);
   sl::tc_fence_before();
   __syncthreads();
   sl::tc_fence_after();
