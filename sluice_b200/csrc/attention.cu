@@ -43,8 +43,16 @@ constexpr float kLagBf16 = 32.f, kLagF16 = 12.f;
 // registers a thread: 168 at launch, then shared out between the softmax warps
 // and the others (256 x 208 + 128 x 88 = 384 x 168)
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
-constexpr int kCubic = 0;             // pairs of each 8 whose exponential is the cubic
+constexpr int kReaders = 11;          // warps that follow the stretches
+constexpr int kSegs = 4;              // stretches looked up ahead
+constexpr int kItemUnits = 3;         // what starting and ending an item costs, in key tiles
 constexpr int kMarks = 16;           // items that the value guards may be ahead by
+
+// What the join needs to know of a CTA's first stretch: the item it is a later
+// part of (unit0 < 0: of none).
+struct Later {
+  int unit0, q0, q_len, k_len, tok, head, pad[2];
+};
 
 struct Params {
   CUtensorMap q, k, v, ks;
@@ -64,6 +72,7 @@ struct Params {
   float lag;                         // how far the maximum may lag behind, in scores
   float* part;                       // [2 * grid][rows_cap][v_dim]
   float2* part_ml;                   // [2 * grid][rows_cap] (maximum, sum)
+  Later* later;                      // [grid]
   int32_t* status;
 };
 
@@ -173,28 +182,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x of a pair without the special-function unit, for x from -125 (below: as
-// -125) to 127: x = n + f, n the nearest whole number (found by adding and
-// taking off 1.5 * 2^23, whose low mantissa bits then hold n), a cubic in f
-// that is nowhere off by more than 7.5e-5 of 2^f on [-1/2, 1/2] (the minimax
-// one in the relative error, by Remez' exchange), and n added to its exponent.
-// 7.5e-5 is a fifty-second of a bf16 half step, a sixth of an fp16 one. What
-// should be zero is 2^-125 against weights of 2^-32 at least in their sum.
-__device__ __forceinline__ float2 ex2_cubic(float2 x) {
-  const float2 big = make_float2(12582912.f, 12582912.f);
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
-  const float2 t = __fadd2_rn(x, big);
-  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-  float2 y = __ffma2_rn(f, make_float2(0.05517167f, 0.05517167f),
-                        make_float2(0.24261113f, 0.24261113f));
-  y = __ffma2_rn(y, f, make_float2(0.69326097f, 0.69326097f));
-  y = __ffma2_rn(y, f, make_float2(0.99992806f, 0.99992806f));
-  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
-  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
-  return y;
-}
 // 32 bytes to a 32-byte aligned address
 __device__ __forceinline__ void store32(void* to, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(r[0]),
@@ -297,7 +284,7 @@ __device__ __forceinline__ int seen(const Seq& s, int tok) {
 __device__ __forceinline__ int tiles_of(const Params& p, const Seq& s) {
   return (s.q_len + 2 * p.half_tokens - 1) / (2 * p.half_tokens);
 }
-// key tiles of item `t` (at least one unit of work, to write its rows)
+// key tiles of item `t`
 __device__ __forceinline__ int reach(const Params& p, const Seq& s, int t) {
   const int last = min(s.q_len, (t + 1) * 2 * p.half_tokens) - 1;
   return (seen(s, last) + kTile - 1) / kTile;
@@ -306,7 +293,7 @@ __device__ __forceinline__ int64_t work_of(const Params& p, const Seq& s) {
   const int nt = tiles_of(p, s);
   if (!p.split) return nt;
   int64_t w = 0;
-  for (int t = 0; t < nt; ++t) w += max(1, reach(p, s, t));
+  for (int t = 0; t < nt; ++t) w += kItemUnits + reach(p, s, t);
   return w;
 }
 
@@ -403,7 +390,7 @@ __device__ __forceinline__ void uniform(Seg& g) {
 //   whole items: the longest first, dealt out in turns that go back and forth;
 //   split: an equal run of key tiles, item after item.
 struct Walk {
-  int total, at, end, round;
+  int total, at, end, round, unit0;  // unit0: the first unit of the last stretch's item
 
   __device__ void start(const Params& p, const int* cum) {
     total = units(p, cum);
@@ -417,8 +404,10 @@ struct Walk {
     return static_cast<int>(min(static_cast<int64_t>(cum[kCoarse]) * p.kv_heads,
                                 static_cast<int64_t>(1 << 30)));
   }
+  // where CTA c's share begins: equal ones, the first with one unit more
   __device__ static int share(const Params& p, int total, int c) {
-    return static_cast<int>(static_cast<int64_t>(total) * c / p.grid);
+    const int each = total / p.grid;
+    return each * c + min(c, total - each * p.grid);
   }
   __device__ bool next(const Params& p, const int* cum, int per, Seg& g) {
     if (!p.split) {
@@ -436,16 +425,22 @@ struct Walk {
       g.j1 = g.n;
       return true;
     }
-    if (at >= end) return false;
-    int j, n;
-    locate(p, cum, per, at, g, j, n);
-    g.j0 = j;
-    g.j1 = min(n, j + end - at);
-    at += g.j1 - j;
-    g.j1 = min(g.j1, g.n);  // (an item without keys is one empty unit)
-    return true;
+    // (a share may begin or end within an item's first units, which are no key
+    // tiles: that stretch is empty, and skipped unless it is the whole item)
+    while (at < end) {
+      int j, n;
+      locate(p, cum, per, at, g, j, n);
+      unit0 = at - j;
+      const int to = min(n, j + end - at);
+      at += to - j;
+      g.j0 = max(0, j - kItemUnits);
+      g.j1 = max(0, to - kItemUnits);
+      if (g.j0 < g.j1 || (g.n == 0 && to == n)) return true;
+    }
+    return false;
   }
-  // The item that unit u falls in: u is its key tile j of n units.
+  // The item that unit u falls in, u its j-th of n units: kItemUnits for the
+  // item itself, then one for each key tile.
   __device__ static void locate(const Params& p, const int* cum, int per, int u, Seg& g, int& j,
                                 int& n) {
     const int lane = threadIdx.x & 31;
@@ -456,7 +451,7 @@ struct Walk {
     const int nt = tiles_of(p, s);
     for (int t0 = 0;; t0 += 32) {
       const int t = t0 + lane;
-      const int own = t < nt ? max(1, reach(p, s, t)) * p.kv_heads : 0;
+      const int own = t < nt ? (kItemUnits + reach(p, s, t)) * p.kv_heads : 0;
       int v = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -473,7 +468,7 @@ struct Walk {
       r -= __shfl_sync(0xffffffffu, v, 31);
     }
     fill_seg(p, s, g);
-    n = max(1, g.n);
+    n = kItemUnits + g.n;
     g.head = min(r / n, p.kv_heads - 1);
     j = r - r / n * n;
   }
@@ -493,6 +488,8 @@ struct Cfg {
 struct Sync {
   uint64_t full[kBars], empty[kBars], clean[kBars];
   uint64_t q_full[2], q_empty[2], s_full[2], pv_done[2], o_free[2], drain[2];
+  uint64_t seg_full[kSegs], seg_empty[kSegs];
+  Seg seg[kSegs];
   uint32_t tmem;
   int mark[kMarks];
   int warp_sum[kCoarse / 32];
@@ -588,6 +585,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       sl::mbar_init(&sy.drain[h], 1);
     }
     for (int i = 0; i < kMarks; ++i) sy.mark[i] = -1;
+    for (int i = 0; i < kSegs; ++i) {
+      sl::mbar_init(&sy.seg_full[i], 1);
+      sl::mbar_init(&sy.seg_empty[i], kReaders);
+    }
     sl::fence_barrier_init();
   }
   if (warp == 8) sl::tmem_alloc(&sy.tmem, 512);
@@ -607,9 +608,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
   const uint32_t s_col[2] = {tmem, tmem + kTile};
   const uint32_t o_col[2] = {tmem + 2 * kTile, tmem + 2 * kTile + kVDim};
   Outlook out;
-  Walk walk;
-  walk.start(p, sy.cum);
+  // The stretches of this CTA's share, as the guard's warp publishes them, one
+  // ahead of its own work: looking one up takes microseconds. (Waited for even
+  // when something else has run out, so that all roles stop at the same one.)
   Seg g;
+  int n_seg = 0;
+  auto next_seg = [&]() -> bool {
+    const int i = n_seg % kSegs;
+    Outlook here;
+    if (!here.wait(&sy.seg_full[i], (n_seg / kSegs) & 1)) return out.ok = false;
+    g = sy.seg[i];
+    ++n_seg;
+    __syncwarp();
+    if (lane == 0) sl::mbar_arrive(&sy.seg_empty[i]);
+    return g.seq >= 0;
+  };
 
   if (warp < 8) {
     // ---------------------------------------------------------- softmax
@@ -633,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       __syncwarp();
       bar_arrive(kBarTurn + 4 * (h ^ 1) + quad, 64);
     };
-    while (walk.next(p, sy.cum, per, g)) {
+    while (next_seg()) {
       const int first = g.tok + h * p.half_tokens;
       const int j1 = min(g.j1, g.nh[h]);
       const bool has = g.j0 < g.j1;
@@ -662,12 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
 #pragma unroll
           for (int c = c0 / 2; c < c0 / 2 + 32; ++c) {
             float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
-            if (c % 8 < kCubic) {
-              x = ex2_cubic(x);
-            } else {
-              x.x = ex2(x.x);
-              x.y = ex2(x.y);
-            }
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
             sum = __fadd2_rn(sum, x);
             r[c] = pack2<kBf16>(x.x, x.y);
           }
@@ -861,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       __syncwarp();
       at.step<C::kSlots>(C::kChunks);
     };
-    while (walk.next(p, sy.cum, per, g)) {
+    while (next_seg()) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const int j1 = min(g.j1, g.nh[h]);
@@ -943,7 +952,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       if (lane == 0) sl::mbar_arrive_expect_tx(&sy.full[at.bar()], slots * kSlotBytes);
       return true;
     };
-    while (walk.next(p, sy.cum, per, g)) {
+    while (next_seg()) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
       auto load_q = [&](int h) -> bool {
@@ -1008,7 +1017,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     // does see are marked for the output to put back.
     Tiles at;
     int n_item = 0;
-    while (walk.next(p, sy.cum, per, g)) {
+    Walk walk;
+    walk.start(p, sy.cum);
+    Seg ahead;
+    auto publish = [&]() {
+      const int i = n_seg % kSegs;
+      if (n_seg >= kSegs && !out.wait(&sy.seg_empty[i], (n_seg / kSegs - 1) & 1)) return;
+      if (!walk.next(p, sy.cum, per, ahead)) ahead.seq = -1;
+      if (lane == 0) {
+        sy.seg[i] = ahead;
+        sl::mbar_arrive(&sy.seg_full[i]);
+      }
+      __syncwarp();
+      ++n_seg;
+    };
+    publish();
+    if (p.split && lane == 0) {
+      const bool later = ahead.seq >= 0 && ahead.j0 > 0;
+      Later w = {};
+      w.unit0 = later ? walk.unit0 : -1;
+      w.q0 = ahead.q0;
+      w.q_len = ahead.q_len;
+      w.k_len = ahead.k_len;
+      w.tok = ahead.tok;
+      w.head = ahead.head;
+      p.later[blockIdx.x] = w;
+    }
+    while (out.ok && ahead.seq >= 0) {
+      g = ahead;
+      publish();
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const int mark = n_item++;
@@ -1037,7 +1074,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         }
         at.step<C::kSlots>(C::kVSlots);
       }
-      if (!out.ok) break;
     }
   }
   if (!out.ok && lane == 0) atomicMax(p.status, SL_ERR_TIMEOUT);
@@ -1047,31 +1083,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
   if (warp == 8) sl::tmem_dealloc(tmem, 512);
 }
 
-// Joins the partial results of an item that several CTAs share. Block c looks
-// at the boundary between CTAs c and c + 1: the first boundary inside an item
-// joins all of the item's stretches, in order.
+// Joins the partial results of an item that several CTAs share. Block c is the
+// one to do it where CTA c holds an item's first stretch and CTA c + 1 a later
+// one: in the order of the stretches, whatever order they were done in.
 constexpr int kJoinThreads = 256;
 
 template <int kVDim, bool kBf16>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(
     const __grid_constant__ Params p) {
-  __shared__ int cum[kCoarse + 1], warp_sum[kCoarse / 32];
   sl::pdl_wait();
   sl::pdl_trigger();
-  const int per = (p.B + kCoarse - 1) / kCoarse;
-  build_table(p, cum, warp_sum, per);
-  const int total = Walk::units(p, cum);
   const int c = blockIdx.x;
-  const int u = Walk::share(p, total, c + 1);
-  if (u >= total) return;
-  Seg g;
-  int j, n;
-  Walk::locate(p, cum, per, u, g, j, n);
-  const int u0 = u - j;  // the item's first unit
-  // whole on this side, or joined by an earlier boundary (the same boundary,
-  // too, where a CTA's share is empty)
-  if (j == 0 || Walk::share(p, total, c) > u0 || Walk::share(p, total, c) == u) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Later g = p.later[c + 1];
+  if (g.unit0 < 0 || p.later[c].unit0 == g.unit0) return;
+  // CTAs c .. e - 1 have a stretch each
+  int e = c + 1;
+  for (;;) {
+    const int s = e + lane;
+    const unsigned same =
+        __ballot_sync(0xffffffffu, s < p.grid && p.later[min(s, p.grid - 1)].unit0 == g.unit0);
+    e += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+    if (same != 0xffffffffu) break;
+  }
   const int rows = 2 * p.half_tokens * p.group;
   constexpr int kCols = kVDim / 32;
   for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows;
@@ -1080,19 +1114,34 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(
     if (tok >= g.q_len) break;
     const int lim = clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len);
     float m = -INFINITY, l = 0.f, o[kCols] = {};
-    for (int s = c; s < p.grid && Walk::share(p, total, s) < u0 + n; ++s) {
-      if (Walk::share(p, total, s) == Walk::share(p, total, s + 1)) continue;
-      const int slot = 2 * s + (s == c && Walk::share(p, total, s) <= u0 ? 1 : 0);
-      const int64_t at = static_cast<int64_t>(slot) * p.rows_cap + r;
-      const float2 ml = p.part_ml[at];
-      const float m1 = max2(m, ml.x);
-      const float base = m1 == -INFINITY ? 0.f : m1;
-      const float a = ex2((m - base) * p.scale_log2), b = ex2((ml.x - base) * p.scale_log2);
-      const float* src = p.part + at * kVDim + lane * kCols;
+    // a lane per stretch for the maxima and sums, then all lanes for the
+    // outputs, whose loads do not wait for one another
+    for (int s0 = c; s0 < e; s0 += 32) {
+      const int s = s0 + lane;
+      const bool has = s < e;
+      const int64_t at = has ? (2 * static_cast<int64_t>(s) + (s == c)) * p.rows_cap + r : 0;
+      const float2 ml = has ? p.part_ml[at] : make_float2(-INFINITY, 0.f);
+      float top = max2(m, ml.x);
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) o[i] = o[i] * a + src[i] * b;
-      l = l * a + ml.y * b;
-      m = m1;
+      for (int x = 16; x > 0; x >>= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float mine = ex2((ml.x - base) * p.scale_log2), old = ex2((m - base) * p.scale_log2);
+      float sum = has ? ml.y * mine : 0.f;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l = l * old + sum;
+      m = top;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] *= old;
+#pragma unroll 8
+      for (int k = 0; k < min(32, e - s0); ++k) {
+        const float w = __shfl_sync(0xffffffffu, mine, k);
+        const float* src = p.part +
+            ((2 * static_cast<int64_t>(s0 + k) + (s0 + k == c)) * p.rows_cap + r) * kVDim +
+            lane * kCols;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[i] = fmaf(src[i], w, o[i]);
+      }
     }
     const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
     uint16_t* dst = static_cast<uint16_t*>(p.out) +
@@ -1154,9 +1203,10 @@ Shape shape_of(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads, int sms) 
   const int64_t tokens = 2 * (kTile / group);
   const int64_t items = (Tq + B * (tokens - 1)) / tokens;
   r.items = (items < Tq ? items : Tq) * kv_heads;
-  r.units = r.items * (Tk / kTile + 2);
+  r.units = r.items * (Tk / kTile + 1 + kItemUnits);
   // few items with long key ranges: share out the key tiles instead
-  r.split = r.items < sms && Tk / B >= 8 * kTile && r.units < kMostUnits;
+  r.split = r.units < kMostUnits &&
+      ((r.items < sms && Tk / B >= 8 * kTile) || (r.items < 4 * sms && (Tk - Tq) / B >= 8 * kTile));
   r.grid = r.split ? (r.units < sms ? r.units : sms) : (r.items < sms ? r.items : sms);
   const int64_t rows = Tq * group;
   r.rows_cap = static_cast<int>(rows < 2 * kTile ? rows : 2 * kTile);
@@ -1171,7 +1221,7 @@ int launch_all(const Params& p, cudaStream_t st) {
   SL_CUDA_TRY(sl::launch(kern, dim3(p.grid), dim3(kThreads), kSmemBytes, st, p));
   if (p.split && p.grid > 1)
     SL_CUDA_TRY(sl::launch(attention_join_kernel<kVDim, kBf16>,
-                           dim3(p.grid - 1, p.rows_cap > 64 ? 4 : 1), dim3(kJoinThreads), 0, st,
+                           dim3(p.grid - 1, (p.rows_cap + 31) / 32), dim3(kJoinThreads), 0, st,
                            p));
   return SL_OK;
 }
@@ -1187,7 +1237,8 @@ extern "C" size_t sl_prompt_attention_workspace_bytes(int B, int64_t Tq, int64_t
   // (without a device: the size for this part's 148)
   const Shape r = shape_of(B, Tq, Tk, heads, kv_heads, sms > 0 ? sms : 148);
   if (!r.split) return kHeaderBytes;
-  return static_cast<size_t>(kHeaderBytes + 2 * r.grid * r.rows_cap * (4 * (int64_t)v_dim + 8));
+  return static_cast<size_t>(kHeaderBytes + r.grid * static_cast<int64_t>(sizeof(Later)) +
+                             2 * r.grid * r.rows_cap * (4 * static_cast<int64_t>(v_dim) + 8));
 }
 
 extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspace,
@@ -1259,7 +1310,8 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.lag = (bf16 ? kLagBf16 : kLagF16) / p.scale_log2;
   p.status = static_cast<int32_t*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
+  p.later = reinterpret_cast<Later*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
+  p.part = reinterpret_cast<float*>(p.later + r.grid);
   p.part_ml = reinterpret_cast<float2*>(p.part + 2 * r.grid * r.rows_cap * a.v_dim);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a.dim == 64) return bf16 ? launch_all<64, 64, true>(p, st) : launch_all<64, 64, false>(p, st);
