@@ -428,6 +428,19 @@ int sl_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, float eps,
                   int rank, int vdim, int max_len, float scale, void* out,
                   sl_stream_t stream);
 
+/* The same step over a paged cache bf16 [num_blocks, block_size, rank + rope]:
+ * position l of sequence b is row l mod block_size of block
+ * block_table[b][l / block_size] (i32, rows ld_table apart, table_width wide;
+ * sl_plan_kv_blocks fills it). The same arithmetic, in the same order.
+ * block_size a multiple of 32, max_len at most table_width * block_size. A
+ * position whose block is outside the pool is not written. */
+int sl_mla_decode_paged(const void* qkv, int ld_qkv, const void* kv_norm, float eps,
+                        const void* w_uk, const void* w_uv, const float* rope_cos_sin,
+                        const int64_t* pos, void* cache, int num_blocks, int block_size,
+                        const int32_t* block_table, int64_t ld_table, int table_width, int B,
+                        int nh, int nope, int rope, int rank, int vdim, int max_len, float scale,
+                        void* out, sl_stream_t stream);
+
 /* Not part of the reference's MoE operator surface: the residual add and
  * RMSNorm between the decoder's sublayers in this build's benchmark harness
  * (vLLM's fused add + RMSNorm, which the reference's model runs). For each of
@@ -499,7 +512,9 @@ enum {
  * ld_table apart) holds ceil(context / block_size) blocks and is given the
  * blocks that context + new tokens need, in request order, from the ring
  * free_blocks (i32 [num_free_slots]), whose free entries are the positions
- * [free_range[0], free_range[1]) modulo num_free_slots.
+ * [free_range[0], free_range[1]) modulo num_free_slots. Without a ring
+ * (free_blocks, free_range and free_range_out NULL) the table rows are
+ * complete, and nothing is taken.
  *   cu_new, cu_total  i32 [B + 1]: offsets of the new, and of all, tokens
  *   positions, slots  i64 [T]: of each new token, its position in its
  *                     sequence and its cache row block * block_size + offset

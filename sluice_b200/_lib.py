@@ -126,6 +126,8 @@ _SIGNATURES = {
     "sl_linear_small": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp]),
     "sl_mla_decode": (_i, [_vp, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                            _i, _i, _f, _vp, _vp]),
+    "sl_mla_decode_paged": (_i, [_vp, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i64, _i,
+                                 _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
     "sl_plan_kv_blocks": (_i, [_vp, _vp, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _vp, _i64, _i64,
                                _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "sl_rotary": (_i, [_vp, _vp, _i, _i, _i, _f, _i, _c.POINTER(RotaryPart),

@@ -84,12 +84,23 @@ __device__ __forceinline__ int col16(int lane, int i) {
   return i < 8 ? 8 * lane + i : 256 + 8 * lane + (i - 8);
 }
 
+// Where a sequence's cached rows are: one run of max_len rows (kPaged false),
+// or blocks of block_size rows (a multiple of kRingRows, so that a chunk lies in
+// one block) listed in the sequence's block table row. A block id outside the
+// pool reads block 0 and writes nothing (the planner has reported it).
+struct Pages {
+  const int32_t* table;
+  int64_t ld;
+  int block_size, blocks;
+};
+
+template <bool kPaged>
 __global__ void __launch_bounds__(kMlaThreads) mla_decode_kernel(
     const __nv_bfloat16* __restrict__ qkv, int ld_qkv, const __nv_bfloat16* __restrict__ kv_norm,
     float eps, const __nv_bfloat16* __restrict__ w_uk, const __nv_bfloat16* __restrict__ w_uv,
     const float2* __restrict__ rope_cs, const int64_t* __restrict__ pos,
     __nv_bfloat16* __restrict__ cache, int nh, int nope, int rope, int vdim, int max_len,
-    float scale, __nv_bfloat16* __restrict__ out) {
+    float scale, __nv_bfloat16* __restrict__ out, Pages pages) {
   extern __shared__ __align__(16) uint8_t sm_raw[];
   const int h = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -110,6 +121,14 @@ __global__ void __launch_bounds__(kMlaThreads) mla_decode_kernel(
   const int nk = (nope + kRingRows - 1) / kRingRows;
   const int nv = (vdim + kRingRows - 1) / kRingRows;
   int P = 0, nc = 0;
+  // the cache row of position l, -1 where its block is none
+  auto cache_row = [&](int l) -> int64_t {
+    if (!kPaged) return static_cast<int64_t>(b) * max_len + l;
+    const int blk = pages.table[b * pages.ld + l / pages.block_size];
+    return blk < 0 || blk >= pages.blocks
+        ? -1
+        : static_cast<int64_t>(blk) * pages.block_size + l % pages.block_size;
+  };
   auto issue = [&](int j) {
     const __nv_bfloat16* src;
     int rows;
@@ -120,7 +139,8 @@ __global__ void __launch_bounds__(kMlaThreads) mla_decode_kernel(
       row_bytes = kRank * 2;
     } else if (j < nk + nc) {
       const int c = j - nk;
-      src = cache + (static_cast<size_t>(b) * max_len + c * kRingRows) * dk;
+      const int64_t row = cache_row(c * kRingRows);
+      src = cache + static_cast<size_t>(row < 0 ? 0 : row) * dk;
       rows = min(kRingRows, P - c * kRingRows);
       row_bytes = static_cast<size_t>(dk) * 2;
     } else {
@@ -164,7 +184,16 @@ __global__ void __launch_bounds__(kMlaThreads) mla_decode_kernel(
                      : "memory");
       }
     };
-    prefetch(cache + static_cast<size_t>(b) * max_len * dk, static_cast<size_t>(P) * dk * 2);
+    if (kPaged) {
+      for (int l = 0; l < P; l += pages.block_size) {
+        const int64_t row = cache_row(l);
+        if (row >= 0)
+          prefetch(cache + static_cast<size_t>(row) * dk,
+                   static_cast<size_t>(min(pages.block_size, P - l)) * dk * 2);
+      }
+    } else {
+      prefetch(cache + static_cast<size_t>(b) * max_len * dk, static_cast<size_t>(P) * dk * 2);
+    }
     prefetch(w_uv + static_cast<size_t>(h) * vdim * kRank, static_cast<size_t>(vdim) * kRank * 2);
   }
   const __nv_bfloat16* row = qkv + static_cast<size_t>(b) * ld_qkv;
@@ -307,8 +336,9 @@ __global__ void __launch_bounds__(kMlaThreads) mla_decode_kernel(
         for (int w = 0; w < kMlaWarps; ++w) t += part[w * kRank + c];
         q[c] = sl::bf16_round(t);
       }
-      if (h == 0) {
-        __nv_bfloat16* dst = cache + (static_cast<size_t>(b) * max_len + P) * dk;
+      const int64_t new_row = h == 0 ? cache_row(P) : -1;
+      if (new_row >= 0) {
+        __nv_bfloat16* dst = cache + static_cast<size_t>(new_row) * dk;
         for (int i = tid; i < dk; i += blockDim.x) dst[i] = __float2bfloat16(kv[i]);
       }
       __syncthreads();
@@ -522,11 +552,12 @@ extern "C" int sl_add_rmsnorm(void* h, const void* delta, const void* w, float e
   return SL_OK;
 }
 
-extern "C" int sl_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, float eps,
-                             const void* w_uk, const void* w_uv, const float* rope_cos_sin,
-                             const int64_t* pos, void* cache, int B, int nh, int nope, int rope,
-                             int rank, int vdim, int max_len, float scale, void* out,
-                             sl_stream_t stream) {
+namespace {
+
+int run_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, float eps, const void* w_uk,
+                   const void* w_uv, const float* rope_cos_sin, const int64_t* pos, void* cache,
+                   int B, int nh, int nope, int rope, int rank, int vdim, int max_len, float scale,
+                   void* out, const Pages* pages, sl_stream_t stream) {
   if (B < 0 || nh <= 0 || nope <= 0 || rope <= 0 || rope % 2 || rank <= 0 || vdim <= 0 ||
       max_len <= 0 || ld_qkv < nh * (nope + rope) + rank + rope)
     return SL_ERR_INVALID;
@@ -544,9 +575,11 @@ extern "C" int sl_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, f
       sizeof(float) * (2 * static_cast<size_t>(rank + rope) + kMlaWarps * kRank + nope +
                        2 * kMlaWarps + 32) + sizeof(int) * kRingSlots;
   if (smem > 220 * 1024 || B > 65535) return SL_ERR_UNSUPPORTED;
-  static std::atomic<uint64_t> smem_set{0};
-  if (smem > 48 * 1024) SL_CUDA_TRY(sl::ensure_smem_limit(mla_decode_kernel, static_cast<int>(smem), smem_set));
-  SL_CUDA_TRY(sl::launch(mla_decode_kernel, dim3(nh, B), dim3(kMlaThreads), smem,
+  static std::atomic<uint64_t> smem_set[2];
+  auto kern = pages ? mla_decode_kernel<true> : mla_decode_kernel<false>;
+  if (smem > 48 * 1024)
+    SL_CUDA_TRY(sl::ensure_smem_limit(kern, static_cast<int>(smem), smem_set[pages ? 1 : 0]));
+  SL_CUDA_TRY(sl::launch(kern, dim3(nh, B), dim3(kMlaThreads), smem,
                          reinterpret_cast<cudaStream_t>(stream),
                          static_cast<const __nv_bfloat16*>(qkv), ld_qkv,
                          static_cast<const __nv_bfloat16*>(kv_norm), eps,
@@ -554,6 +587,34 @@ extern "C" int sl_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, f
                          static_cast<const __nv_bfloat16*>(w_uv),
                          reinterpret_cast<const float2*>(rope_cos_sin), pos,
                          static_cast<__nv_bfloat16*>(cache), nh, nope, rope, vdim, max_len, scale,
-                         static_cast<__nv_bfloat16*>(out)));
+                         static_cast<__nv_bfloat16*>(out), pages ? *pages : Pages{}));
   return SL_OK;
+}
+
+}  // namespace
+
+extern "C" int sl_mla_decode(const void* qkv, int ld_qkv, const void* kv_norm, float eps,
+                             const void* w_uk, const void* w_uv, const float* rope_cos_sin,
+                             const int64_t* pos, void* cache, int B, int nh, int nope, int rope,
+                             int rank, int vdim, int max_len, float scale, void* out,
+                             sl_stream_t stream) {
+  return run_mla_decode(qkv, ld_qkv, kv_norm, eps, w_uk, w_uv, rope_cos_sin, pos, cache, B, nh,
+                        nope, rope, rank, vdim, max_len, scale, out, nullptr, stream);
+}
+
+extern "C" int sl_mla_decode_paged(const void* qkv, int ld_qkv, const void* kv_norm, float eps,
+                                   const void* w_uk, const void* w_uv, const float* rope_cos_sin,
+                                   const int64_t* pos, void* cache, int num_blocks,
+                                   int block_size, const int32_t* block_table, int64_t ld_table,
+                                   int table_width, int B, int nh, int nope, int rope, int rank,
+                                   int vdim, int max_len, float scale, void* out,
+                                   sl_stream_t stream) {
+  if (num_blocks <= 0 || block_size <= 0 || table_width <= 0 || ld_table < table_width ||
+      max_len > static_cast<int64_t>(table_width) * block_size)
+    return SL_ERR_INVALID;
+  if (block_size % kRingRows) return SL_ERR_UNSUPPORTED;
+  if (B > 0 && !block_table) return SL_ERR_INVALID;
+  const Pages pages = {block_table, ld_table, block_size, num_blocks};
+  return run_mla_decode(qkv, ld_qkv, kv_norm, eps, w_uk, w_uv, rope_cos_sin, pos, cache, B, nh,
+                        nope, rope, rank, vdim, max_len, scale, out, &pages, stream);
 }

@@ -69,10 +69,12 @@ __device__ __forceinline__ Lengths plan_lengths(const PlanArgs& a, int r) {
   // (a total past 31 bits fits no table row: more blocks than it has entries,
   // or entries past its memory)
   const bool huge = total > 0x7fffffff;
-  const int held = blocks_of(a, l.context);
+  int held = blocks_of(a, l.context);
   const int need = huge ? held : blocks_of(a, static_cast<int>(total));
   l.refused = need > a.width || huge;
   l.invalid |= held > a.width || huge;
+  // (without a ring every block is in the table)
+  if (a.free_blocks == nullptr) held = need;
   l.held = held;
   l.take = l.refused ? 0 : need - held;
   return l;
@@ -139,8 +141,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   }
   sl::pdl_wait();
   sl::pdl_trigger();
-  int64_t head = a.range[0];
-  int64_t avail = a.range[1] - head;
+  const bool ring = a.free_blocks != nullptr;
+  int64_t head = ring ? a.range[0] : 0;
+  int64_t avail = ring ? a.range[1] - head : 0;
   const bool bad_range = avail < 0 || avail > a.N || head < 0;
   if (bad_range) head = avail = 0;
   __syncthreads();
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
 
   const int gwarp = (blockIdx.x * blockDim.x + tid) >> 5, nwarps = (gridDim.x * blockDim.x) >> 5;
   // the i-th free block: head and i are at most the ring's size
-  const int64_t ring_at = head % a.N;
+  const int64_t ring_at = ring ? head % a.N : 0;
   auto new_block = [&](int i) -> const int32_t* {
     int64_t at = ring_at + i;
     if (at >= a.N) at -= a.N;
@@ -182,7 +185,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   };
   // where the cache block of a row is found (nullptr: the row has none)
   auto block_at = [&](int r, int context, int pos) -> const int32_t* {
-    const int blk = block_index(a, pos), held = blocks_of(a, context), o = off[r];
+    const int blk = block_index(a, pos), o = off[r];
+    const int held = ring ? blocks_of(a, context) : a.width;
     // a refused request's new rows have no slot, even inside its last block
     if (o < 0 && pos >= context) return nullptr;
     if (blk < held) return blk < a.width ? a.table + r * a.ld_table + blk : nullptr;
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
                     : s_short                      ? SL_KV_PLAN_NO_BLOCKS
                                                    : SL_KV_PLAN_OK;
       a.status[1] = s_end;
-      if (a.write_range) {
+      if (ring && a.write_range) {
         const int64_t first = a.range[0], tail = a.range[1];
         a.range_out[0] = first + s_end;
         a.range_out[1] = tail;
@@ -442,11 +446,13 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
                                  int64_t* positions, int64_t* slots, int64_t* kv_slots,
                                  int32_t* status, sl_stream_t stream) {
   if (B <= 0 || block_size <= 0 || table_width <= 0 || ld_table < table_width ||
-      num_free_slots <= 0 || T < 0 || Tk < 0 || (Tk > 0 && !kv_slots))
+      T < 0 || Tk < 0 || (Tk > 0 && !kv_slots))
     return SL_ERR_INVALID;
+  const bool ring = free_blocks || free_range || free_range_out;
+  if (ring && num_free_slots <= 0) return SL_ERR_INVALID;
   if (B > kPlanMaxRequests) return SL_ERR_UNSUPPORTED;
-  if (!context_lens || !new_lens || !block_table || !free_blocks || !free_range ||
-      !free_range_out || !cu_new || !cu_total || !status || (T > 0 && (!positions || !slots)))
+  if (!context_lens || !new_lens || !block_table ||
+      (ring && (!free_blocks || !free_range || !free_range_out)) || !cu_new || !cu_total || !status || (T > 0 && (!positions || !slots)))
     return SL_ERR_INVALID;
   int shift = -1;
   if ((block_size & (block_size - 1)) == 0)
@@ -463,7 +469,7 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
   const int sms = sl_device_sm_count();
   if (sms <= 0) return SL_ERR_CUDA;
   grid = grid < 1 ? 1 : (grid > sms ? sms : grid);
-  const bool in_place = free_range_out == free_range;
+  const bool in_place = ring && free_range_out == free_range;
   a.write_range = !(in_place && grid > 1);
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(B) + 2);
   static std::atomic<uint64_t> smem_set{0};

@@ -24,8 +24,12 @@ Attention is decode-only MLA in its absorbed form over a compressed cache
 ``q_nope W_uk . c_kv + q_pe . k_pe`` over every cached position (fixed
 shapes, masked beyond the sequence's length, so a step captures in one CUDA
 graph); the output is ``softmax . c_kv`` projected through ``W_uv`` and the
-output projection. Prompt tokens are fed through the same decode step, one
-position per step. Rotary embedding: RoPE (theta 10000) on adjacent dim
+output projection. Prompts go through the same decode step, one position per
+step, or (``prefill``, on a CUDA device) whole or in chunks through the prompt
+pass (``sluice_b200.prompt``): the block planner's slot maps, rotary positions
+in place, keys and values expanded from the latents, causal attention over the
+packed sequences. The cache is one run of ``max_len`` rows per sequence, or a
+pool of blocks that the sequences share (``cache_blocks``). Rotary embedding: RoPE (theta 10000) on adjacent dim
 pairs. In the PyTorch form the causal mask is an additive bias folded into
 the score GEMM; the fused kernel reads each sequence's positions 0..P.
 """
@@ -88,12 +92,19 @@ class DecoderHarness:
     hidden states ``x`` [batch, H]."""
 
     def __init__(self, cfg: DecoderConfig, moe, batch: int, max_len: int, seed: int = 0,
-                 device="cuda", std: float = 0.02, fused_attention: bool | None = None):
+                 device="cuda", std: float = 0.02, fused_attention: bool | None = None,
+                 cache_blocks: int | None = None, block_size: int = 64):
         """``fused_attention`` (default: on a CUDA device) runs each layer's
         attention core as the library's one-launch MLA decode kernel
         (``sl_mla_decode``) and each residual add with the RMSNorm after it
         as one launch (``sl_add_rmsnorm``); otherwise, and on the host, as
-        PyTorch ops."""
+        PyTorch ops.
+
+        ``cache_blocks`` gives the sequences a shared pool of so many blocks
+        of ``block_size`` positions (a multiple of 32) per layer instead of
+        ``max_len`` rows each; they take blocks as they grow, up to
+        ``max_len`` positions, and ``reset`` returns them
+        (``check_blocks`` raises if the pool ran out)."""
         self.cfg = cfg
         self.moe = moe
         self.batch = batch
@@ -133,14 +144,34 @@ class DecoderHarness:
             self.layers.append(lw)
         L = cfg.num_layers
         # compressed cache per layer and position: [c_kv (rank) | k_pe (rope)]
-        self.cache = torch.zeros(L, batch, max_len, cfg.kv_lora_rank + cfg.qk_rope, dtype=bf,
-                                 device=dev)
+        self.paged = cache_blocks is not None
+        if self.paged:
+            if block_size <= 0 or block_size % 32 or cache_blocks <= 0:
+                raise ValueError("a paged cache needs blocks of a multiple of 32 positions")
+            rows = (cache_blocks, block_size)
+            self.block_size = block_size
+            self.block_table = torch.full((batch, -(-max_len // block_size)), -1,
+                                          dtype=torch.int32, device=dev)
+            self.free_blocks = torch.arange(cache_blocks, dtype=torch.int32, device=dev)
+            self.free_range = torch.tensor([0, cache_blocks], device=dev)
+        else:
+            # every sequence owns one block of max_len rows
+            rows = (batch, max_len)
+            self.block_size = max_len
+            self.block_table = torch.arange(batch, dtype=torch.int32, device=dev)[:, None]
+            self.free_blocks = self.free_range = None
+        self.cache = torch.zeros(L, *rows, cfg.kv_lora_rank + cfg.qk_rope, dtype=bf, device=dev)
+        self.kv_status = torch.zeros((), dtype=torch.int32, device=dev)
+        self._ones = torch.ones(batch, dtype=torch.int32, device=dev)
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.qk_rope, 2).float() / cfg.qk_rope))
         ang = torch.arange(max_len).float()[:, None] * inv[None, :]
         self.freqs = torch.polar(torch.ones_like(ang), ang).to(dev)   # complex64
         self.rope_cs = torch.view_as_real(self.freqs).contiguous()    # [max_len, r/2, 2]
         self.fused_attention = (self.device.type == "cuda") if fused_attention is None \
             else bool(fused_attention)
+        if self.paged and not self.fused_attention:
+            raise ValueError("a paged cache needs the fused attention")
+        self._rotary = None   # of the prompt pass, made with its first prompt
         self.pos = torch.zeros(batch, dtype=torch.long, device=dev)
         self.scale = 1.0 / math.sqrt(dq)
         self._ar = torch.arange(max_len, device=dev)
@@ -152,6 +183,37 @@ class DecoderHarness:
 
     def reset(self) -> None:
         self.pos.zero_()
+        if self.paged:
+            self.block_table.fill_(-1)
+            torch.arange(self.free_blocks.numel(), out=self.free_blocks)
+            self.free_range[0] = 0
+            self.free_range[1] = self.free_blocks.numel()
+        self.kv_status.zero_()
+
+    def _plan(self, context: torch.Tensor, new: torch.Tensor, tokens: int, kv_tokens: int = 0):
+        from .prompt import plan_kv_blocks
+        plan = plan_kv_blocks(context, new, self.block_table, self.free_blocks, self.free_range,
+                              self.block_size, tokens, num_kv_tokens=kv_tokens)
+        torch.maximum(self.kv_status, plan.status[0], out=self.kv_status)
+        return plan
+
+    _BLOCKS = ("block_table", "free_blocks", "free_range", "kv_status")
+
+    def save_blocks(self) -> dict:
+        """Copies of what the block planner keeps."""
+        return {n: getattr(self, n).clone() for n in self._BLOCKS if getattr(self, n) is not None}
+
+    def restore_blocks(self, saved: dict) -> None:
+        for n, t in saved.items():
+            getattr(self, n).copy_(t)
+
+    def check_blocks(self) -> None:
+        """Raise if a step since ``reset`` found no block for a position, or
+        no room below ``max_len`` (synchronises)."""
+        from .prompt import KvPlanError
+        status = int(self.kv_status.item())
+        if status:
+            raise KvPlanError(status)
 
     def _attention(self, li: int, x: torch.Tensor, mask_bias: torch.Tensor,
                    freqs: torch.Tensor) -> torch.Tensor:
@@ -162,6 +224,15 @@ class DecoderHarness:
         if self.fused_attention:
             from ._lib import check, lib, ptr
             o = torch.empty(B, nh * cfg.v_head, dtype=x.dtype, device=x.device)
+            if self.paged:
+                cache, table = self.cache[li], self.block_table
+                check(lib().sl_mla_decode_paged(
+                    ptr(qkv), qkv.shape[1], ptr(lw["kv_norm"]), cfg.rms_eps, ptr(lw["w_uk_t"]),
+                    ptr(lw["w_uv"]), ptr(self.rope_cs), ptr(self.pos), ptr(cache),
+                    cache.shape[0], self.block_size, ptr(table), table.shape[1], table.shape[1],
+                    B, nh, cfg.qk_nope, cfg.qk_rope, R, cfg.v_head, self.max_len, self.scale,
+                    ptr(o), torch.cuda.current_stream().cuda_stream), "sl_mla_decode_paged")
+                return self._linear(o, lw["wo"])
             check(lib().sl_mla_decode(ptr(qkv), qkv.shape[1], ptr(lw["kv_norm"]), cfg.rms_eps,
                                       ptr(lw["w_uk_t"]), ptr(lw["w_uv"]), ptr(self.rope_cs),
                                       ptr(self.pos), ptr(self.cache[li]), B, nh, cfg.qk_nope,
@@ -224,6 +295,8 @@ class DecoderHarness:
         the greedy next ids [batch]; the positions advance by one."""
         cfg = self.cfg
         h = self.embed[ids]
+        if self.paged:
+            self._plan(self.pos.to(torch.int32), self._ones, self.batch)
         # per step: the positions' rotations and the causal mask as an additive
         # bias over the cache (0 up to each sequence's position, -inf after)
         freqs = self.freqs[self.pos]
@@ -242,6 +315,92 @@ class DecoderHarness:
         self.pos.add_(1)
         return logits.argmax(dim=-1)
 
+    def _prompt_attention(self, li: int, x: torch.Tensor, plan, has_context: bool) -> torch.Tensor:
+        """The attention of packed prompt rows x [T, H]: their latents and
+        rotated keys go to the cache, keys and values are expanded from the
+        latents of the whole sequences (the cached beginnings included)."""
+        from .prompt import prompt_attention
+        cfg, lw = self.cfg, self.layers[li]
+        nh, R = cfg.num_heads, cfg.kv_lora_rank
+        dq = cfg.qk_nope + cfg.qk_rope
+        T = x.shape[0]
+        qkv = F.linear(x, lw["wqkv"])
+        q, k_pe = qkv[:, :nh * dq].view(T, nh, dq), qkv[:, nh * dq + R:].view(T, 1, cfg.qk_rope)
+        self._rotary(plan.positions, q, k_pe, q_offset=cfg.qk_nope, out_q=q, out_k=k_pe)
+        c = _rms(qkv[:, nh * dq:nh * dq + R], lw["kv_norm"], cfg.rms_eps)
+        rows = torch.cat([c, k_pe[:, 0]], dim=-1)
+        cache = self.cache[li].flatten(0, 1)
+        cache.index_copy_(0, plan.slots, rows)
+        if has_context:
+            rows = cache[plan.kv_slots]
+        if "w_ukv" not in lw:
+            # W_uk and W_uv of each head as one map from the latent
+            lw["w_ukv"] = torch.cat([lw["w_uk"], lw["w_uv"]], dim=1).flatten(0, 1)
+        kv = F.linear(rows[:, :R], lw["w_ukv"]).view(-1, nh, cfg.qk_nope + cfg.v_head)
+        o = prompt_attention(q, kv[..., :cfg.qk_nope], kv[..., cfg.qk_nope:], plan.cu_new,
+                             plan.cu_total, k_shared=rows[:, R:], scale=self.scale)
+        return F.linear(o.flatten(1), lw["wo"])
+
+    def prefill(self, ids: torch.Tensor, lengths: list[int],
+                context: list[int] | None = None) -> torch.Tensor:
+        """Prompts, or the next chunks of prompts, in one pass: ``ids`` [T] are
+        the sequences' tokens one after the other, ``lengths`` [batch] how many
+        each has (0: none in this pass). They continue at the sequences'
+        positions, which advance by ``lengths``. Returns the greedy next ids
+        [batch] behind each sequence's last token (-1 for a sequence without
+        tokens). ``context`` are the positions, where the caller knows them;
+        otherwise they are read back. CUDA with the fused attention only; the
+        MoE layers take the pass as one step of T rows."""
+        if not self.fused_attention:
+            raise ValueError("prefill runs on a CUDA device with the fused attention")
+        cfg, dev = self.cfg, self.device
+        if len(lengths) != self.batch or any(n < 0 for n in lengths):
+            raise ValueError(f"lengths must be {self.batch} counts")
+        T = sum(lengths)
+        if tuple(ids.shape) != (T,):
+            raise ValueError(f"ids must hold the {T} tokens of lengths, got {tuple(ids.shape)}")
+        if context is None:
+            context = self.pos.tolist()
+        elif len(context) != self.batch:
+            raise ValueError(f"context must be {self.batch} positions")
+        if any(c + n > self.max_len for c, n in zip(context, lengths)):
+            raise ValueError(f"a sequence would pass max_len {self.max_len}")
+        nxt = torch.full((self.batch,), -1, dtype=torch.long, device=dev)
+        if T == 0:
+            return nxt
+        if self._rotary is None:
+            from .prompt import Rotary
+            self._rotary = Rotary(cfg.qk_rope, base=cfg.rope_theta, interleaved=True, device=dev)
+        new = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        # sequences without tokens in this pass have no keys in it either
+        seen = [c if n else 0 for c, n in zip(context, lengths)]
+        has_context = any(seen)
+        # (kept apart until the plan is known to hold: a position without a
+        # block has no cache row to write)
+        blocks0 = self.save_blocks()
+        plan = self._plan(torch.tensor(seen, dtype=torch.int32, device=dev), new, T,
+                          T + sum(seen) if has_context else 0)
+        try:
+            plan.check()
+        except RuntimeError:
+            self.restore_blocks(blocks0)
+            raise
+        h = self.embed[ids]
+        x = self._add_norm(h, None, self.layers[0]["in_norm"])
+        for li in range(cfg.num_layers):
+            lw = self.layers[li]
+            x = self._add_norm(h, self._prompt_attention(li, x, plan, has_context),
+                               lw["post_norm"])
+            f = self._dense_ffn(li, x) if li < cfg.first_dense else \
+                self.moe(li - cfg.first_dense, x)
+            last = self.layers[li + 1]["in_norm"] if li + 1 < cfg.num_layers else self.final_norm
+            x = self._add_norm(h, f, last)
+        live = [b for b, n in enumerate(lengths) if n]
+        ends = plan.cu_new[1:].long()[live] - 1
+        nxt[live] = F.linear(x[ends], self.head).argmax(dim=-1)
+        self.pos.add_(new)
+        return nxt
+
 
 class OffloadedDecoder:
     """The decoder on this GPU with its MoE layers behind slot caches: the
@@ -250,7 +409,8 @@ class OffloadedDecoder:
     layers exchange tokens with the other ranks). A decode step replays as
     one CUDA graph that also feeds its greedy ids back as the next input."""
 
-    def __init__(self, cfg: DecoderConfig, stack, batch: int, max_len: int, seed: int = 0):
+    def __init__(self, cfg: DecoderConfig, stack, batch: int, max_len: int, seed: int = 0,
+                 cache_blocks: int | None = None, block_size: int = 64):
         self.cfg = cfg
         self.stack = stack
         self.device = stack.device
@@ -259,7 +419,8 @@ class OffloadedDecoder:
             raise ValueError(f"{len(layers)} MoE layers for a decoder with {cfg.num_moe_layers}")
         self.layers = layers          # the MoE layers (slot caches, stream timers)
         self.model = DecoderHarness(cfg, lambda li, x: layers[li](x), batch, max_len, seed,
-                                    self.device)
+                                    self.device, cache_blocks=cache_blocks,
+                                    block_size=block_size)
         self.graph = None
         self._ids = torch.zeros(batch, dtype=torch.long, device=self.device)
         self._out = None
@@ -273,12 +434,14 @@ class OffloadedDecoder:
         """Capture one decode step (after one eager warm-up step, whose
         position is then rewound)."""
         ids0 = self._ids.clone()
+        blocks0 = self.model.save_blocks()
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(s):
             self._step()
         torch.cuda.current_stream(self.device).wait_stream(s)
         self.model.pos.sub_(1)
+        self.model.restore_blocks(blocks0)
         self._ids.copy_(ids0)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
@@ -301,19 +464,33 @@ class OffloadedDecoder:
                        non_blocking=True)
         return out_host
 
+    def prefill(self, ids: torch.Tensor, lengths: list[int],
+                context: list[int] | None = None) -> torch.Tensor:
+        """Prompts, or their next chunks, in one pass
+        (``DecoderHarness.prefill``; the MoE layers' steps beyond the slot
+        envelope run in expert waves); the sequences that had tokens go on
+        from their greedy next ids. One GPU only."""
+        nxt = self.model.prefill(ids, lengths, context)
+        self._ids.copy_(torch.where(nxt >= 0, nxt, self._ids))
+        return nxt
+
     def save(self) -> dict:
-        """The sequences' state (KV caches, positions, next input ids)."""
+        """The sequences' state (KV caches and their blocks, positions, next
+        input ids)."""
         m = self.model
-        return {"cache": m.cache.clone(), "pos": m.pos.clone(), "ids": self._ids.clone()}
+        return {"cache": m.cache.clone(), "pos": m.pos.clone(), "ids": self._ids.clone(),
+                "blocks": m.save_blocks()}
 
     def restore(self, saved: dict) -> None:
         m = self.model
         m.cache.copy_(saved["cache"])
         m.pos.copy_(saved["pos"])
         self._ids.copy_(saved["ids"])
+        m.restore_blocks(saved["blocks"])
 
     def check(self) -> None:
         self.stack.check()
+        self.model.check_blocks()
 
     def stats(self) -> dict:
         return self.stack.stats()

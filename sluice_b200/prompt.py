@@ -94,8 +94,8 @@ class KvPlan(NamedTuple):
 
 
 def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
-                   block_table: torch.Tensor, free_blocks: torch.Tensor,
-                   free_range: torch.Tensor, block_size: int, num_tokens: int, *,
+                   block_table: torch.Tensor, free_blocks: torch.Tensor | None,
+                   free_range: torch.Tensor | None, block_size: int, num_tokens: int, *,
                    num_kv_tokens: int = 0,
                    free_range_out: torch.Tensor | None = None) -> KvPlan:
     """Give every request the cache blocks its new tokens need and map the
@@ -107,7 +107,9 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     ``free_blocks`` int32 [N] is a ring of free block ids whose entries
     [free_range[0], free_range[1]) (int64 [2], taken modulo N) are free: blocks
     are taken from the front in request order, and ``free_range_out`` (default:
-    ``free_range`` itself) receives the range that is left. ``num_tokens`` is
+    ``free_range`` itself) receives the range that is left. With ``free_blocks``
+    and ``free_range`` None the table rows are complete and nothing is taken
+    (a cache whose sequences own their blocks). ``num_tokens`` is
     the number of packed rows to fill (at least the sum of ``new_lens``: rows
     behind the last request get position and slot -1); ``num_kv_tokens`` > 0
     asks for the cache rows of all context + new tokens too. A request that
@@ -117,8 +119,12 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     B = context_lens.numel()
     _vector("context_lens", context_lens, torch.int32)
     _vector("new_lens", new_lens, torch.int32, B)
-    _vector("free_blocks", free_blocks, torch.int32)
-    _vector("free_range", free_range, torch.int64, 2)
+    if (free_blocks is None) != (free_range is None) or \
+            (free_blocks is None and free_range_out is not None):
+        raise ValueError("free_blocks and free_range come together")
+    if free_blocks is not None:
+        _vector("free_blocks", free_blocks, torch.int32)
+        _vector("free_range", free_range, torch.int64, 2)
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
             block_table.stride(1) != 1 or block_table.shape[0] != B:
         raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows")
@@ -139,8 +145,8 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     small = context_lens.new_empty(2 * B + 4)
     r, c = rows.data_ptr(), small.data_ptr()
     _call(dev, "sl_plan_kv_blocks", ptr(context_lens), ptr(new_lens), B, int(block_size),
-          ptr(block_table), ld, width, ptr(free_blocks), free_blocks.numel(), ptr(free_range),
-          ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
+          ptr(block_table), ld, width, ptr(free_blocks),
+          0 if free_blocks is None else free_blocks.numel(), ptr(free_range), ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
           r + 8 * num_tokens, r + 16 * num_tokens if num_kv_tokens else None, c + 8 * (B + 1))
     positions, slots, kv = rows.split_with_sizes([num_tokens, num_tokens, num_kv_tokens])
     cu_new, cu_total, status = small.split_with_sizes([B + 1, B + 1, 2])
