@@ -668,30 +668,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         sl::tc_fence_after();
         uint32_t r[kTile];
         auto s = [&](int c) { return __uint_as_float(r[c]); };
-        float2 sum;
-        // Scores [c0, c0 + 64) as weights, in place and packed.
-        auto weights = [&](int c0) {
-          const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
 #pragma unroll
-          for (int c = c0 / 2; c < c0 / 2 + 32; ++c) {
-            float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
-            x.x = ex2(x.x);
-            x.y = ex2(x.y);
-            sum = __fadd2_rn(sum, x);
-            r[c] = pack2<kBf16>(x.x, x.y);
-          }
-        };
-        // Handed over in halves: the product with the first 64 values runs
-        // while the weights of the others are formed.
-        auto hand_over = [&](int c0) {
-          tmem_st32(s_at + c0 / 2, r + c0 / 2);
-          if (c0 != 0) pass_turn();
-          tmem_wait_st();
-          sl::tc_fence_before();
-          __syncwarp();
-          bar_arrive(kBarWeights + 2 * h + (c0 != 0), 160);
-        };
-        auto row_max = [&]() {
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
+        if ((j + 1) * kTile > lim_first) {
+          const int left = lim - j * kTile;
+#pragma unroll
+          for (int c = 0; c < kTile; ++c)
+            if (c >= left) r[c] = 0xff800000u;  // -inf
+        }
+        float top;
+        {
           float t[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) t[i] = max3(s(32 * i), s(32 * i + 1), s(32 * i + 2));
@@ -701,54 +689,57 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
             for (int i = 0; i < 4; ++i) t[i] = max3(t[i], s(32 * i + c), s(32 * i + c + 1));
 #pragma unroll
           for (int i = 0; i < 4; ++i) t[i] = max2(t[i], s(32 * i + 31));
-          return max2(max3(t[0], t[1], t[2]), t[3]);
-        };
-        // The weights are formed against the maximum so far, which may lag behind this tile's by a factor
-        // 2^kLag: the sums and the weights' type hold that. The tile's own
-        // maximum is found meanwhile; only where it is beyond that (or NaN)
-        // the rows move to it and the work is done again.
-        // (a score of +inf leaves no finite weights: the row is NaN, as inf - inf
-        // makes it)
-        auto no_inf = [](float x) { return x == INFINITY ? __int_as_float(0x7fffffff) : x; };
-        float top = 0.f;
-#pragma unroll 1
-        for (bool again = false;; again = true) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, r + 32 * c);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_fence_ld(r + 32 * c);
-          if ((j + 1) * kTile > lim_first) {
-            const int left = lim - j * kTile;
-#pragma unroll
-            for (int c = 0; c < kTile; ++c)
-              if (c >= left) r[c] = 0xff800000u;  // -inf
-          }
-          if (again) {
-            top = no_inf(top);
-            const bool move = live && !(top <= m + p.lag);
-            const float corr = move ? ex2((m - top) * p.scale_log2) : 1.f;
-            if (move) m = top;
-            l *= corr;
-            if (j > g.j0) {
-              // the sums so far, once the products before this tile are in
-              out.wait(&sy.pv_done[h], (n_s - 1) & 1);
-              sl::tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
-            }
-          } else {
-            if (j == g.j0 && live) m = no_inf(row_max());
-            take_turn();
-          }
-          base = m == -INFINITY ? 0.f : -m * p.scale_log2;
-          sum = make_float2(0.f, 0.f);
-          top = row_max();
-          weights(0);
-          if (again || !__any_sync(0xffffffffu, live && !(top <= m + p.lag))) break;
+          top = max2(max3(t[0], t[1], t[2]), t[3]);
         }
+        // The weights are formed against a maximum that may lag behind this
+        // tile's by a factor 2^kLag (the sums and the weights' type hold that);
+        // only where it is beyond, or NaN, the rows move to it.
+        const bool move = live && !(top <= m + p.lag);
+        if (__any_sync(0xffffffffu, move)) {
+          // a score of +inf leaves no finite weights: the row is NaN, as
+          // inf - inf makes it
+          if (top == INFINITY) top = __int_as_float(0x7fffffff);
+          const float corr = move ? ex2((m - top) * p.scale_log2) : 1.f;
+          if (move) m = top;
+          base = m == -INFINITY ? 0.f : -m * p.scale_log2;
+          l *= corr;
+          if (j > g.j0) {
+            // the sums so far, once the products before this tile are in
+            out.wait(&sy.pv_done[h], (n_s - 1) & 1);
+            sl::tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kVDim / 8; ++c) tmem_scale8(o_at + 8 * c, corr);
+          }
+        }
+        float2 sum = make_float2(0.f, 0.f);
+        // Scores 2 c0 .. 2 c1 - 1 as weights, in place and packed.
+        auto weights = [&](int c0, int c1) {
+          const float2 sc = make_float2(p.scale_log2, p.scale_log2), bs = make_float2(base, base);
+#pragma unroll
+          for (int c = c0; c < c1; ++c) {
+            float2 x = __ffma2_rn(make_float2(s(2 * c), s(2 * c + 1)), sc, bs);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum = __fadd2_rn(sum, x);
+            r[c] = pack2<kBf16>(x.x, x.y);
+          }
+        };
+        // Handed over in halves: the product with the first 64 values runs
+        // while the weights of the others are formed.
+        auto hand_over = [&](int part) {
+          tmem_wait_st();
+          sl::tc_fence_before();
+          __syncwarp();
+          bar_arrive(kBarWeights + 2 * h + part, 160);
+        };
+        take_turn();
+        weights(0, 32);
+        tmem_st32(s_at, r);
         hand_over(0);
-        weights(64);
-        hand_over(64);
+        weights(32, 64);
+        tmem_st32(s_at + 32, r + 32);
+        pass_turn();
+        hand_over(1);
         l += sum.x + sum.y;
         ++n_s;
       }
