@@ -140,16 +140,21 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
         raise ValueError("num_tokens and num_kv_tokens are counts")
     dev = _device_index(context_lens, new_lens, block_table, free_blocks, free_range,
                         free_range_out)
-    # one allocation for the 64-bit outputs, one for the others
-    rows = context_lens.new_empty(2 * num_tokens + num_kv_tokens, dtype=torch.int64)
-    small = context_lens.new_empty(2 * B + 4)
-    r, c = rows.data_ptr(), small.data_ptr()
-    _call(dev, "sl_plan_kv_blocks", ptr(context_lens), ptr(new_lens), B, int(block_size),
-          ptr(block_table), ld, width, ptr(free_blocks),
-          0 if free_blocks is None else free_blocks.numel(), ptr(free_range), ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
+    # one allocation: the 64-bit outputs, then the 32-bit ones
+    n64 = 2 * num_tokens + num_kv_tokens
+    buf = torch.empty(n64 + B + 2, dtype=torch.int64, device=context_lens.device)
+    r = buf.data_ptr()
+    c = r + 8 * n64
+    _call(dev, "sl_plan_kv_blocks", context_lens.data_ptr(), new_lens.data_ptr(), B,
+          int(block_size), block_table.data_ptr(), ld, width, ptr(free_blocks),
+          0 if free_blocks is None else free_blocks.numel(), ptr(free_range),
+          ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
           r + 8 * num_tokens, r + 16 * num_tokens if num_kv_tokens else None, c + 8 * (B + 1))
-    positions, slots, kv = rows.split_with_sizes([num_tokens, num_tokens, num_kv_tokens])
-    cu_new, cu_total, status = small.split_with_sizes([B + 1, B + 1, 2])
+    # (views; "unsafe" to autograd only, which has no part in this)
+    positions, slots, kv, rest = torch.unsafe_split_with_sizes(
+        buf, (num_tokens, num_tokens, num_kv_tokens, B + 2))
+    cu_new, cu_total, status = torch.unsafe_split_with_sizes(rest.view(torch.int32),
+                                                             (B + 1, B + 1, 2))
     return KvPlan(cu_new, cu_total, positions, slots, kv if num_kv_tokens else None, status)
 
 
@@ -232,8 +237,15 @@ class Rotary:
     def _part(self, name: str, x: torch.Tensor, out: torch.Tensor | None, offset: int, T: int):
         """(the call's description of one tensor, its output, its input)."""
         in_place = out is x
-        copied, x_strides = _rotary_input(name, x.shape, x.stride(), offset, T, self.rotary_dim,
-                                          self.interleaved)
+        copied, x_strides, new = _rotary_input(name, x.shape, x.stride(), offset, T,
+                                               self.rotary_dim, self.interleaved)
+        if out is None and new is not None and not (
+                self.interleaved and x.data_ptr() % (2 * x.element_size())):
+            # the usual call: a new output like a contiguous input
+            out = torch.empty_like(x)
+            part = _lib.RotaryPart.from_buffer_copy(new)
+            part.x, part.y = x.data_ptr(), out.data_ptr()
+            return part, out, x
         if copied or (self.interleaved and x.data_ptr() % (2 * x.element_size())):
             if in_place:
                 raise ValueError(f"{name} cannot be rotated in place: its columns must be "
@@ -286,7 +298,9 @@ class Rotary:
 
 @functools.lru_cache(maxsize=512)
 def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int, interleaved: bool):
-    """(whether the input has to be copied first, its strides), by its layout."""
+    """(whether the input has to be copied first, its strides, and, for a
+    contiguous input, the description of a call that writes a new tensor,
+    without the addresses), by its layout."""
     if len(shape) != 3 or shape[0] != T:
         raise ValueError(f"{name} must be [{T}, heads, dim], got {tuple(shape)}")
     if not 0 <= offset <= shape[2] - rot:
@@ -294,7 +308,12 @@ def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int, inte
                          f"{shape[2]}")
     # pairs are read as two elements at once, so they start on even ones
     odd = interleaved and any(s % 2 for s, n in zip(strides[:2], shape) if n > 1)
-    return (shape[2] > 1 and strides[2] != 1) or odd, strides
+    copied = (shape[2] > 1 and strides[2] != 1) or odd
+    new = None
+    if not copied and strides == (shape[1] * shape[2], shape[2], 1):
+        new = _lib.RotaryPart(None, None, strides[0], strides[1], strides[0], strides[1],
+                              shape[1], shape[2], offset)
+    return copied, strides, new
 
 
 def _ranges_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -375,12 +394,15 @@ def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
     a.heads, a.kv_heads, a.dim, a.v_dim, a.shared_dim = heads, kv_heads, dim, v_dim, shared
     a.dtype = _DTYPES[dtype]
     a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    return a
+    return a, (Tq, heads, v_dim)
 
 
-def _workspace_bytes(a) -> int:
-    return max(256, lib().sl_prompt_attention_workspace_bytes(a.B, a.Tq, a.Tk, a.heads,
-                                                              a.kv_heads, a.v_dim))
+@functools.lru_cache(maxsize=512)
+def _workspace_bytes(B: int, Tq: int, Tk: int, heads: int, kv_heads: int, v_dim: int,
+                     dev: int) -> int:
+    with torch.cuda.device(dev):   # (the size goes by the device's SMs)
+        return max(256, lib().sl_prompt_attention_workspace_bytes(B, Tq, Tk, heads, kv_heads,
+                                                                  v_dim))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -409,13 +431,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         k_shared = _tiled(k_shared)
     _vector("cu_q", cu_q, torch.int32)
     _vector("cu_k", cu_k, torch.int32)
-    a = _lib.AttentionArgs.from_buffer_copy(_attention_layout(
+    layout, shape = _attention_layout(
         (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),
         None if k_shared is None else (k_shared.shape, k_shared.stride()),
         None if out is None else (out.shape, out.stride()), q.dtype, cu_q.numel(), cu_k.numel(),
-        scale))
+        scale)
+    a = _lib.AttentionArgs.from_buffer_copy(layout)
     if out is None:
-        out = q.new_empty(a.Tq, a.heads, a.v_dim)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
     elif out.data_ptr() % 16:
         raise ValueError("out needs a 16-byte aligned address")
     elif any(_ranges_meet(out, t) for t in (q, k, v, k_shared) if t is not None):
@@ -427,13 +450,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
     if a.shared_dim:
         a.k_shared = k_shared.data_ptr()
-    # (the size goes by the device's SMs: asked for with it current)
-    if torch.cuda.current_device() == dev:
-        n = _workspace_bytes(a)
-    else:
-        with torch.cuda.device(dev):
-            n = _workspace_bytes(a)
-    workspace = q.new_empty(n, dtype=torch.uint8)
+    n = _workspace_bytes(a.B, a.Tq, a.Tk, a.heads, a.kv_heads, a.v_dim, dev)
+    workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
     _call(dev, "sl_prompt_attention", ctypes.byref(a), workspace.data_ptr(), n)
     prompt_attention.last_workspace = workspace
     return out
