@@ -326,7 +326,7 @@ struct alignas(sizeof(E) * V) RotVec {
 // columns and the V columns rot / 2 further (half: V pairs). V elements are
 // one load: 16 bytes where the sizes, strides and addresses allow it.
 template <typename E, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
   // (cos, sin) * factor of each token, [pair within a unit][unit]: lanes of
   // neighbouring units read neighbouring words
   extern __shared__ float2 cs[];
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(RotArgs a) {
   const int t0 = blockIdx.x * a.per_cta;
   const int nt = min(a.per_cta, a.T - t0);
   const int nq = a.t[0].heads * a.t[0].units, n = nq + a.t[1].heads * a.t[1].units;
-  constexpr int U = kInterleaved ? 4 : 2;  // items in flight per thread
+  constexpr int U = kInterleaved ? 2 : 1;  // items in flight per thread
   Vec lo[U], hi[U];
   E* dst[U];
   int pair[U];   // first pair's place in cs, -1: not rotated
