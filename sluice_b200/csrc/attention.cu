@@ -41,8 +41,8 @@ constexpr int kBars = 16;            // barriers of tiles in flight
 // weights have the exponents of the 32-bit sums, fp16 ones end at 2^16.
 constexpr float kLagBf16 = 32.f, kLagF16 = 12.f;
 // registers a thread: 168 at launch, then shared out between the softmax warps
-// and the others (256 x 208 + 128 x 88 = 384 x 168)
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+// and the others (256 x 216 + 128 x 72 = 384 x 168)
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 constexpr int kReaders = 11;          // warps that follow the stretches
 constexpr int kSegs = 4;              // stretches looked up ahead
 constexpr int kItemUnits = 3;         // what starting and ending an item costs, in key tiles
@@ -251,6 +251,7 @@ __device__ __forceinline__ void bar_arrive(int id, int n) {
 }
 constexpr int kBarTurn = 1;     // + 4 * half + quad: this half's turn; 64 threads
 constexpr int kBarWeights = 9;  // + 2 * half + part: weights are there; 160 threads
+constexpr int kBarTwin = 13;    // half 1's result is there; 256 threads
 
 // --------------------------------------------------------------------- work
 // One stretch of an item's key tiles: [j0, j1) of n.
@@ -262,6 +263,10 @@ struct Seg {
   int nh[2];                  // key tiles that each half's last row reaches
   int lim0;                   // keys that the item's first row sees
 };
+
+// Where an item's rows fill one half only, both halves take them, each every
+// other key tile of the stretch, and their results are joined at its end.
+__device__ __forceinline__ bool is_twin(const Seg& g) { return g.nh[1] == 0 && g.j1 - g.j0 >= 2; }
 
 struct Seq {
   int q0, q_len, k0, k_len;
@@ -491,11 +496,12 @@ struct Sync {
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   Seg seg[kSegs];
   uint32_t tmem;
+  float2 twin[kTile];  // half 1's (maximum, sum) of each row
   int mark[kMarks];
   int warp_sum[kCoarse / 32];
   int cum[kCoarse + 1];
 };
-constexpr int kSmemBytes = 14 * kSlotBytes + 1024 + static_cast<int>(sizeof(Sync));
+constexpr int kSmemBytes = 14 * kSlotBytes + static_cast<int>(sizeof(Sync));
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 // A role's place in the sequence of tiles (keys, values, keys, ...): the
@@ -562,14 +568,17 @@ template <int kDim, int kVDim, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     const __grid_constant__ Params p) {
   using C = Cfg<kDim, kVDim>;
-  extern __shared__ uint8_t sm_raw[];
-  uint8_t* buf = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t buf[];
   uint8_t* ring = buf + C::kQBytes;
   Sync& sy = *reinterpret_cast<Sync*>(buf + C::kBufBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int per = (p.B + kCoarse - 1) / kCoarse;
 
+  if (sl::smem_u32(buf) & 1023) {
+    // (the swizzled tiles want it; there is no static shared memory before it)
+    if (tid == 0) *p.status = SL_ERR_UNSUPPORTED;
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
       sl::mbar_init(&sy.full[i], 1);
@@ -647,8 +656,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       bar_arrive(kBarTurn + 4 * (h ^ 1) + quad, 64);
     };
     while (next_seg()) {
-      const int first = g.tok + h * p.half_tokens;
-      const int j1 = min(g.j1, g.nh[h]);
+      const bool twin = is_twin(g);
+      const int first = g.tok + (twin ? 0 : h * p.half_tokens);
+      const int j0 = twin ? g.j0 + h : g.j0, step = twin ? 2 : 1;
+      const int j1 = twin ? g.j1 : min(g.j1, g.nh[h]);
       const bool has = g.j0 < g.j1;
       const int mark = has ? n_item++ : -1;
       if (first >= g.q_len) {
@@ -663,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       const int lim = live ? clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len) : 0;
       const int lim_first = clampi(first + 1 + g.k_len - g.q_len, 0, g.k_len);
       float m = -INFINITY, l = 0.f, base = 0.f;  // base: -m in powers of 2
-      for (int j = g.j0; j < j1; ++j) {
+      for (int j = j0; j < j1; j += step) {
         out.wait(&sy.s_full[h], n_s & 1);
         sl::tc_fence_after();
         uint32_t r[kTile];
@@ -703,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           if (move) m = top;
           base = m == -INFINITY ? 0.f : -m * p.scale_log2;
           l *= corr;
-          if (j > g.j0) {
+          if (j > j0) {
             // the sums so far, once the products before this tile are in
             out.wait(&sy.pv_done[h], (n_s - 1) & 1);
             sl::tc_fence_after();
@@ -744,7 +755,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         ++n_s;
       }
       // (the other half may have more tiles)
-      for (int j = max(g.j0, j1); j < g.j1; ++j) {
+      const int spare = twin ? (g.j1 - g.j0) & h : g.j1 - max(g.j0, j1);
+      for (int j = 0; j < spare; ++j) {
         take_turn();
         pass_turn();
       }
@@ -754,13 +766,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       const int prow = h * p.half_tokens * p.group + row;
       const int pslot = 2 * blockIdx.x + (g.j0 > 0 ? 0 : 1);
       float* part = p.part + (static_cast<int64_t>(pslot) * p.rows_cap + prow) * kVDim;
-      if (!whole && live) p.part_ml[static_cast<int64_t>(pslot) * p.rows_cap + prow] =
-          make_float2(m, l);
-      const bool ran = g.j0 < j1;
+      const bool ran = j0 < j1;
       if (ran) {
         out.wait(&sy.pv_done[h], (n_s - 1) & 1);
         sl::tc_fence_after();
       }
+      // twin: half 0 puts the two results together, row by row (the same TMEM
+      // lanes, the other accumulator)
+      float own = 1.f, others = 0.f;
+      if (twin) {
+        if (h == 1) {
+          sy.twin[row] = make_float2(m, l);
+          sl::tc_fence_before();
+          __syncwarp();
+          bar_arrive(kBarTwin, 256);
+          continue;
+        }
+        bar_wait(kBarTwin, 256);
+        sl::tc_fence_after();
+        const float2 ml = sy.twin[row];
+        const float top = max2(m, ml.x), to = top == -INFINITY ? 0.f : top;
+        own = ex2((m - to) * p.scale_log2);
+        others = ex2((ml.x - to) * p.scale_log2);
+        m = top;
+        l = l * own + ml.y * others;
+      }
+      if (!whole && live) p.part_ml[static_cast<int64_t>(pslot) * p.rows_cap + prow] =
+          make_float2(m, l);
       const bool repair = has && sy.mark[mark % kMarks] == mark;
       // no key seen: zeros; only keys that score -inf: 0 / 0
       const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
@@ -775,6 +807,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (twin) {
+          uint32_t o1[32];
+          tmem_ld32(o_col[1] + lanes + c, o1);
+          tmem_fence_ld(o1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            o[i] = __float_as_uint(__uint_as_float(o[i]) * own + __uint_as_float(o1[i]) * others);
         }
         if (repair && live) {
           // values that are not finite were taken out of the tiles that not
@@ -820,7 +860,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       if (ran) {
         sl::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sl::mbar_arrive(&sy.o_free[h]);
+        if (lane == 0) {
+          sl::mbar_arrive(&sy.o_free[h]);
+          if (twin) sl::mbar_arrive(&sy.o_free[1]);
+        }
       }
     }
     // (the last turn that half 1 passed on)
@@ -864,14 +907,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     while (next_seg()) {
       uniform(g);
       if (g.j0 >= g.j1) continue;
-      const int j1 = min(g.j1, g.nh[h]);
-      const bool any = g.j0 < j1;
+      const bool twin = is_twin(g);
+      const int j1 = twin ? g.j1 : min(g.j1, g.nh[h]);
+      const int j0 = twin ? g.j0 + h : g.j0;  // this half's first tile
+      auto takes = [&](int j) { return twin ? ((j - j0) & 1) == 0 && j < j1 : j < j1; };
+      const bool any = j0 < j1;
       if (any) out.wait(&sy.q_full[h], n_o & 1);
       out.wait(&sy.full[at.bar()], at.phase());
       sl::tc_fence_after();
-      key_tile(any);
+      key_tile(takes(g.j0));
       for (int j = g.j0; j < g.j1; ++j) {
-        const bool mine = j < j1;
+        const bool mine = takes(j);
         // this tile's values and the next one's keys are here, as a rule, long
         // before the weights
         out.wait(&sy.full[at.bar()], at.phase());
@@ -886,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         const bool next = j + 1 < g.j1;
         if (next) out.wait(&sy.full[at.bar()], at.phase());
         if (mine) {
-          if (j == g.j0 && n_o > 0) out.wait(&sy.o_free[h], (n_o - 1) & 1);
+          if (j == j0 && n_o > 0) out.wait(&sy.o_free[h], (n_o - 1) & 1);
           // O += P V in two halves of 64 keys, as the weights come in
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -899,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_ts(o_d, s_d + 32 * half + 8 * k, v_lo + 128 * k, idesc_o,
-                        j > g.j0 || half + k > 0);
+                        j > j0 || half + k > 0);
             }
           }
           if (leader && out.ok) {
@@ -910,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           sl::mbar_arrive(&sy.empty[v_bar]);
         }
         __syncwarp();
-        if (next) key_tile(j + 1 < j1);
+        if (next) key_tile(takes(j + 1));
       }
       if (any) {
         ++n_o;
@@ -947,7 +993,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       uniform(g);
       if (g.j0 >= g.j1) continue;
       auto load_q = [&](int h) -> bool {
-        if (g.j0 >= min(g.j1, g.nh[h])) return true;
+        const bool twin = is_twin(g);
+        if (g.j0 >= min(g.j1, g.nh[h]) && !twin) return true;
         if (n_q[h] > 0 && !out.wait(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
         ++n_q[h];
         if (lane == 0) {
@@ -955,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
             tma_load_3d(buf + (h * C::kChunks + c) * kSlotBytes, &p.q, &sy.q_full[h], 64 * c,
-                        g.head * p.group, g.q0 + g.tok + h * p.half_tokens);
+                        g.head * p.group, g.q0 + g.tok + (twin ? 0 : h * p.half_tokens));
         }
         return true;
       };
