@@ -54,6 +54,17 @@ struct Later {
   int unit0, q0, q_len, k_len, tok, head, pad[2];
 };
 
+// x / d of 0 <= x < 2^31 by a multiplication: mul = ceil(2^(31 + shift) / d),
+// 2^shift >= d (a division by a number that is not known when compiling is a
+// long subroutine, and the lookups of a stretch are all divisions).
+struct Divisor {
+  uint32_t mul;
+  int shift, d;
+};
+__device__ __forceinline__ int quotient(const Divisor& v, int x) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * v.mul) >> (31 + v.shift));
+}
+
 struct Params {
   CUtensorMap q, k, v, ks;
   void* out;
@@ -66,6 +77,7 @@ struct Params {
   int shared;                        // the last 64 key columns come from ks
   int wide;                          // the output's rows are 32-byte aligned
   int grid;                          // CTAs
+  Divisor by_tokens, by_heads, by_grid;  // tokens of an item, key heads, CTAs
   int split;                         // 1: equal shares of all key tiles per CTA
   int rows_cap;                      // rows of a partial result
   float scale_log2;                  // scale / ln 2
@@ -287,7 +299,7 @@ __device__ __forceinline__ int seen(const Seq& s, int tok) {
   return clampi(tok + 1 + s.k_len - s.q_len, 0, s.k_len);
 }
 __device__ __forceinline__ int tiles_of(const Params& p, const Seq& s) {
-  return (s.q_len + 2 * p.half_tokens - 1) / (2 * p.half_tokens);
+  return quotient(p.by_tokens, s.q_len) + (quotient(p.by_tokens, s.q_len) * p.by_tokens.d < s.q_len);
 }
 // key tiles of item `t`
 __device__ __forceinline__ int reach(const Params& p, const Seq& s, int t) {
@@ -411,7 +423,7 @@ struct Walk {
   }
   // where CTA c's share begins: equal ones, the first with one unit more
   __device__ static int share(const Params& p, int total, int c) {
-    const int each = total / p.grid;
+    const int each = quotient(p.by_grid, total);
     return each * c + min(c, total - each * p.grid);
   }
   __device__ bool next(const Params& p, const int* cum, int per, Seg& g) {
@@ -421,9 +433,10 @@ struct Walk {
       const int i = round * G + ((round & 1) ? G - 1 - c : c);
       if (i >= total) return false;
       ++round;
-      g.head = i % p.kv_heads;
+      const int ord = quotient(p.by_heads, i);
+      g.head = i - ord * p.kv_heads;
       int rest;
-      const Seq s = find_seq(p, cum, per, i / p.kv_heads, g.seq, rest);
+      const Seq s = find_seq(p, cum, per, ord, g.seq, rest);
       g.tile = tiles_of(p, s) - 1 - rest;
       fill_seg(p, s, g);
       g.j0 = 0;
@@ -451,8 +464,9 @@ struct Walk {
     const int lane = threadIdx.x & 31;
     // units of a sequence count all heads: tile after tile, head after head
     int rest;
-    const Seq s = find_seq(p, cum, per, u / p.kv_heads, g.seq, rest);
-    int r = rest * p.kv_heads + u % p.kv_heads;
+    const int ord = quotient(p.by_heads, u);
+    const Seq s = find_seq(p, cum, per, ord, g.seq, rest);
+    int r = rest * p.kv_heads + u - ord * p.kv_heads;
     const int nt = tiles_of(p, s);
     for (int t0 = 0;; t0 += 32) {
       const int t = t0 + lane;
@@ -474,8 +488,16 @@ struct Walk {
     }
     fill_seg(p, s, g);
     n = kItemUnits + g.n;
-    g.head = min(r / n, p.kv_heads - 1);
-    j = r - r / n * n;
+    // r / n (the estimate is off by one at most: r < 2^22)
+    g.head = static_cast<int>(__fdividef(static_cast<float>(r), static_cast<float>(n)));
+    j = r - g.head * n;
+    if (j < 0) {
+      --g.head;
+      j += n;
+    } else if (j >= n) {
+      ++g.head;
+      j -= n;
+    }
   }
 };
 
@@ -659,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       const bool twin = is_twin(g);
       const int first = g.tok + (twin ? 0 : h * p.half_tokens);
       const int j0 = twin ? g.j0 + h : g.j0, step = twin ? 2 : 1;
-      const int j1 = twin ? g.j1 : min(g.j1, g.nh[h]);
+      const int j1 = twin ? g.j1 : min(g.j1, h ? g.nh[1] : g.nh[0]);
       const bool has = g.j0 < g.j1;
       const int mark = has ? n_item++ : -1;
       if (first >= g.q_len) {
@@ -908,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const bool twin = is_twin(g);
-      const int j1 = twin ? g.j1 : min(g.j1, g.nh[h]);
+      const int j1 = twin ? g.j1 : min(g.j1, h ? g.nh[1] : g.nh[0]);
       const int j0 = twin ? g.j0 + h : g.j0;  // this half's first tile
       auto takes = [&](int j) { return twin ? ((j - j0) & 1) == 0 && j < j1 : j < j1; };
       const bool any = j0 < j1;
@@ -994,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       if (g.j0 >= g.j1) continue;
       auto load_q = [&](int h) -> bool {
         const bool twin = is_twin(g);
-        if (g.j0 >= min(g.j1, g.nh[h]) && !twin) return true;
+        if (g.j0 >= min(g.j1, h ? g.nh[1] : g.nh[0]) && !twin) return true;
         if (n_q[h] > 0 && !out.wait(&sy.q_empty[h], (n_q[h] - 1) & 1)) return false;
         ++n_q[h];
         if (lane == 0) {
@@ -1345,6 +1367,15 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   p.grid = static_cast<int>(r.grid);
   p.split = r.split;
   p.rows_cap = r.rows_cap;
+  auto divisor = [](int d) {
+    Divisor v = {0, 0, d};
+    while ((1 << v.shift) < d) ++v.shift;
+    v.mul = static_cast<uint32_t>(((1ull << (31 + v.shift)) + d - 1) / d);
+    return v;
+  };
+  p.by_tokens = divisor(2 * p.half_tokens);
+  p.by_heads = divisor(p.kv_heads);
+  p.by_grid = divisor(p.grid);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.lag = (bf16 ? kLagBf16 : kLagF16) / p.scale_log2;
   p.status = static_cast<int32_t*>(workspace);
