@@ -322,7 +322,8 @@ struct alignas(sizeof(E) * V) RotVec {
   E e[V];
 };
 
-// A unit is V adjacent columns of a head (interleaved: V / 2 pairs), or V
+// (products and sums are written out, so that every form of the kernel rounds
+// alike.) A unit is V adjacent columns of a head (interleaved: V / 2 pairs), or V
 // columns and the V columns rot / 2 further (half: V pairs). V elements are
 // one load: 16 bytes where the sizes, strides and addresses allow it.
 template <typename E, int V, bool kInterleaved>
@@ -398,16 +399,16 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
           for (int k = 0; k < V / 2; ++k) {
             const float2 c = cs[pair[u] + k * a.rot_units];
             const float x0 = to_f(lo[u].e[2 * k]), x1 = to_f(lo[u].e[2 * k + 1]);
-            lo[u].e[2 * k] = from_f<E>(x0 * c.x - x1 * c.y);
-            lo[u].e[2 * k + 1] = from_f<E>(x1 * c.x + x0 * c.y);
+            lo[u].e[2 * k] = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
+            lo[u].e[2 * k + 1] = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
           }
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k) {
             const float2 c = cs[pair[u] + k * a.rot_units];
             const float x0 = to_f(lo[u].e[k]), x1 = to_f(hi[u].e[k]);
-            lo[u].e[k] = from_f<E>(x0 * c.x - x1 * c.y);
-            hi[u].e[k] = from_f<E>(x1 * c.x + x0 * c.y);
+            lo[u].e[k] = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
+            hi[u].e[k] = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
           }
         }
       }

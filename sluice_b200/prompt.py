@@ -45,6 +45,13 @@ def _device_index(first: torch.Tensor, *others) -> int:
     return dev
 
 
+def _no_gradient(*tensors) -> None:
+    """Refuse what autograd would silently cut off."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("this operator has no backward pass: call it under torch.no_grad(), or "
+                         "with detached tensors")
+
+
 def _call(dev: int, name: str, *args) -> None:
     """``name`` of the library with ``args`` and the current stream of device
     ``dev``, which is made the current one where it is not."""
@@ -284,6 +291,7 @@ class Rotary:
             raise ValueError("q and k must share one of bfloat16, float16, float32")
         T = positions.numel()
         _vector("positions", positions, torch.int64)
+        _no_gradient(q, k)
         if k is None and out_k is not None:
             raise ValueError("out_k without k")
         pq, out_q, q = self._part("q", q, out_q, q_offset, T)
@@ -426,6 +434,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     for name, t in (("k", k), ("v", v), ("k_shared", k_shared), ("out", out)):
         if t is not None and t.dtype != q.dtype:
             raise ValueError(f"{name} is {t.dtype}, q is {q.dtype}")
+    _no_gradient(q, k, v, k_shared)
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     if k_shared is not None:
         k_shared = _tiled(k_shared)

@@ -117,6 +117,9 @@ def _plan_args(B=2, width=4):
     dict(free_range=torch.tensor([0, 8], dtype=torch.int32)),
     dict(free_blocks=torch.zeros(16, dtype=torch.int32)[::2]), dict(num_tokens=-1),
     dict(free_range_out=torch.zeros(3, dtype=torch.int64)),
+    dict(free_blocks=None), dict(free_range=None),
+    dict(free_blocks=None, free_range=None, free_range_out=torch.tensor([0, 8])),
+    dict(free_blocks=None, free_range=None),   # (CPU tensors)
     dict()])   # (CPU tensors)
 def test_plan_refuses(change):
     with pytest.raises(ValueError):
@@ -153,6 +156,17 @@ def test_attention_refuses_an_output_over_an_input():
     a = _qkv(heads=2)
     with pytest.raises(ValueError, match="overlaps"):
         prompt.prompt_attention(**a, out=a["q"])
+
+
+def test_operators_without_a_backward_pass_refuse_gradients():
+    a = _qkv()
+    a["k"].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        prompt.prompt_attention(**a)
+    with pytest.raises(ValueError, match="backward"):
+        prompt.Rotary(64, device="cpu")(torch.arange(8), a["v"].clone().requires_grad_())
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        prompt.prompt_attention(**a)
 
 
 def test_rotary_refuses():
@@ -192,6 +206,15 @@ def test_c_entries_refuse_without_a_gpu():
     assert plan() == BAD and plan(B=0) == BAD and plan(bs=0) == BAD and plan(ld=7) == BAD
     assert plan(width=0) == BAD and plan(n=0) == BAD and plan(T=-1) == BAD and plan(Tk=4) == BAD
     assert plan(B=8193) == UNS
+
+    def paged(blocks=8, bs=64, ld=4, width=4, max_len=256, rank=512):
+        return L.sl_mla_decode_paged(None, 16 * 192 + rank + 64, None, 1e-6, None, None, None,
+                                     None, None, blocks, bs, None, ld, width, 8, 16, 128, 64, rank,
+                                     128, max_len, 0.07, None, None)
+
+    assert paged() == BAD and paged(blocks=0) == BAD and paged(ld=3) == BAD
+    assert paged(width=0) == BAD and paged(max_len=257) == BAD
+    assert paged(bs=48, max_len=192) == UNS
 
     def rot(T=4, rot=64, inter=1, dtype=0, heads=2, dim=128, offset=0, stride=128, x=16):
         p = _lib.RotaryPart(x, x, heads * stride, stride, heads * stride, stride, heads, dim,

@@ -102,6 +102,40 @@ def test_plan_without_blocks_left():
     assert ref[7] and p.status[0].item() == _lib.KV_PLAN_NO_BLOCKS
 
 
+def test_plan_of_complete_tables_and_large_block_ids():
+    """Without a ring every block is in the table, and none is taken; slots pass
+    32 bits."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    ids = [[2 ** 30 + 5, 7, -1], [2 ** 31 - 1, 2 ** 27, 3]]
+    table = torch.tensor(ids, **i32)
+    for bs in (64, 100):
+        context, new = [10, 0], [bs + 20, 2 * bs + 1]
+        p = prompt.plan_kv_blocks(torch.tensor(context, **i32), torch.tensor(new, **i32), table, None,
+                                  None, bs, sum(new), num_kv_tokens=sum(new) + sum(context))
+        p.check()
+        want = [ids[r][q // bs] * bs + q % bs for r in (0, 1)
+                for q in range(context[r], context[r] + new[r])]
+        assert p.slots.tolist() == want and table.tolist() == ids
+        assert p.kv_slots.tolist() == [ids[0][q // bs] * bs + q % bs
+                                       for q in range(context[0] + new[0])] + want[new[0]:]
+        assert p.status.tolist() == [0, 0]
+    # a row that is too narrow, and an entry that is no block
+    p = prompt.plan_kv_blocks(torch.tensor([0, 0], **i32), torch.tensor([193, 5], **i32), table, None,
+                              None, 64, 198)
+    assert p.status[0].item() == _lib.KV_PLAN_NO_BLOCKS
+    assert p.slots[:193].eq(-1).all() and p.slots[193:].ge(0).all()
+    p = prompt.plan_kv_blocks(torch.tensor([0, 0], **i32), torch.tensor([140, 5], **i32), table, None,
+                              None, 64, 145)
+    assert p.slots[128:140].eq(-1).all() and p.slots[:128].ge(0).all()
+    # the same from a ring of such ids
+    free = torch.tensor([2 ** 31 - 2, 2 ** 28], **i32)
+    p = prompt.plan_kv_blocks(torch.tensor([0], **i32), torch.tensor([100], **i32),
+                              torch.full((1, 2), -1, **i32), free,
+                              torch.tensor([1, 3], device="cuda"), 64, 100)
+    assert p.slots.tolist() == [2 ** 28 * 64 + q for q in range(64)] + \
+        [(2 ** 31 - 2) * 64 + q for q in range(36)]
+
+
 def test_plan_survives_bad_lengths_and_ranges():
     """Lengths below zero, more tokens than the outputs hold, contexts past the
     table row, a range larger than its ring: flagged, nothing out of place."""
@@ -198,6 +232,17 @@ def test_rotary_far_positions_keep_their_phase():
     ref = oprompt.rotary(x, pos, freqs, 1.0, 0, True)
     tol = 1e-6 + pos.double()[:, None, None] * 2.0 ** -50
     assert ((y.double() - ref).abs() <= tol).all()
+
+
+def test_rotary_of_rows_past_32_bit_offsets():
+    big = torch.empty(3, 1 << 30, device="cuda", dtype=torch.bfloat16)
+    x = big[:, -256:].view(3, 2, 128)
+    x.copy_(torch.randn(3, 2, 128, device="cuda", generator=_gen(2)))
+    pos, r = torch.tensor([5, 77, 12345], device="cuda"), prompt.Rotary(128)
+    want = r(pos, x.contiguous())
+    assert torch.equal(r(pos, x), want)
+    r(pos, x, out_q=x)
+    assert torch.equal(x, want)
 
 
 def test_rotary_leaves_padding_rows_and_other_layouts():
@@ -440,6 +485,54 @@ def test_attention_survives_bad_offsets():
                                 out=big[16:80])
         torch.cuda.synchronize()
         assert big[:16].eq(5.0).all() and big[80:].eq(5.0).all()
+
+
+def test_attention_over_a_cache_past_32_bit_offsets():
+    """2.2 million keys of 8 heads: element offsets past 2^31."""
+    Tk, g = 2_200_003, _gen(20)
+    q = torch.randn(3, 16, 128, device="cuda", generator=g).bfloat16()
+    k = torch.empty(Tk, 8, 128, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    v = torch.empty(Tk, 8, 128, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    lens = [5, Tk - 1005, 1000]
+    cu_q = torch.tensor([0, 1, 2, 3], device="cuda", dtype=torch.int32)
+    cu_k = torch.tensor([0] + lens, device="cuda").cumsum(0).int()
+    out = prompt.prompt_attention(q, k, v, cu_q, cu_k)
+    for b, h in ((1, 0), (1, 15), (2, 9)):
+        kk = k[cu_k[b]:cu_k[b + 1], h // 2].double()
+        vv = v[cu_k[b]:cu_k[b + 1], h // 2].double()
+        p = torch.softmax(kk @ q[b, h].double() * 128 ** -0.5, dim=0)
+        ref, mag = p @ vv, p @ vv.abs()
+        # (sums of 17 000 tiles in 32 bits on top: 2^-24 each, half of them
+        # rounding alike at most)
+        tol = _bounds(ref, mag, torch.bfloat16, lens[b], 6.0) + 2.0 ** -11 * mag
+        assert ((out[b, h].double() - ref).abs() <= tol).all()
+
+
+def test_first_call_of_a_process_in_a_capture():
+    """A process whose first calls are captured ones, replayed twice."""
+    import os
+    import subprocess
+    import sys
+
+    code = (
+        "import torch\n"
+        "from sluice_b200 import prompt\n"
+        "cu = torch.tensor([0, 1], device='cuda', dtype=torch.int32)\n"
+        "ck = torch.tensor([0, 3000], device='cuda', dtype=torch.int32)\n"
+        "q = torch.randn(1, 8, 128, device='cuda').bfloat16()\n"
+        "k = torch.randn(3000, 2, 128, device='cuda').bfloat16()\n"
+        "pos = torch.tensor([7], device='cuda')\n"
+        "r = prompt.Rotary(128)\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    o = prompt.prompt_attention(r(pos, q), k, k, cu, ck)\n"
+        "g.replay(); a = o.clone(); g.replay()\n"
+        "assert torch.equal(a, o) and torch.equal(o, prompt.prompt_attention(r(pos, q), k, k, cu, ck))\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_attention_empty_calls():
