@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     uint32_t clean_phase = 0;
     // S = Q K^T with the key tile at `at`, or (this half sees none of it) let
     // it go
-    auto key_tile = [&](bool mine) {
+    auto key_tile = [&](bool mine, bool last) {
       if (leader && out.ok) {
         if (mine) {
 #pragma unroll
@@ -919,6 +919,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           }
           sl::umma_commit(&sy.s_full[h]);
           sl::umma_commit(&sy.empty[at.bar()]);
+          // the next item's queries may come in while this one's last weights
+          // are formed
+          if (last) sl::umma_commit(&sy.q_empty[h]);
         } else {
           sl::mbar_arrive(&sy.empty[at.bar()]);
         }
@@ -937,7 +940,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       if (any) out.wait(&sy.q_full[h], n_o & 1);
       out.wait(&sy.full[at.bar()], at.phase());
       sl::tc_fence_after();
-      key_tile(takes(g.j0));
+      const int j_last = twin ? j1 - 1 - ((j1 - 1 - j0) & 1) : j1 - 1;
+      key_tile(takes(g.j0), g.j0 == j_last);
       for (int j = g.j0; j < g.j1; ++j) {
         const bool mine = takes(j);
         // this tile's values and the next one's keys are here, as a rule, long
@@ -978,13 +982,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           sl::mbar_arrive(&sy.empty[v_bar]);
         }
         __syncwarp();
-        if (next) key_tile(takes(j + 1));
+        if (next) key_tile(takes(j + 1), j + 1 == j_last);
       }
-      if (any) {
-        ++n_o;
-        if (leader && out.ok) sl::umma_commit(&sy.q_empty[h]);
-        __syncwarp();
-      }
+      n_o += any;
     }
     // everything issued is in before TMEM and the barriers go
     if (leader) sl::umma_commit(&sy.drain[h]);
