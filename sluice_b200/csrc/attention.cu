@@ -403,15 +403,64 @@ __device__ __forceinline__ void uniform(Seg& g) {
   g.lim0 = __shfl_sync(kAll, g.lim0, 0);
 }
 
-// Walks a CTA's share of the work. Every role's warp walks it by itself.
-//   whole items: the longest first, dealt out in turns that go back and forth;
+// How many items of a sequence reach x key tiles or more (they are its last
+// ones: what an item reaches grows with its place).
+__device__ __forceinline__ int items_from(const Params& p, const Seq& s, int x) {
+  const int nt = tiles_of(p, s);
+  if (x <= 0) return nt;
+  const int need = (x - 1) * kTile + 1;  // keys that the item's last row sees, at least
+  if (nt == 0 || s.k_len < need) return 0;
+  const int m = need - (s.k_len - s.q_len);  // ... which is so from this row on
+  const int t = m <= p.by_tokens.d ? 0 : quotient(p.by_tokens, m + p.by_tokens.d - 1) - 1;
+  return nt - min(t, nt - 1);
+}
+
+// The ord-th item, as (sequence, place), in the order of the key tiles that
+// items reach, most first; of up to 32 sequences, a lane each.
+__device__ __noinline__ int2 pick_item(const Params& p, int ord) {
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  Seq mine = {0, 0, 0, 0};
+  if (lane < p.B) mine = load_seq(p, lane);
+  // the largest x that more than ord items reach
+  int x = 0, past = 0;  // past: items that reach hi
+  int hi = __reduce_max_sync(kAll, (mine.k_len + kTile - 1) / kTile) + 1;
+  while (hi - x > 1) {
+    const int mid = (x + hi) >> 1;
+    const int n = __reduce_add_sync(kAll, items_from(p, mine, mid));
+    if (n > ord) {
+      x = mid;
+    } else {
+      hi = mid;
+      past = n;
+    }
+  }
+  const int from = items_from(p, mine, x), own = from - items_from(p, mine, x + 1);
+  int v = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(kAll, v, o);
+    if (lane >= o) v += u;
+  }
+  const int rest = ord - past;
+  const int l = max(0, __ffs(__ballot_sync(kAll, v > rest)) - 1);
+  return make_int2(l, __shfl_sync(kAll, tiles_of(p, mine) - from + rest - (v - own), l));
+}
+
+// Walks a CTA's share of the work.
+//   whole items: the longest first (of up to 32 sequences; of more, sequence
+//   after sequence), dealt out in turns that go back and forth;
 //   split: an equal run of key tiles, item after item.
 struct Walk {
   int total, at, end, round, unit0;  // unit0: the first unit of the last stretch's item
+  bool sorted;
 
   __device__ void start(const Params& p, const int* cum) {
     total = units(p, cum);
     round = 0;
+    // (one sequence is in order already, and the order does not matter where no
+    // CTA takes a second item)
+    sorted = !p.split && p.B > 1 && p.B <= 32 && total > p.grid;
     if (p.split) {
       at = share(p, total, blockIdx.x);
       end = share(p, total, blockIdx.x + 1);
@@ -435,9 +484,17 @@ struct Walk {
       ++round;
       const int ord = quotient(p.by_heads, i);
       g.head = i - ord * p.kv_heads;
-      int rest;
-      const Seq s = find_seq(p, cum, per, ord, g.seq, rest);
-      g.tile = tiles_of(p, s) - 1 - rest;
+      Seq s;
+      if (sorted) {
+        const int2 at = pick_item(p, ord);
+        g.seq = at.x;
+        g.tile = at.y;
+        s = load_seq(p, g.seq);
+      } else {
+        int rest;
+        s = find_seq(p, cum, per, ord, g.seq, rest);
+        g.tile = tiles_of(p, s) - 1 - rest;
+      }
       fill_seg(p, s, g);
       g.j0 = 0;
       g.j1 = g.n;
@@ -1079,7 +1136,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     int n_item = 0;
     Walk walk;
     walk.start(p, sy.cum);
-    Seg ahead;
+    Seg ahead = {};
     auto publish = [&]() {
       const int i = n_seg % kSegs;
       if (n_seg >= kSegs && !out.wait(&sy.seg_empty[i], (n_seg / kSegs - 1) & 1)) return;
@@ -1091,21 +1148,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       __syncwarp();
       ++n_seg;
     };
-    publish();
-    if (p.split && lane == 0) {
-      const bool later = ahead.seq >= 0 && ahead.j0 > 0;
-      Later w = {};
-      w.unit0 = later ? walk.unit0 : -1;
-      w.q0 = ahead.q0;
-      w.q_len = ahead.q_len;
-      w.k_len = ahead.k_len;
-      w.tok = ahead.tok;
-      w.head = ahead.head;
-      p.later[blockIdx.x] = w;
-    }
-    while (out.ok && ahead.seq >= 0) {
+    // (one call in the loop: the lookup's code is fetched once)
+    for (bool begun = false;; begun = true) {
       g = ahead;
+      if (begun && (g.seq < 0 || !out.ok)) break;
       publish();
+      if (!begun) {
+        if (p.split && lane == 0) {
+          const bool later = ahead.seq >= 0 && ahead.j0 > 0;
+          Later w = {};
+          w.unit0 = later ? walk.unit0 : -1;
+          w.q0 = ahead.q0;
+          w.q_len = ahead.q_len;
+          w.k_len = ahead.k_len;
+          w.tok = ahead.tok;
+          w.head = ahead.head;
+          p.later[blockIdx.x] = w;
+        }
+        continue;
+      }
       uniform(g);
       if (g.j0 >= g.j1) continue;
       const int mark = n_item++;
