@@ -1214,54 +1214,75 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(
     const __grid_constant__ Params p) {
   sl::pdl_wait();
   sl::pdl_trigger();
+  constexpr unsigned kAll = 0xffffffffu;
   const int c = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Later g = p.later[c + 1];
-  if (g.unit0 < 0 || p.later[c].unit0 == g.unit0) return;
-  // CTAs c .. e - 1 have a stretch each
-  int e = c + 1;
-  for (;;) {
-    const int s = e + lane;
-    const unsigned same =
-        __ballot_sync(0xffffffffu, s < p.grid && p.later[min(s, p.grid - 1)].unit0 == g.unit0);
-    e += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
-    if (same != 0xffffffffu) break;
+  // CTAs c .. c + n - 1 have a stretch each
+  int n = 1;
+  for (int s0 = c;; s0 += 32) {
+    const int unit = s0 + lane < p.grid ? p.later[s0 + lane].unit0 : -1;
+    const unsigned other = __ballot_sync(kAll, unit != g.unit0 || unit < 0);
+    if (s0 == c) {
+      if (!(other & 1) || (other & 2)) return;  // not the first boundary inside an item
+      n = (other >> 1) == 0 ? 32 : __ffs(other >> 1);
+      if (n < 32) break;
+    } else {
+      n += other == 0 ? 32 : __ffs(other) - 1;
+      if (other) break;
+    }
   }
   const int rows = 2 * p.half_tokens * p.group;
-  constexpr int kCols = kVDim / 32;
-  for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows;
-       r += gridDim.y * (kJoinThreads / 32)) {
+  constexpr int kCols = kVDim / 32;  // of a lane
+  constexpr int kAhead = 4;          // results of a row whose loads do not wait for its weights
+  using Vec = typename std::conditional<kCols == 4, float4, float2>::type;
+  const int step = gridDim.y * (kJoinThreads / 32);
+  for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < rows; r += step) {
     const int token = r / p.group, tok = g.tok + token;
     if (tok >= g.q_len) break;
     const int lim = clampi(tok + 1 + g.k_len - g.q_len, 0, g.k_len);
     float m = -INFINITY, l = 0.f, o[kCols] = {};
-    // a lane per stretch for the maxima and sums, then all lanes for the
-    // outputs, whose loads do not wait for one another
-    for (int s0 = c; s0 < e; s0 += 32) {
-      const int s = s0 + lane;
-      const bool has = s < e;
-      const int64_t at = has ? (2 * static_cast<int64_t>(s) + (s == c)) * p.rows_cap + r : 0;
-      const float2 ml = has ? p.part_ml[at] : make_float2(-INFINITY, 0.f);
+    // the row of stretch s (of the first one's second slot, of the others' first)
+    auto at = [&](int s) {
+      return (2 * static_cast<int64_t>(c + s) + (s == 0)) * p.rows_cap + r;
+    };
+    auto load = [&](int s) {
+      return reinterpret_cast<const Vec*>(p.part + at(s) * kVDim)[lane];
+    };
+    // a lane per stretch for the maxima and sums, then all lanes for the outputs
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      const int here = min(32, n - s0);
+      const float2 ml = lane < here ? p.part_ml[at(s0 + lane)] : make_float2(-INFINITY, 0.f);
+      Vec v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (k < here) v[k] = load(s0 + k);
       float top = max2(m, ml.x);
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) top = max2(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int x = 16; x > 0; x >>= 1) top = max2(top, __shfl_xor_sync(kAll, top, x));
       const float base = top == -INFINITY ? 0.f : top;
       const float mine = ex2((ml.x - base) * p.scale_log2), old = ex2((m - base) * p.scale_log2);
-      float sum = has ? ml.y * mine : 0.f;
+      float sum = lane < here ? ml.y * mine : 0.f;
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(kAll, sum, x);
       l = l * old + sum;
       m = top;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) o[i] *= old;
-#pragma unroll 8
-      for (int k = 0; k < min(32, e - s0); ++k) {
-        const float w = __shfl_sync(0xffffffffu, mine, k);
-        const float* src = p.part +
-            ((2 * static_cast<int64_t>(s0 + k) + (s0 + k == c)) * p.rows_cap + r) * kVDim +
-            lane * kCols;
+      for (int k0 = 0; k0 < here; k0 += kAhead) {
+        if (k0 > 0) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) o[i] = fmaf(src[i], w, o[i]);
+          for (int k = 0; k < kAhead; ++k)
+            if (k0 + k < here) v[k] = load(s0 + k0 + k);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const float w = __shfl_sync(kAll, mine, min(k0 + k, 31));
+          if (k0 + k >= here) continue;
+          const float* x = reinterpret_cast<const float*>(&v[k]);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) o[i] = fmaf(x[i], w, o[i]);
+        }
       }
     }
     const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
