@@ -1346,12 +1346,29 @@ Shape shape_of(int B, int64_t Tq, int64_t Tk, int heads, int kv_heads, int sms) 
   const int64_t items = (Tq + B * (tokens - 1)) / tokens;
   r.items = (items < Tq ? items : Tq) * kv_heads;
   r.units = r.items * (Tk / kTile + 1 + kItemUnits);
-  // few items with long key ranges: share out the key tiles instead
-  r.split = r.units < kMostUnits &&
-      ((r.items < sms && Tk / B >= 8 * kTile) || (r.items < 4 * sms && (Tk - Tq) / B >= 8 * kTile));
-  r.grid = r.split ? (r.units < sms ? r.units : sms) : (r.items < sms ? r.items : sms);
   const int64_t rows = Tq * group;
   r.rows_cap = static_cast<int>(rows < 2 * kTile ? rows : 2 * kTile);
+  // Whole items, or equal shares of all key tiles and a join? In key tiles
+  // (about 1.7 us each), for sequences of average length: whole items take as
+  // long as the longest, as their even share, and, where all are about as long
+  // (little of what they reach is their own diagonal), as their full turns;
+  // shares take the even share and 6 for the join, 9 for one of full items.
+  // Measured, shares against whole items in us: one token over 2048 keys of 4
+  // heads 11.2 / 22.6, 8 over 512 12.0 / 10.4, 32 over 4096 52 / 47, 64 over
+  // 2048 of 8 heads 92.5 / 96.3; 512 tokens behind 1024, 16 heads of 192, 26.9 /
+  // 31.0, a prompt of 1024 28.0 / 24.1, of 8192 on 2 heads 48 / 109.
+  const double longest = static_cast<double>(Tk) / B / kTile;
+  const double seen = static_cast<double>(Tk) - 0.5 * static_cast<double>(Tq);
+  const double average = (seen > 0 ? seen : 0) / B / kTile;
+  const double even = r.items * (average + kItemUnits) / sms;
+  double whole = longest + kItemUnits;
+  if (even > whole) whole = even;
+  if (4 * average >= 3 * longest) {
+    const double turns = static_cast<double>((r.items + sms - 1) / sms) * (average + kItemUnits);
+    if (turns > whole) whole = turns;
+  }
+  r.split = r.units < kMostUnits && even + (r.rows_cap < kTile ? 6 : 9) < whole;
+  r.grid = r.split ? (r.units < sms ? r.units : sms) : (r.items < sms ? r.items : sms);
   return r;
 }
 
