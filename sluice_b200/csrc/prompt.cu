@@ -192,25 +192,29 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
     if (blk < held) return blk < a.width ? a.table + r * a.ld_table + blk : nullptr;
     return new_block(o + (blk - held));
   };
-  // rows of a packed batch, kPlanChunk consecutive ones per warp and turn: a
-  // lane's four are looked up together, so that their loads overlap
+  // rows of a packed batch, consecutive ones per warp and turn (four a lane, or
+  // fewer where that would leave warps without any): a lane's are looked up
+  // together, so that their loads overlap
+  constexpr int kEach = kPlanChunk / 32;
   auto fill = [&](const int* cu, int64_t rows, bool all_rows) {
     const int used = cu[a.B];
-    for (int64_t c0 = static_cast<int64_t>(gwarp) * kPlanChunk; c0 < rows;
-         c0 += static_cast<int64_t>(nwarps) * kPlanChunk) {
+    const int64_t turn = static_cast<int64_t>(nwarps) * 32;
+    const int each = rows >= kEach * turn ? kEach : static_cast<int>((rows + turn - 1) / turn);
+    const int chunk = 32 * each;
+    for (int64_t c0 = static_cast<int64_t>(gwarp) * chunk; c0 < rows;
+         c0 += static_cast<int64_t>(nwarps) * chunk) {
       int lo = 0, hi = 0;
       if (c0 < used) {
         lo = find_request(cu, static_cast<int>(c0), 0, a.B - 1);
-        const int64_t last = min(c0 + kPlanChunk, min(rows, static_cast<int64_t>(used))) - 1;
+        const int64_t last = min(c0 + chunk, min(rows, static_cast<int64_t>(used))) - 1;
         hi = find_request(cu, static_cast<int>(last), lo, a.B - 1);
       }
-      constexpr int kEach = kPlanChunk / 32;
       int pos[kEach], block[kEach];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const int64_t t = c0 + lane + 32 * i;
         pos[i] = block[i] = -1;
-        if (t < rows && t < used) {
+        if (i < each && t < rows && t < used) {
           const int r = find_request(cu, static_cast<int>(t), lo, hi);
           const int context = (cu_total[r + 1] - cu_total[r]) - (cu_new[r + 1] - cu_new[r]);
           pos[i] = static_cast<int>(t) - cu[r] + (all_rows ? 0 : context);
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const int64_t t = c0 + lane + 32 * i;
-        if (t >= rows) continue;
+        if (i >= each || t >= rows) continue;
         const int64_t slot = block[i] < 0 ? -1
             : static_cast<int64_t>(block[i]) * a.bs + (pos[i] - block_index(a, pos[i]) * a.bs);
         if (all_rows) {
@@ -236,13 +240,20 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   fill(cu_new, a.T, false);
   if (a.kv_slots != nullptr) fill(cu_total, a.Tk, true);
 
-  // the table rows of the requests that take blocks: a warp per request
-  for (int r = gwarp; r < a.B; r += nwarps) {
-    const int o = off[r];
-    const Lengths l = plan_lengths(a, r);
-    if (o < 0 || l.take == 0) continue;
-    int32_t* row = a.table + static_cast<int64_t>(r) * a.ld_table + l.held;
-    for (int i = lane; i < l.take; i += 32) row[i] = *new_block(o + i);
+  // the table rows of the requests that take blocks: a lane looks at each of
+  // the warp's (nwarps apart), the warp writes a row
+  for (int r0 = gwarp; r0 < a.B; r0 += 32 * nwarps) {
+    const int r = r0 + nwarps * lane;
+    Lengths l = {};
+    if (r < a.B) l = plan_lengths(a, r);
+    const int o = r < a.B ? off[r] : -1;
+    for (unsigned takers = __ballot_sync(0xffffffffu, o >= 0 && l.take > 0); takers;
+         takers &= takers - 1) {
+      const int w = __ffs(takers) - 1;
+      const int first = __shfl_sync(0xffffffffu, o, w), n = __shfl_sync(0xffffffffu, l.take, w);
+      int32_t* row = a.table + (r0 + nwarps * w) * a.ld_table + __shfl_sync(0xffffffffu, l.held, w);
+      for (int i = lane; i < n; i += 32) row[i] = *new_block(first + i);
+    }
   }
   if (blockIdx.x == 0) {
     // offsets that a reader may follow: never past the rows that were filled
@@ -464,7 +475,7 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
   // a CTA per turn of its warps, at most one per SM; a small batch in a small
   // CTA, whose scan has fewer warps to wait for
   const int64_t rows = T + Tk;
-  const int threads = B <= 256 && rows <= 1024 ? 256 : kPlanThreads;
+  const int threads = B <= 64 && rows <= 1024 ? 256 : kPlanThreads;
   const int64_t per_cta = kPlanChunk * (threads / 32);
   int64_t grid = (rows + per_cta - 1) / per_cta;
   const int sms = sl_device_sm_count();
