@@ -334,24 +334,33 @@ struct alignas(sizeof(E) * V) RotVec {
 };
 
 // (products and sums are written out, so that every form of the kernel rounds
-// alike.) A unit is V adjacent columns of a head (interleaved: V / 2 pairs), or V
-// columns and the V columns rot / 2 further (half: V pairs). V elements are
-// one load: 16 bytes where the sizes, strides and addresses allow it.
+// alike.) A unit is two vectors of V columns, rot / 2 columns apart, V pairs:
+// element k of both (half), or the neighbours within each (interleaved; with V =
+// 1 a unit is two neighbours). A vector is one load: 16 bytes where the sizes,
+// strides and addresses allow it.
+//
+// Bound by the rows' bytes: many CTAs of few rows in flight each (6 per SM with
+// one unit a thread; 4 with two took 65 us where this takes 54, for 16384 rows of
+// 36 heads of 128 columns of bf16: 5.6 TB/s). The first rows are asked for before
+// the angles are formed. Vectors of 8, 4, 2 and 1 elements there: 54, 83, 112 and
+// 160 us, so the widest that fits is taken.
 template <typename E, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
   // (cos, sin) * factor of each token, [pair within a unit][unit]: lanes of
   // neighbouring units read neighbouring words
   extern __shared__ float2 cs[];
-  constexpr int kPairs = kInterleaved ? V / 2 : V;  // of a unit
   __shared__ int s_skip[32];
   using Vec = RotVec<E, V>;
   sl::pdl_wait();
   sl::pdl_trigger();
   const int half = a.rot >> 1;
+  // interleaved vectors hold whole pairs, or (V = 1) an element of one each
+  constexpr bool kWithin = kInterleaved && V > 1;
+  const int to_hi = kInterleaved && V == 1 ? 1 : half;  // from a unit's first vector to its second
   const int t0 = blockIdx.x * a.per_cta;
   const int nt = min(a.per_cta, a.T - t0);
   const int nq = a.t[0].heads * a.t[0].units, n = nq + a.t[1].heads * a.t[1].units;
-  constexpr int U = kInterleaved ? 2 : 1;  // items in flight per thread
+  constexpr int U = 1;  // items in flight per thread
   Vec lo[U], hi[U];
   E* dst[U];
   int pair[U];   // first pair's place in cs, -1: not rotated
@@ -372,7 +381,7 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
       const int unit = idx - head * x.units;
       int col;
       if (unit < a.rot_units) {
-        col = x.offset + unit * V;
+        col = x.offset + unit * (kInterleaved && V == 1 ? 2 : V);
         pair[u] = t * half + unit;
       } else {
         // columns that are not rotated: those before the rotated ones, then
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
       const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
       dst[u] = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
       lo[u] = *reinterpret_cast<const Vec*>(src);
-      if (!kInterleaved && pair[u] >= 0) hi[u] = *reinterpret_cast<const Vec*>(src + half);
+      if (pair[u] >= 0) hi[u] = *reinterpret_cast<const Vec*>(src + to_hi);
     }
   };
   // the first rows are on their way while the angles are formed
@@ -396,7 +405,12 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
     const double turns = static_cast<double>(p) * a.turns[j];
     float s, c;
     sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    cs[t * half + j % kPairs * a.rot_units + j / kPairs] = make_float2(c * a.factor, s * a.factor);
+    // pair j's place in its unit, and the unit
+    constexpr int kIn = V > 1 ? V / 2 : 1;
+    const int back = kWithin && j >= half / 2 ? half / 2 : 0;
+    const int k = kWithin ? (back ? kIn : 0) + (j - back) % kIn : j % V;
+    const int unit = kWithin ? (j - back) / kIn : j / V;
+    cs[t * half + k * a.rot_units + unit] = make_float2(c * a.factor, s * a.factor);
     if (j == 0) s_skip[t] = p < 0;
   }
   __syncthreads();
@@ -405,26 +419,20 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
     for (int u = 0; u < U; ++u) {
       if (token[u] < 0) continue;
       if (pair[u] >= 0 && !s_skip[token[u]]) {
-        if constexpr (kInterleaved) {
 #pragma unroll
-          for (int k = 0; k < V / 2; ++k) {
-            const float2 c = cs[pair[u] + k * a.rot_units];
-            const float x0 = to_f(lo[u].e[2 * k]), x1 = to_f(lo[u].e[2 * k + 1]);
-            lo[u].e[2 * k] = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
-            lo[u].e[2 * k + 1] = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float2 c = cs[pair[u] + k * a.rot_units];
-            const float x0 = to_f(lo[u].e[k]), x1 = to_f(hi[u].e[k]);
-            lo[u].e[k] = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
-            hi[u].e[k] = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
-          }
+        for (int k = 0; k < V; ++k) {
+          const float2 c = cs[pair[u] + k * a.rot_units];
+          constexpr int kIn = V > 1 ? V / 2 : 1;  // pairs of one vector
+          E& e0 = !kWithin ? lo[u].e[k] : k < kIn ? lo[u].e[2 * k % V] : hi[u].e[2 * k % V];
+          E& e1 = !kWithin ? hi[u].e[k]
+                           : k < kIn ? lo[u].e[(2 * k + 1) % V] : hi[u].e[(2 * k + 1) % V];
+          const float x0 = to_f(e0), x1 = to_f(e1);
+          e0 = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
+          e1 = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
         }
       }
       *reinterpret_cast<Vec*>(dst[u]) = lo[u];
-      if (!kInterleaved && pair[u] >= 0) *reinterpret_cast<Vec*>(dst[u] + half) = hi[u];
+      if (pair[u] >= 0) *reinterpret_cast<Vec*>(dst[u] + to_hi) = hi[u];
     }
     i0 += U * kRotThreads;
     if (i0 >= nt * n) break;
@@ -441,10 +449,7 @@ cudaError_t launch_rotary(const RotArgs& a, int v, dim3 grid, size_t smem, cudaS
       return cudaErrorInvalidValue;
     case 4: return sl::launch(rotary_kernel<E, 4, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
     case 2: return sl::launch(rotary_kernel<E, 2, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
-    default:
-      if constexpr (!kInterleaved)
-        return sl::launch(rotary_kernel<E, 1, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
-      return cudaErrorInvalidValue;
+    default: return sl::launch(rotary_kernel<E, 1, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
   }
 }
 
@@ -520,7 +525,7 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
   const int size = dtype == SL_DTYPE_FP32 ? 4 : 2;
   // the widest unit that divides every size, stride and address
   auto fits = [&](int v) {
-    if ((interleaved ? rot : rot / 2) % v || (interleaved && v < 2)) return false;
+    if (rot % (2 * v)) return false;
     for (const sl_rotary_part* p : parts) {
       if (p->heads == 0) continue;
       const int64_t all = static_cast<int64_t>(p->dim) | p->offset | p->x_token | p->x_head |
@@ -533,16 +538,13 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
   };
   int v = 16 / size;
   while (v > 1 && !fits(v)) v >>= 1;
-  // interleaved pairs sit in one unit: a tensor that starts in the middle of
-  // a pair's alignment is refused rather than split
-  if (!fits(v)) return SL_ERR_UNSUPPORTED;
   RotArgs a = {};
   a.positions = positions;
   a.turns = turns;
   a.factor = factor;
   a.T = T;
   a.rot = rot;
-  a.rot_units = (interleaved ? rot : rot / 2) / v;
+  a.rot_units = rot / 2 / v;
   int items = 0;
   for (int i = 0; i < 2; ++i) {
     const sl_rotary_part* p = parts[i];

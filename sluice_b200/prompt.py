@@ -245,18 +245,17 @@ class Rotary:
         """(the call's description of one tensor, its output, its input)."""
         in_place = out is x
         copied, x_strides, new = _rotary_input(name, x.shape, x.stride(), offset, T,
-                                               self.rotary_dim, self.interleaved)
-        if out is None and new is not None and not (
-                self.interleaved and x.data_ptr() % (2 * x.element_size())):
+                                               self.rotary_dim)
+        if out is None and new is not None:
             # the usual call: a new output like a contiguous input
             out = torch.empty_like(x)
             part = _lib.RotaryPart.from_buffer_copy(new)
             part.x, part.y = x.data_ptr(), out.data_ptr()
             return part, out, x
-        if copied or (self.interleaved and x.data_ptr() % (2 * x.element_size())):
+        if copied:
             if in_place:
                 raise ValueError(f"{name} cannot be rotated in place: its columns must be "
-                                 "contiguous and its pairs aligned")
+                                 "contiguous")
             x = x.clone(memory_format=torch.contiguous_format)
             x_strides = x.stride()
         if out is None:
@@ -305,7 +304,7 @@ class Rotary:
 
 
 @functools.lru_cache(maxsize=512)
-def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int, interleaved: bool):
+def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int):
     """(whether the input has to be copied first, its strides, and, for a
     contiguous input, the description of a call that writes a new tensor,
     without the addresses), by its layout."""
@@ -314,9 +313,7 @@ def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int, inte
     if not 0 <= offset <= shape[2] - rot:
         raise ValueError(f"{name}'s columns [{offset}, {offset + rot}) are not within its "
                          f"{shape[2]}")
-    # pairs are read as two elements at once, so they start on even ones
-    odd = interleaved and any(s % 2 for s, n in zip(strides[:2], shape) if n > 1)
-    copied = (shape[2] > 1 and strides[2] != 1) or odd
+    copied = shape[2] > 1 and strides[2] != 1
     new = None
     if not copied and strides == (shape[1] * shape[2], shape[2], 1):
         new = _lib.RotaryPart(None, None, strides[0], strides[1], strides[0], strides[1],

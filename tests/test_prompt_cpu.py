@@ -190,9 +190,9 @@ def test_rotary_refuses():
     buf = torch.zeros(5, 2, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="overlaps"):
         r(pos, buf[:4], out_q=buf[1:])
-    odd = torch.zeros(4, 2, 129, dtype=torch.bfloat16)[..., 1:]
+    wide = torch.zeros(4, 2, 256, dtype=torch.bfloat16)[..., ::2]
     with pytest.raises(ValueError, match="in place"):
-        r(pos, odd, out_q=odd)
+        r(pos, wide, out_q=wide)
 
 
 def test_c_entries_refuse_without_a_gpu():

@@ -267,6 +267,8 @@ def test_rotary_leaves_padding_rows_and_other_layouts():
             keep = odd.clone()
             assert torch.equal(r(pos, odd), r(pos, odd.contiguous()))
             assert torch.equal(odd, keep)
+            r(pos, odd, out_q=odd)   # in place, whatever the alignment
+            assert torch.equal(odd, r(pos, keep))
     empty = torch.empty(0, 2, 64, device="cuda")
     assert r(torch.empty(0, dtype=torch.long, device="cuda"), empty).shape == empty.shape
 
