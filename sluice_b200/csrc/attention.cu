@@ -4,24 +4,42 @@
 //   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(scale q_i . k_j - m_i),
 //   j <= i + keys - queries
 //
-// One pass over the keys with a running maximum m and sum (the sum of the
-// rounded-off weights is never formed again). An item is 2 x 128 rows of one
-// sequence and key head; its rows are (token, head of the group) pairs, so a
-// single token of a wide group fills rows that would otherwise be empty, and
-// a key tile is read once for all heads of its group. Per item and 128-key
-// tile: S = Q K^T (128 x 128 per 128 rows, fp32, in TMEM), the softmax
-// warpgroup of those rows reads a row per thread, writes the weights P over S
-// in the inputs' type, and O += P V takes P from TMEM. The two halves of an
-// item run half a step apart: while one half's weights are formed the tensor
-// core works for the other.
+// One pass over the keys with a running maximum m and a running sum, both in 32
+// bits; the weights are rounded once, to the inputs' type, as the second
+// product's operand. An item is 2 x 128 rows of one sequence and key head; its
+// rows are (token, head of the group) pairs, so a single token of a wide group
+// fills rows that would otherwise be empty, and a key tile is read once for all
+// heads of its group. Per item and 128-key tile: S = Q K^T (128 x 128 per 128
+// rows, fp32, in TMEM), the softmax warpgroup of those rows reads a row per
+// thread, writes the weights P over S, and O += P V takes P from TMEM.
 //
 // Roles (12 warps): 0-3 and 4-7 softmax of the two halves (a row per thread)
 // and their output; 8 and 11 issue the MMAs of a half each; 9 the tile loads
-// (TMA); 10 cleans the value tiles that hold keys which some row may not see.
+// (TMA); 10 publishes the stretches of work one ahead and cleans the value tiles
+// that hold keys which some row may not see.
 //
 // Shared memory: the item's queries (2 x 128 rows) and a ring of 16 KB slots
 // that the key and value tiles pass through: 64 columns of 128 keys, or 64
-// values rows of 128 columns.
+// value rows of 128 columns.
+//
+// What bounds it. A tile of both halves is 2048 cycles of MMAs (dim 128; 2560 at
+// 192) and 2048 of exponentials (16 a cycle and SM). One half's chain - scores,
+// maximum, exponentials, hand-over, both products - is longer than either, so
+// the halves run half a step apart: their warps take turns at the exponentials
+// (without the turns both wait for the special-function units, then both for the
+// tensor core: 4096 tokens on 16 heads of 192 / 128 took 95 us instead of 74).
+// Then the hand-overs count: named barriers instead of mbarriers between warps,
+// waits without a suspend hint or a vote (82 -> 74 us), the maximum taken outside
+// the turn (16384 tokens on 32 / 4 heads of 128: 1.93 -> 1.77 ms). Now, device time:
+//   4096 tokens, 16 heads of 192 / 128        73 us, 1170 TFLOP/s, 0.71 of cuBLAS's burst
+//   16384 tokens, 32 / 4 heads of 128       1.77 ms, 1240 TFLOP/s, 0.91 of cuBLAS's
+//                                             sustained rate (the power cap; 1.60 ms before)
+//   8 single tokens over 60 000 keys, 32 / 4  33 us, 19 of them the bytes; 8 until the first
+//                                             scores are there, 5 for the join
+// Measured and not kept: part of the exponentials as a cubic on the FMA pipes
+// (73.5 us with a quarter against 72.5), 16 softmax warps with a row in two
+// threads (90 against 82), the turn passed on after half the weights (80
+// against 74), the scores waited for within the turn (85 against 82).
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
@@ -75,7 +93,8 @@ struct Params {
   int64_t v_token, v_head;
   int B, Tq, Tk, heads, kv_heads, group, half_tokens;  // tokens of a half: 128 / group
   int shared;                        // the last 64 key columns come from ks
-  int wide;                          // the output's rows are 32-byte aligned
+  int wide;                          // the output's rows are 32-byte aligned: stores of 32 bytes
+                                     // (2048 tokens, 16 heads of 128: 38.8 us, of 16 bytes 40.8)
   int grid;                          // CTAs
   Divisor by_tokens, by_heads, by_grid;  // tokens of an item, key heads, CTAs
   int split;                         // 1: equal shares of all key tiles per CTA
@@ -277,7 +296,8 @@ struct Seg {
 };
 
 // Where an item's rows fill one half only, both halves take them, each every
-// other key tile of the stretch, and their results are joined at its end.
+// other key tile of the stretch, and their results are joined at its end (short
+// prompts with such tails 38 -> 36 us; from two tiles on, so that each has one).
 __device__ __forceinline__ bool is_twin(const Seg& g) { return g.nh[1] == 0 && g.j1 - g.j0 >= 2; }
 
 struct Seq {
@@ -448,8 +468,9 @@ __device__ __noinline__ int2 pick_item(const Params& p, int ord) {
 }
 
 // Walks a CTA's share of the work.
-//   whole items: the longest first (of up to 32 sequences; of more, sequence
-//   after sequence), dealt out in turns that go back and forth;
+//   whole items: the longest first (of up to 32 sequences, a lane each; of more,
+//   sequence after sequence), dealt out in turns that go back and forth (16
+//   prompts of 1 to 1024 tokens: 28 us, sequence after sequence 37);
 //   split: an equal run of key tiles, item after item.
 struct Walk {
   int total, at, end, round, unit0;  // unit0: the first unit of the last stretch's item

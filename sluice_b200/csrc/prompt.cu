@@ -18,6 +18,11 @@ namespace {
 // free ring, not from the table, so no CTA waits for another's table writes;
 // the ring's range is read by all and written by none of a launch of several
 // CTAs that updates it in place (plan_range_kernel then writes it).
+//
+// Bound by latency: the lengths, the scan, a search and a table entry follow one
+// another. Eight single tokens take 3.5 us, 256 take 4.1, 72 000 rows 6.2, 2.2
+// million (17 MB, 2.6 us at copy bandwidth) 16; with a row a lane at a time and
+// one warp for the table the last two took 35 and 40 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxRequests = 8192;
 constexpr int kPlanChunk = 128;  // consecutive rows that a warp fills in a turn, four a lane
@@ -477,15 +482,21 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
   PlanArgs a = {context_lens, new_lens, B, block_size, shift, table_width, num_free_slots, T, Tk,
                 block_table, ld_table, free_blocks, free_range, free_range_out, cu_new, cu_total,
                 positions, slots, Tk > 0 ? kv_slots : nullptr, status, 1};
-  // a CTA per turn of its warps, at most one per SM; a small batch in a small
-  // CTA, whose scan has fewer warps to wait for
+  // Warps for a turn of the rows, up to 32 per SM. In small CTAs a scan has fewer
+  // warps to wait for, in large ones fewer CTAs repeat it and there are more lanes
+  // for it (us with 256, 512, 1024 threads): 8 requests 3.5, 3.7, 4.3; 256 of 64
+  // rows 4.8, 5.2, 6.7; 1024 of 64 rows 7.5, 6.6, 7.4; 1024 of 2.2 million rows
+  // together, several turns a warp, 20.6, 17.9, 16.1.
   const int64_t rows = T + Tk;
-  const int threads = B <= 64 && rows <= 1024 ? 256 : kPlanThreads;
-  const int64_t per_cta = kPlanChunk * (threads / 32);
-  int64_t grid = (rows + per_cta - 1) / per_cta;
   const int sms = sl_device_sm_count();
   if (sms <= 0) return SL_ERR_CUDA;
-  grid = grid < 1 ? 1 : (grid > sms ? sms : grid);
+  const int threads = rows > static_cast<int64_t>(sms) * 32 * kPlanChunk ? kPlanThreads
+                      : B <= 256                                         ? 256
+                                                                         : 512;
+  const int64_t per_cta = kPlanChunk * (threads / 32);
+  const int64_t most = static_cast<int64_t>(sms) * (kPlanThreads / threads);
+  int64_t grid = (rows + per_cta - 1) / per_cta;
+  grid = grid < 1 ? 1 : (grid > most ? most : grid);
   const bool in_place = ring && free_range_out == free_range;
   a.write_range = !(in_place && grid > 1);
   const size_t smem = sizeof(int) * (3 * static_cast<size_t>(B) + 2);
