@@ -349,10 +349,14 @@ class DecoderHarness:
         positions, which advance by ``lengths``. Returns the greedy next ids
         [batch] behind each sequence's last token (-1 for a sequence without
         tokens). ``context`` are the positions, where the caller knows them;
-        otherwise they are read back. CUDA with the fused attention only; the
+        otherwise they are read back. Raises ``KvPlanError``, with nothing
+        changed, where the pool has too few blocks left or a position before
+        the new tokens has none. CUDA with the fused attention only; the
         MoE layers take the pass as one step of T rows."""
         if not self.fused_attention:
             raise ValueError("prefill runs on a CUDA device with the fused attention")
+        from ._lib import KV_PLAN_BAD_INPUT
+        from .prompt import KvPlanError
         cfg, dev = self.cfg, self.device
         if len(lengths) != self.batch or any(n < 0 for n in lengths):
             raise ValueError(f"lengths must be {self.batch} counts")
@@ -382,6 +386,11 @@ class DecoderHarness:
                           T + sum(seen) if has_context else 0)
         try:
             plan.check()
+            # positions that the caller's context or an earlier step without a
+            # block left without a cache row
+            rows = plan.slots if plan.kv_slots is None else torch.cat([plan.slots, plan.kv_slots])
+            if int(rows.min()) < 0:
+                raise KvPlanError(KV_PLAN_BAD_INPUT)
         except RuntimeError:
             self.restore_blocks(blocks0)
             raise

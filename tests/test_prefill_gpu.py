@@ -152,6 +152,16 @@ def test_pool_that_runs_out():
     with pytest.raises(prompt.KvPlanError):
         h.check_blocks()
     assert h.block_table[:, 1].tolist() == [3, -1, -1]
+    # a prompt goes on only behind positions that have cache rows: sequence 2's
+    # last one found no block, and no sequence may be said to be further than
+    # its blocks reach
+    state = [t.clone() for t in (h.cache, h.block_table, h.free_range)]
+    for lengths, context in (([0, 0, 3], None), ([3, 3, 3], [33, 21, 33]), ([0, 5, 0], [0, 40, 0])):
+        with pytest.raises(prompt.KvPlanError):
+            h.prefill(torch.cat(_tokens(lengths)).cuda(), lengths, context=context)
+        assert all(torch.equal(a, b) for a, b in zip(state, (h.cache, h.block_table, h.free_range)))
+    h.prefill(torch.cat(_tokens([4, 11, 0])).cuda(), [4, 11, 0])
+    assert h.pos.tolist() == [37, 32, 33]
 
 
 def test_prefill_refuses():
