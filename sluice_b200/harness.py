@@ -479,6 +479,10 @@ class OffloadedDecoder:
         (``DecoderHarness.prefill``; the MoE layers' steps beyond the slot
         envelope run in expert waves); the sequences that had tokens go on
         from their greedy next ids. One GPU only."""
+        from .ep import EPDecodeStack
+        if isinstance(self.stack, EPDecodeStack):
+            # (its exchanges want the same number of rows on every rank)
+            raise ValueError("prefill takes the MoE layers of one GPU, not an EPDecodeStack")
         nxt = self.model.prefill(ids, lengths, context)
         self._ids.copy_(torch.where(nxt >= 0, nxt, self._ids))
         return nxt

@@ -257,3 +257,12 @@ def test_c_entries_refuse_without_a_gpu():
     assert att(q=264) == BAD and att(k_token=132) == BAD and att(dim=192, shared_dim=64) == BAD
     assert L.sl_prompt_attention_workspace_bytes(0, 1, 1, 1, 1, 64) == 0
     assert L.sl_prompt_attention_workspace_bytes(1, 1, 1, 1, 1, 64) >= 256
+
+
+def test_prefill_refuses_expert_parallel_layers():
+    from sluice_b200.ep import EPDecodeStack
+    from sluice_b200.harness import OffloadedDecoder
+    d = OffloadedDecoder.__new__(OffloadedDecoder)
+    d.stack = EPDecodeStack.__new__(EPDecodeStack)
+    with pytest.raises(ValueError, match="EPDecodeStack"):
+        d.prefill(torch.zeros(2, dtype=torch.long), [1, 1])
