@@ -108,7 +108,8 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     """Give every request the cache blocks its new tokens need and map the
     batch's tokens to cache rows.
 
-    ``context_lens`` / ``new_lens`` int32 [B]: tokens cached and to add.
+    ``context_lens`` / ``new_lens`` int32 [B], B at most 8192: tokens cached and
+    to add.
     ``block_table`` int32 [B, width]: row r's first ceil(context / block_size)
     entries are its blocks; the blocks it takes are written behind them.
     ``free_blocks`` int32 [N] is a ring of free block ids whose entries
@@ -143,6 +144,8 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
         free_range_out = free_range
     else:
         _vector("free_range_out", free_range_out, torch.int64, 2)
+        if abs(free_range_out.data_ptr() - free_range.data_ptr()) == 8:
+            raise ValueError("free_range_out overlaps half of free_range")
     if num_tokens < 0 or num_kv_tokens < 0:
         raise ValueError("num_tokens and num_kv_tokens are counts")
     dev = _device_index(context_lens, new_lens, block_table, free_blocks, free_range,
@@ -270,7 +273,7 @@ class Rotary:
                 raise ValueError(f"out_{name} overlaps {name}; pass {name} itself to rotate it "
                                  "in place")
         y_strides = out.stride()
-        if 0 in y_strides and any(s == 0 and n > 1 for s, n in zip(y_strides, out.shape)):
+        if not _own_rows(out.shape, y_strides):
             raise ValueError(f"out_{name} has rows that share memory")
         _, heads, dim = x.shape
         return _lib.RotaryPart(x.data_ptr(), out.data_ptr(), x_strides[0], x_strides[1],
@@ -290,13 +293,18 @@ class Rotary:
             raise ValueError("q and k must share one of bfloat16, float16, float32")
         T = positions.numel()
         _vector("positions", positions, torch.int64)
-        _no_gradient(q, k)
+        _no_gradient(q, k, out_q, out_k)
         if k is None and out_k is not None:
             raise ValueError("out_k without k")
+        given_q, given_k = out_q, out_k
         pq, out_q, q = self._part("q", q, out_q, q_offset, T)
         pk = None
         if k is not None:
             pk, out_k, k = self._part("k", k, out_k, k_offset, T)
+            if given_q is not None and (_meet(out_q, k) or _meet(out_q, out_k)):
+                raise ValueError("out_q overlaps k or out_k")
+            if given_k is not None and _meet(out_k, q):
+                raise ValueError("out_k overlaps q")
         _call(_device_index(q, positions, k, self.turns), "sl_rotary", ptr(positions),
               ptr(self.turns), T, self.rotary_dim, self.interleaved, self.factor, dtype,
               ctypes.byref(pq), None if pk is None else ctypes.byref(pk))
@@ -329,6 +337,41 @@ def _ranges_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
 
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [T, heads, columns] tensors with contiguous columns may
+    share memory: their address ranges meet, and not just because they are
+    different columns, or heads, of the rows of one buffer."""
+    if not _ranges_meet(a, b):
+        return False
+    apart, rest = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    if rest or a.element_size() != b.element_size():
+        return True
+    for d in range(2):
+        # every address modulo the step of a token, or of a head (a divisor of
+        # the tokens')
+        step = a.stride(d)
+        if step <= 0 or b.stride(d) != step or \
+                (d == 1 and any(t.shape[0] > 1 and t.stride(0) % step for t in (a, b))):
+            continue
+        of_a, of_b = (1 + sum((n - 1) * s for n, s in zip(t.shape[d + 1:], t.stride()[d + 1:]))
+                      for t in (a, b))
+        if of_a <= apart % step and apart % step + of_b <= step:
+            return False
+    return True
+
+
+@functools.lru_cache(maxsize=512)
+def _own_rows(shape, strides) -> bool:
+    """Whether every row (contiguous columns) of such a layout has memory of
+    its own: each step goes past all that is inside it."""
+    inner = shape[-1]
+    for step, n in sorted((s, n) for s, n in zip(strides[:-1], shape) if n > 1):
+        if step < inner:
+            return False
+        inner += step * (n - 1)
+    return True
 
 
 # ---------------------------------------------------------------- attention
@@ -388,6 +431,8 @@ def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
         raise ValueError(f"out must be [{Tq}, {heads}, {v_dim}], got {tuple(out[0])}")
     elif out[1][2] != 1 or any(s % 8 or s <= 0 for s, n in zip(out[1][:2], out[0]) if n > 1):
         raise ValueError("out needs contiguous columns and strides in multiples of 8 elements")
+    elif not _own_rows(*out):
+        raise ValueError("out has rows that share memory")
     a = _lib.AttentionArgs()
     a.q_token, a.q_head = _strides(*q)
     a.k_token, a.k_head = _strides(*k)
@@ -424,14 +469,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     [B + 1]); its queries are its last tokens, so a prompt behind a cached
     beginning, or a single next token, has fewer queries than keys. With
     ``k_shared`` [Tk, 64] (dim 192), ``k`` has the first 128 columns and the
-    last 64 are one row for all heads. ``scale`` defaults to dim^-0.5. A query
+    last 64 are one row for all heads. ``scale`` (positive) defaults to dim^-0.5. A query
     that sees no key gets zeros; rows of ``q`` outside every sequence leave
     ``out`` as it was there (a new ``out`` is not initialised).
     """
     for name, t in (("k", k), ("v", v), ("k_shared", k_shared), ("out", out)):
         if t is not None and t.dtype != q.dtype:
             raise ValueError(f"{name} is {t.dtype}, q is {q.dtype}")
-    _no_gradient(q, k, v, k_shared)
+    _no_gradient(q, k, v, k_shared, out)
     q, k, v = _tiled(q), _tiled(k), _tiled(v)
     if k_shared is not None:
         k_shared = _tiled(k_shared)

@@ -100,6 +100,9 @@ def test_plan_oracle_is_a_block_allocator():
         assert got[6] == head + len(ring) - len(free)
 
 
+_THREE = torch.tensor([0, 8, 8])
+
+
 def _plan_args(B=2, width=4):
     return dict(context_lens=torch.zeros(B, dtype=torch.int32),
                 new_lens=torch.ones(B, dtype=torch.int32),
@@ -117,6 +120,7 @@ def _plan_args(B=2, width=4):
     dict(free_range=torch.tensor([0, 8], dtype=torch.int32)),
     dict(free_blocks=torch.zeros(16, dtype=torch.int32)[::2]), dict(num_tokens=-1),
     dict(free_range_out=torch.zeros(3, dtype=torch.int64)),
+    dict(free_range=_THREE[:2], free_range_out=_THREE[1:]),
     dict(free_blocks=None), dict(free_range=None),
     dict(free_blocks=None, free_range=None, free_range_out=torch.tensor([0, 8])),
     dict(free_blocks=None, free_range=None),   # (CPU tensors)
@@ -266,3 +270,38 @@ def test_prefill_refuses_expert_parallel_layers():
     d.stack = EPDecodeStack.__new__(EPDecodeStack)
     with pytest.raises(ValueError, match="EPDecodeStack"):
         d.prefill(torch.zeros(2, dtype=torch.long), [1, 1])
+
+
+def test_rotary_refuses_outputs_over_the_other_tensor():
+    r = prompt.Rotary(64, device="cpu")
+    pos = torch.arange(4)
+    fused = torch.zeros(4, 5 * 64, dtype=torch.bfloat16)
+    q, k = fused[:, :192].view(4, 3, 64), fused[:, 192:].view(4, 2, 64)
+    for bad in (dict(q=k, k=k, out_q=k, out_k=k),             # rotated twice
+                dict(q=torch.zeros_like(q), k=k, out_q=fused[:, 64:256].view(4, 3, 64)),
+                dict(q=q, k=k, out_k=fused[:, :128].view(4, 2, 64)),
+                dict(q=q, k=q, out_q=fused.new_empty(4, 3, 64),
+                     out_k=torch.as_strided(q, (4, 3, 64), (320, 32, 1)))):
+        with pytest.raises(ValueError, match="overlaps|share"):
+            r(pos, **bad)
+    # columns, or heads, of one buffer do not meet: only the device is refused
+    rows = torch.zeros(4, 3, 128, dtype=torch.bfloat16)
+    for a, b in ((q, k), (q[:1], k[:1]), (rows[..., :64], rows[..., 64:]),
+                 (rows[:1, :, 64:], rows[:1, :, :64])):
+        with pytest.raises(ValueError, match="CUDA"):
+            r(pos[:a.shape[0]], a, b, out_q=a, out_k=b)
+
+
+def test_outputs_whose_rows_share_memory_are_refused():
+    buf = torch.zeros(8 * 4 * 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share"):
+        prompt.prompt_attention(**_qkv(), out=buf.as_strided((8, 4, 128), (256, 64, 1)))
+    with pytest.raises(ValueError, match="share"):
+        prompt.prompt_attention(**_qkv(), out=buf.as_strided((8, 4, 128), (128, 128, 1)))
+    with pytest.raises(ValueError, match="backward"):
+        prompt.prompt_attention(**_qkv(), out=torch.zeros(8, 4, 128, dtype=torch.bfloat16,
+                                                          requires_grad=True))
+    with pytest.raises(ValueError, match="share"):
+        x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+        prompt.Rotary(64, device="cpu")(torch.arange(4), x,
+                                        out_q=buf.as_strided((4, 2, 64), (64, 64, 1)))

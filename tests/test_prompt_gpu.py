@@ -1,6 +1,7 @@
 """The prompt pass's operators against their 64-bit and integer oracles."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -582,3 +583,116 @@ def test_attention_repeats_bit_for_bit():
     first = prompt.prompt_attention(q, k, v, cu_q, cu_k)
     for _ in range(5):
         assert torch.equal(prompt.prompt_attention(q, k, v, cu_q, cu_k), first)
+
+
+@pytest.mark.parametrize("B", [32, 33, 300, 700])
+@pytest.mark.parametrize("most", [3, 150])
+def test_attention_of_many_sequences(B, most):
+    """Lengths from none to ``most`` tokens, some behind a beginning, sequences
+    without queries or keys among them, more of them than the work table has
+    entries."""
+    g = torch.Generator().manual_seed(B + most)
+    q_lens = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    k_lens = [n + int(c) for n, c in zip(q_lens, torch.randint(0, most, (B,), generator=g))]
+    k_lens[3] = 0
+    _check_attention(q_lens, k_lens, 2, 1, 128, 128, seed=B)
+
+
+# ------------------------------------------------------------- all together
+def test_steps_of_all_three_in_one_graph():
+    """Plan, rotary positions, cache and attention captured as one step of a
+    padded batch; each replay has other lengths, down to none at all."""
+    B, T, Tk, bs, width, heads, kv_heads, dim = 4, 256, 700, 32, 9, 4, 2, 128
+    gen = _gen(21)
+    spare = B * width * bs   # the cache row of padding
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.randperm(B * width, device="cuda", generator=gen).int().view(B, width)
+    context, new = torch.zeros(B, **i32), torch.zeros(B, **i32)
+    q, k, v = (torch.empty(T, n, dim, device="cuda", dtype=torch.bfloat16)
+               for n in (heads, kv_heads, kv_heads))
+    kc, vc = (torch.zeros(spare + 1, kv_heads, dim, device="cuda", dtype=torch.bfloat16)
+              for _ in range(2))
+    out = torch.empty(T, heads, dim, device="cuda", dtype=torch.bfloat16)
+    rot = prompt.Rotary(64)
+
+    def step():
+        plan = prompt.plan_kv_blocks(context, new, table, None, None, bs, T, num_kv_tokens=Tk)
+        rot(plan.positions, q, k, q_offset=64, k_offset=64, out_q=q, out_k=k)
+        rows = torch.where(plan.slots < 0, spare, plan.slots)
+        kc.index_copy_(0, rows, k)
+        vc.index_copy_(0, rows, v)
+        rows = torch.where(plan.kv_slots < 0, spare, plan.kv_slots)
+        prompt.prompt_attention(q, kc[rows], vc[rows], plan.cu_new, plan.cu_total, out=out)
+        context.add_(new)
+        return plan
+
+    def fill():
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, device="cuda", generator=gen))
+        out.fill_(7.0)
+
+    fill()
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan = step()
+    context.zero_()
+    keys = [k[:0].clone() for _ in range(B)]
+    values = [v[:0].clone() for _ in range(B)]
+    for lens in ([100, 1, 0, 155], [20, 1, 30, 1], [1, 1, 1, 1], [0, 0, 0, 0], [0, 250, 1, 5]):
+        fill()
+        new.copy_(torch.tensor(lens))
+        pos = torch.cat([torch.arange(len(keys[b]), len(keys[b]) + n) for b, n in enumerate(lens)]
+                        + [torch.full((T - sum(lens),), -1)]).cuda()
+        want_q, want_k = rot(pos, q, k, q_offset=64, k_offset=64)
+        g.replay()
+        torch.cuda.synchronize()
+        plan.check()
+        assert torch.equal(plan.positions, pos)
+        assert torch.equal(q, want_q) and torch.equal(k, want_k)
+        at = 0
+        for b, n in enumerate(lens):
+            keys[b] = torch.cat([keys[b], k[at:at + n]])
+            values[b] = torch.cat([values[b], v[at:at + n]])
+            at += n
+        k_lens = [len(x) for x in keys]
+        assert context.tolist() == k_lens and plan.cu_total.tolist()[-1] == sum(k_lens)
+        assert out[at:].eq(7.0).all()
+        if at == 0:
+            continue
+        ref, mag = oprompt.attention(q[:at], torch.cat(keys), torch.cat(values), lens, k_lens,
+                                     1 / math.sqrt(dim))
+        tol = _bounds(ref, mag, torch.bfloat16, max(k_lens), torch.cat(values).abs().max().item())
+        assert ((out[:at].double() - ref).abs() <= tol).all()
+
+
+def test_two_threads_at_once():
+    """Calls of two host threads, each on a stream of its own, keep apart."""
+    def inputs(seed):
+        q, k, v, _, cu_q, cu_k = _inputs([70 + seed, 1], [300, 900 + seed], 4, 2, 128, 128, 0,
+                                         torch.bfloat16, seed)
+        return q, k, v, cu_q, cu_k, torch.arange(len(q), device="cuda")
+
+    rot = prompt.Rotary(128, interleaved=False)
+    cases = [inputs(s) for s in (1, 2)]
+
+    def run(q, k, v, cu_q, cu_k, pos):
+        return prompt.prompt_attention(rot(pos, q), k, v, cu_q, cu_k)
+
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                if not torch.equal(run(*cases[i]), want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
