@@ -423,11 +423,9 @@ __device__ __forceinline__ void uniform(Seg& g) {
   g.lim0 = __shfl_sync(kAll, g.lim0, 0);
 }
 
-// How many items of a sequence reach x key tiles or more (they are its last
-// ones: what an item reaches grows with its place).
-__device__ __forceinline__ int items_from(const Params& p, const Seq& s, int x) {
-  const int nt = tiles_of(p, s);
-  if (x <= 0) return nt;
+// How many of a sequence's nt items reach x > 0 key tiles or more (they are its
+// last ones: what an item reaches grows with its place).
+__device__ __forceinline__ int items_from(const Params& p, const Seq& s, int nt, int x) {
   const int need = (x - 1) * kTile + 1;  // keys that the item's last row sees, at least
   if (nt == 0 || s.k_len < need) return 0;
   const int m = need - (s.k_len - s.q_len);  // ... which is so from this row on
@@ -442,20 +440,25 @@ __device__ __noinline__ int2 pick_item(const Params& p, int ord) {
   const int lane = threadIdx.x & 31;
   Seq mine = {0, 0, 0, 0};
   if (lane < p.B) mine = load_seq(p, lane);
-  // the largest x that more than ord items reach
-  int x = 0, past = 0;  // past: items that reach hi
+  // the largest x that more than ord items reach; from: this lane's that do,
+  // more: those that reach further
+  const int nt = tiles_of(p, mine);
+  int x = 0, from = nt, more = 0, past = 0;  // past: all lanes' that reach further
   int hi = __reduce_max_sync(kAll, (mine.k_len + kTile - 1) / kTile) + 1;
   while (hi - x > 1) {
     const int mid = (x + hi) >> 1;
-    const int n = __reduce_add_sync(kAll, items_from(p, mine, mid));
+    const int mine_from = items_from(p, mine, nt, mid);
+    const int n = __reduce_add_sync(kAll, mine_from);
     if (n > ord) {
       x = mid;
+      from = mine_from;
     } else {
       hi = mid;
       past = n;
+      more = mine_from;
     }
   }
-  const int from = items_from(p, mine, x), own = from - items_from(p, mine, x + 1);
+  const int own = from - more;
   int v = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -464,7 +467,7 @@ __device__ __noinline__ int2 pick_item(const Params& p, int ord) {
   }
   const int rest = ord - past;
   const int l = max(0, __ffs(__ballot_sync(kAll, v > rest)) - 1);
-  return make_int2(l, __shfl_sync(kAll, tiles_of(p, mine) - from + rest - (v - own), l));
+  return make_int2(l, __shfl_sync(kAll, nt - from + rest - (v - own), l));
 }
 
 // Walks a CTA's share of the work.
@@ -847,9 +850,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         weights(0, 32);
         tmem_st32(s_at, r);
         hand_over(0);
-        weights(32, 64);
-        tmem_st32(s_at + 32, r + 32);
+        // (the other half's first exponentials come in behind the last ones)
+        weights(32, 60);
         pass_turn();
+        weights(60, 64);
+        tmem_st32(s_at + 32, r + 32);
         hand_over(1);
         l += sum.x + sum.y;
         ++n_s;
