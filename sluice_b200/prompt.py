@@ -47,9 +47,10 @@ def _device_index(first: torch.Tensor, *others) -> int:
 
 def _no_gradient(*tensors) -> None:
     """Refuse what autograd would silently cut off."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("this operator has no backward pass: call it under torch.no_grad(), or "
-                         "with detached tensors")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("this operator has no backward pass: call it under torch.no_grad(), "
+                             "or with detached tensors")
 
 
 def _call(dev: int, name: str, *args) -> None:
@@ -57,10 +58,11 @@ def _call(dev: int, name: str, *args) -> None:
     ``dev``, which is made the current one where it is not."""
     fn = getattr(lib(), name)
     if torch.cuda.current_device() == dev:
-        check(fn(*args, _raw_stream(dev)), name)
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, _raw_stream(dev)), name)
+            rc = fn(*args, _raw_stream(dev))
+    check(rc, name)
 
 
 def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, length: int | None = None) -> None:
@@ -124,8 +126,8 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     the ring or its table row cannot hold takes nothing and its new tokens get
     slot -1; ``KvPlan.check`` raises for it.
     """
-    B = context_lens.numel()
     _vector("context_lens", context_lens, torch.int32)
+    B = len(context_lens)
     _vector("new_lens", new_lens, torch.int32, B)
     if (free_blocks is None) != (free_range is None) or \
             (free_blocks is None and free_range_out is not None):
@@ -133,11 +135,11 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     if free_blocks is not None:
         _vector("free_blocks", free_blocks, torch.int32)
         _vector("free_range", free_range, torch.int64, 2)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
-            block_table.stride(1) != 1 or block_table.shape[0] != B:
+    shape, strides = block_table.shape, block_table.stride()
+    if block_table.dtype != torch.int32 or len(shape) != 2 or strides[1] != 1 or shape[0] != B:
         raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows")
-    width = block_table.shape[1]
-    ld = block_table.stride(0) if B > 1 else width
+    width = shape[1]
+    ld = strides[0] if B > 1 else width
     if ld < width:
         raise ValueError("block_table's rows overlap")
     if free_range_out is None:
@@ -383,7 +385,6 @@ def _tiled(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-@functools.lru_cache(maxsize=512)
 def _tile_strides(shape, strides) -> bool:
     return (shape[-1] <= 1 or strides[-1] == 1) and \
         all(s % 8 == 0 and s > 0 for s, n in zip(strides[:-1], shape) if n > 1)
@@ -403,7 +404,8 @@ def _strides(shape, strides) -> list[int]:
 @functools.lru_cache(maxsize=512)
 def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
     """The call's description by its tensors' layouts, each (shape, strides)
-    (``k_shared`` None; ``out`` None: a new one), without the addresses."""
+    (``k_shared`` None; ``out`` None: a new one), without the addresses; the
+    output's shape; whether the tile loads take the inputs' strides."""
     if len(q[0]) != 3 or len(k[0]) != 3 or len(v[0]) != 3:
         raise ValueError("q, k and v are [tokens, heads, dim]")
     Tq, heads, dim = q[0]
@@ -444,7 +446,8 @@ def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
     a.heads, a.kv_heads, a.dim, a.v_dim, a.shared_dim = heads, kv_heads, dim, v_dim, shared
     a.dtype = _DTYPES[dtype]
     a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    return a, (Tq, heads, v_dim)
+    tiled = all(t is None or _tile_strides(*t) for t in (q, k, v, k_shared))
+    return a, (Tq, heads, v_dim), tiled
 
 
 @functools.lru_cache(maxsize=512)
@@ -477,16 +480,21 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if t is not None and t.dtype != q.dtype:
             raise ValueError(f"{name} is {t.dtype}, q is {q.dtype}")
     _no_gradient(q, k, v, k_shared, out)
-    q, k, v = _tiled(q), _tiled(k), _tiled(v)
-    if k_shared is not None:
-        k_shared = _tiled(k_shared)
     _vector("cu_q", cu_q, torch.int32)
     _vector("cu_k", cu_k, torch.int32)
-    layout, shape = _attention_layout(
-        (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),
-        None if k_shared is None else (k_shared.shape, k_shared.stride()),
-        None if out is None else (out.shape, out.stride()), q.dtype, cu_q.numel(), cu_k.numel(),
-        scale)
+    for copied in (False, True):
+        layout, shape, tiled = _attention_layout(
+            (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),
+            None if k_shared is None else (k_shared.shape, k_shared.stride()),
+            None if out is None else (out.shape, out.stride()), q.dtype, len(cu_q), len(cu_k),
+            scale)
+        addresses = q.data_ptr() | k.data_ptr() | v.data_ptr()
+        if k_shared is not None:
+            addresses |= k_shared.data_ptr()
+        if copied or (tiled and not addresses % 16):
+            break
+        q, k, v = _tiled(q), _tiled(k), _tiled(v)
+        k_shared = None if k_shared is None else _tiled(k_shared)
     a = _lib.AttentionArgs.from_buffer_copy(layout)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=q.device)

@@ -305,3 +305,8 @@ def test_outputs_whose_rows_share_memory_are_refused():
         x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
         prompt.Rotary(64, device="cpu")(torch.arange(4), x,
                                         out_q=buf.as_strided((4, 2, 64), (64, 64, 1)))
+
+
+def test_attention_of_columns_that_no_copy_aligns_ends_in_a_refusal():
+    with pytest.raises(ValueError, match="CUDA"):
+        prompt.prompt_attention(**_qkv(dim=67, v_dim=67))
