@@ -295,14 +295,14 @@ __global__ void plan_range_kernel(int64_t* range, const int32_t* status) {
 // the rest (at most half a turn) goes to 32 bits, so a position of a million
 // keeps as many bits of its phase as position one. Pairs are adjacent columns
 // (interleaved) or columns rot / 2 apart (half).
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 constexpr int kRotMaxPairs = 256;
 
 struct RotTensor {
   const void* x;
   void* y;
   int64_t xs, xh, ys, yh;  // strides of a token and a head, in elements
-  int heads, offset;
+  int heads, offset, copied;  // copied: columns that are not rotated, where they are written
   int units;               // units of a head: its rotated ones, then the copied
   uint32_t units_mul;      // index / units == (index * units_mul) >> 32
 };
@@ -341,16 +341,21 @@ struct alignas(sizeof(E) * V) RotVec {
 // (products and sums are written out, so that every form of the kernel rounds
 // alike.) A unit is two vectors of V columns, rot / 2 columns apart, V pairs:
 // element k of both (half), or the neighbours within each (interleaved; with V =
-// 1 a unit is two neighbours). A vector is one load: 16 bytes where the sizes,
-// strides and addresses allow it.
+// 1 a unit is two neighbours). A vector is 32 bytes where the sizes, strides and
+// addresses allow it.
 //
-// Bound by the rows' bytes: many CTAs of few rows in flight each (6 per SM with
-// one unit a thread; 4 with two took 65 us where this takes 54, for 16384 rows of
-// 36 heads of 128 columns of bf16: 5.6 TB/s). The first rows are asked for before
-// the angles are formed. Vectors of 8, 4, 2 and 1 elements there: 54, 83, 112 and
-// 160 us, so the widest that fits is taken.
+// Bound by the rows' bytes: enough of them have to be in flight (32-byte vectors,
+// 8 CTAs of one unit a thread per SM: 49 us for 16384 rows of 36 heads of 128
+// columns of bf16, 6.15 TB/s; 6 CTAs 51, 9 CTAs 51; 16-byte vectors 53, rows that
+// allow 8, 4 and 2 bytes 76, 104 and 155, so the widest that fits is taken; in
+// fp32 91, 6.6 TB/s). A CTA takes a few tokens, so that there are many of them (3
+// tokens; 8 take 52). Columns that are not rotated go two vectors a unit too (one
+// a unit: 4099 rows with 32 of 128 columns rotated 13.5 us, two 11.2). The first
+// rows are asked for before the angles are formed.
 template <typename E, int V, bool kInterleaved>
-__global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, V * sizeof(E) == 32   ? 8
+                                               : V * sizeof(E) == 16 ? 10
+                                                                     : 12) rotary_kernel(RotArgs a) {
   // (cos, sin) * factor of each token, [pair within a unit][unit]: lanes of
   // neighbouring units read neighbouring words
   extern __shared__ float2 cs[];
@@ -369,6 +374,7 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
   Vec lo[U], hi[U];
   E* dst[U];
   int pair[U];   // first pair's place in cs, -1: not rotated
+  int to[U];     // from the first vector to the second, 0: there is none
   int token[U];  // -1: no item
   auto load = [&](int i0) {
 #pragma unroll
@@ -388,18 +394,20 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
       if (unit < a.rot_units) {
         col = x.offset + unit * (kInterleaved && V == 1 ? 2 : V);
         pair[u] = t * half + unit;
+        to[u] = to_hi;
       } else {
-        // columns that are not rotated: those before the rotated ones, then
-        // those behind them
-        const int c = (unit - a.rot_units) * V;
+        // columns that are not rotated, two vectors a unit: those before the
+        // rotated ones, then those behind them
+        const int c = (unit - a.rot_units) * (2 * V);
         col = c < x.offset ? c : c + a.rot;
         pair[u] = -1;
+        to[u] = c + V >= x.copied ? 0 : c + V == x.offset ? V + a.rot : V;
       }
       token[u] = t;
       const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
       dst[u] = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
       lo[u] = *reinterpret_cast<const Vec*>(src);
-      if (pair[u] >= 0) hi[u] = *reinterpret_cast<const Vec*>(src + to_hi);
+      if (to[u] != 0) hi[u] = *reinterpret_cast<const Vec*>(src + to[u]);
     }
   };
   // the first rows are on their way while the angles are formed
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
         }
       }
       *reinterpret_cast<Vec*>(dst[u]) = lo[u];
-      if (pair[u] >= 0) *reinterpret_cast<Vec*>(dst[u] + to_hi) = hi[u];
+      if (to[u] != 0) *reinterpret_cast<Vec*>(dst[u] + to[u]) = hi[u];
     }
     i0 += U * kRotThreads;
     if (i0 >= nt * n) break;
@@ -448,10 +456,11 @@ __global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(RotArgs a) {
 template <typename E, bool kInterleaved>
 cudaError_t launch_rotary(const RotArgs& a, int v, dim3 grid, size_t smem, cudaStream_t st) {
   switch (v) {
-    case 8:
+    case 16:
       if constexpr (sizeof(E) == 2)
-        return sl::launch(rotary_kernel<E, 8, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
+        return sl::launch(rotary_kernel<E, 16, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
       return cudaErrorInvalidValue;
+    case 8: return sl::launch(rotary_kernel<E, 8, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
     case 4: return sl::launch(rotary_kernel<E, 4, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
     case 2: return sl::launch(rotary_kernel<E, 2, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
     default: return sl::launch(rotary_kernel<E, 1, kInterleaved>, grid, dim3(kRotThreads), smem, st, a);
@@ -547,7 +556,7 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
     }
     return true;
   };
-  int v = 16 / size;
+  int v = 32 / size;
   while (v > 1 && !fits(v)) v >>= 1;
   RotArgs a = {};
   a.positions = positions;
@@ -573,7 +582,8 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
     t.heads = p->heads;
     t.offset = p->offset;
     // in place the columns that are not rotated are left alone
-    t.units = a.rot_units + (in_place ? 0 : (p->dim - rot) / v);
+    t.copied = in_place ? 0 : p->dim - rot;
+    t.units = a.rot_units + (t.copied / v + 1) / 2;
     t.units_mul = t.units == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + t.units - 1) / t.units);
     items += t.heads * t.units;
   }

@@ -223,6 +223,17 @@ def test_rotary_matches_64_bits(dtype, interleaved, T, heads, kv_heads, dim, rot
     assert buf[..., dim:].eq(7.0).all() and buf[:, -1].eq(7.0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,heads,kv_heads,dim,rot,offset", [
+    (7, 3, 2, 112, 32, 16), (5, 2, 1, 72, 16, 8), (9, 1, 1, 48, 32, 0), (9, 1, 1, 80, 32, 32),
+    (300, 4, 1, 160, 32, 112), (3, 2, 2, 9, 2, 3)])
+def test_rotary_copies_an_odd_number_of_vectors(dtype, T, heads, kv_heads, dim, rot, offset):
+    """Columns that are not rotated go in twos of the widest vectors: odd
+    numbers of them, and twos that lie on both sides of the rotated ones."""
+    for interleaved in (True, False):
+        test_rotary_matches_64_bits(dtype, interleaved, T, heads, kv_heads, dim, rot, offset)
+
+
 def test_rotary_far_positions_keep_their_phase():
     pos = torch.tensor([0, 1, 2 ** 24 + 1, 2 ** 31 + 12345, 10 ** 12], device="cuda")
     x = torch.zeros(5, 1, 64, device="cuda")
