@@ -31,9 +31,9 @@
 // Then the hand-overs count: named barriers instead of mbarriers between warps,
 // waits without a suspend hint or a vote (82 -> 74 us), the maximum taken outside
 // the turn (16384 tokens on 32 / 4 heads of 128: 1.93 -> 1.77 ms). Now, device time:
-//   4096 tokens, 16 heads of 192 / 128        73 us, 1170 TFLOP/s, 0.71 of cuBLAS's burst
-//   16384 tokens, 32 / 4 heads of 128       1.77 ms, 1240 TFLOP/s, 0.91 of cuBLAS's
-//                                             sustained rate (the power cap; 1.60 ms before)
+//   4096 tokens, 16 heads of 192 / 128        72 us, 1194 TFLOP/s, 0.73 of cuBLAS's burst
+//   16384 tokens, 32 / 4 heads of 128       1.80 ms, 1220 TFLOP/s, 0.89 of cuBLAS's
+//                                             sustained rate (the power cap; 1.62 ms before)
 //   8 single tokens over 60 000 keys, 32 / 4  33 us, 19 of them the bytes; 8 until the first
 //                                             scores are there, 5 for the join
 // Measured and not kept: part of the exponentials as a cubic on the FMA pipes
@@ -850,7 +850,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         weights(0, 32);
         tmem_st32(s_at, r);
         hand_over(0);
-        // (the other half's first exponentials come in behind the last ones)
+        // (the other half's first exponentials come in behind the last ones: 4096
+        // tokens 72.1 us, the turn passed on after all of them 73.0)
         weights(32, 60);
         pass_turn();
         weights(60, 64);
