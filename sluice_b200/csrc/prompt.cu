@@ -25,6 +25,7 @@ namespace {
 // one warp for the table the last two took 35 and 40 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxRequests = 8192;
+constexpr int kPlanFew = 2;      // blocks that a lane writes by itself
 constexpr int kPlanChunk = 128;  // consecutive rows that a warp fills in a turn, four a lane
 
 struct PlanArgs {
@@ -246,13 +247,25 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   if (a.kv_slots != nullptr) fill(cu_total, a.Tk, true);
 
   // the table rows of the requests that take blocks: a lane looks at each of
-  // the warp's (nwarps apart), the warp writes a row
+  // the warp's (nwarps apart) and writes a few blocks by itself, the warp writes
+  // more (1000 requests that take one block each: 9.3 us, row after row 16.7)
   for (int r0 = gwarp; r0 < a.B; r0 += 32 * nwarps) {
     const int r = r0 + nwarps * lane;
     Lengths l = {};
     if (r < a.B) l = plan_lengths(a, r);
     const int o = r < a.B ? off[r] : -1;
-    for (unsigned takers = __ballot_sync(0xffffffffu, o >= 0 && l.take > 0); takers;
+    const bool few = l.take <= kPlanFew;
+    if (few && o >= 0) {
+      int32_t* row = a.table + r * a.ld_table + l.held;
+      int id[kPlanFew];
+#pragma unroll
+      for (int i = 0; i < kPlanFew; ++i)
+        if (i < l.take) id[i] = *new_block(o + i);
+#pragma unroll
+      for (int i = 0; i < kPlanFew; ++i)
+        if (i < l.take) row[i] = id[i];
+    }
+    for (unsigned takers = __ballot_sync(0xffffffffu, o >= 0 && !few); takers;
          takers &= takers - 1) {
       const int w = __ffs(takers) - 1;
       const int first = __shfl_sync(0xffffffffu, o, w), n = __shfl_sync(0xffffffffu, l.take, w);

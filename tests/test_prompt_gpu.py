@@ -86,6 +86,17 @@ def test_plan_of_many_requests(B, in_place):
     p.check()
 
 
+@pytest.mark.parametrize("bs", [1, 4, 16])
+def test_plan_of_requests_that_take_few_and_many_blocks(bs):
+    """Runs of none to many blocks side by side, in one CTA and in several."""
+    g = torch.Generator().manual_seed(bs)
+    for B, most in ((40, 9), (300, 9), (600, 40)):
+        new = torch.randint(0, most, (B,), generator=g).tolist()
+        context = torch.randint(0, 30, (B,), generator=g).tolist()
+        _check_plan(context, new, bs, seed=B)
+        _check_plan(context, new, bs, seed=B, in_place=False)
+
+
 def test_plan_of_long_requests_and_rows_behind_the_last():
     _check_plan([0, 100000], [70000, 1], 64, T=70500)[0].check()
 
