@@ -601,17 +601,17 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
     items += t.heads * t.units;
   }
   // tokens per CTA: about four units per thread, so that the angles' sines
-  // and cosines and the launch are spread over several rows
+  // and cosines and the launch are spread over several rows; their table takes
+  // 16 KB at most, for 8 CTAs per SM
   int per = 4 * kRotThreads / items;
   per = per < 1 ? 1 : (per > 32 ? 32 : per);
   const int sms = sl_device_sm_count();
   if (sms <= 0) return SL_ERR_CUDA;
-  while (per > 1 && (T + per - 1) / per < 4 * sms) per >>= 1;
+  while (per > 1 && ((T + per - 1) / per < 4 * sms || per * rot * 4 > 16 * 1024)) per >>= 1;
   a.per_cta = per;
   a.inv_items = 1.f / static_cast<float>(items);
   const dim3 grid((T + per - 1) / per);
   const size_t smem = static_cast<size_t>(per) * (rot / 2) * sizeof(float2);
-  if (smem > 48 * 1024) return SL_ERR_UNSUPPORTED;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == SL_DTYPE_BF16)

@@ -289,7 +289,8 @@ class Rotary:
         each head rotated and the others copied. Returns (q', k') (q' alone
         without ``k``), new tensors or ``out_q`` / ``out_k``; passing ``q``
         itself as ``out_q`` rotates in place. Rows at negative positions
-        (padding) keep their values."""
+        (padding) keep their values. Up to 512 rotated columns of up to 4096,
+        and fewer than 2^20 columns in all heads of a token."""
         dtype = _DTYPES.get(q.dtype)
         if dtype is None or (k is not None and k.dtype != q.dtype):
             raise ValueError("q and k must share one of bfloat16, float16, float32")

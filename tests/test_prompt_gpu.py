@@ -245,6 +245,17 @@ def test_rotary_copies_an_odd_number_of_vectors(dtype, T, heads, kv_heads, dim, 
         test_rotary_matches_64_bits(dtype, interleaved, T, heads, kv_heads, dim, rot, offset)
 
 
+@pytest.mark.parametrize("rot", [512, 256])
+def test_rotary_of_many_rows_of_wide_heads(rot):
+    T = 40001
+    x = torch.randn(T, 1, rot, device="cuda", generator=_gen(rot)).bfloat16()
+    pos = torch.arange(T, device="cuda")
+    freqs, factor = prompt.rotary_frequencies(rot)
+    for interleaved in (True, False):
+        y = prompt.Rotary(rot, interleaved=interleaved)(pos, x)
+        _rotary_close(y, oprompt.rotary(x, pos, freqs, factor, 0, interleaved), x, x.dtype, factor)
+
+
 def test_rotary_far_positions_keep_their_phase():
     pos = torch.tensor([0, 1, 2 ** 24 + 1, 2 ** 31 + 12345, 10 ** 12], device="cuda")
     x = torch.zeros(5, 1, 64, device="cuda")
