@@ -631,6 +631,21 @@ def test_attention_of_many_sequences(B, most):
     _check_attention(q_lens, k_lens, 2, 1, 128, 128, seed=B)
 
 
+def test_attention_of_more_sequences_than_a_table_entry_has_lanes():
+    g = torch.Generator().manual_seed(4)
+    q_lens = torch.randint(0, 2, (9000,), generator=g).tolist()
+    k_lens = [n * (1 + i % 5) for i, n in enumerate(q_lens)]
+    _check_attention(q_lens, k_lens, 2, 2, 64, 64, seed=1)
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [
+    ([150], [6000]), ([3, 150], [40, 6000]), ([1] * 40, [3000 + 7 * i for i in range(40)])])
+def test_attention_of_many_items_in_shares(q_lens, k_lens):
+    """More items than a warp has lanes in one sequence, and more sequences than
+    lanes, their key tiles shared out."""
+    _check_attention(q_lens, k_lens, 128, 1, 128, 128, seed=2)
+
+
 # ------------------------------------------------------------- all together
 def test_steps_of_all_three_in_one_graph():
     """Plan, rotary positions, cache and attention captured as one step of a
