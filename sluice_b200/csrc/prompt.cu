@@ -192,11 +192,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   // where the cache block of a row is found (nullptr: the row has none)
   auto block_at = [&](int r, int context, int pos) -> const int32_t* {
     const int blk = block_index(a, pos), o = off[r];
-    const int held = ring ? blocks_of(a, context) : a.width;
     // a refused request's new rows have no slot, even inside its last block
     if (o < 0 && pos >= context) return nullptr;
-    if (blk < held) return blk < a.width ? a.table + r * a.ld_table + blk : nullptr;
-    return new_block(o + (blk - held));
+    // without a ring every block is in the table, or nowhere: a context may
+    // reach past its table row
+    if (!ring || blk < blocks_of(a, context))
+      return blk < a.width ? a.table + r * a.ld_table + blk : nullptr;
+    return new_block(o + (blk - blocks_of(a, context)));
   };
   // rows of a packed batch, consecutive ones per warp and turn (four a lane, or
   // fewer where that would leave warps without any): a lane's are looked up
