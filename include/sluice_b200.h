@@ -527,8 +527,8 @@ enum {
  * blocks the ring or its table row cannot hold takes none: its new tokens
  * get slot -1, its table row stays as it was, and status becomes
  * SL_KV_PLAN_NO_BLOCKS. Negative lengths count as 0, and more tokens than T
- * or Tk are cut off (cu_new and cu_total stay within T and Tk):
- * SL_KV_PLAN_BAD_INPUT.
+ * or Tk (or than 2^31 - 1) are cut off (cu_new and cu_total stay within T and
+ * Tk): SL_KV_PLAN_BAD_INPUT.
  * B in [1, 8192]. */
 int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new_lens, int B,
                       int block_size, int32_t* block_table, int64_t ld_table, int table_width,

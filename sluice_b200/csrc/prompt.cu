@@ -52,10 +52,10 @@ struct Lengths {
   bool invalid, refused;
 };
 
-// x / block size of x >= 0, and the blocks that x rows take
-__device__ __forceinline__ int block_index(const PlanArgs& a, int x) {
-  return a.shift >= 0 ? x >> a.shift
-                      : static_cast<int>(static_cast<unsigned>(x) / static_cast<unsigned>(a.bs));
+// x / block size, and the blocks that x >= 0 rows take. (Positions are unsigned:
+// a refused request's may pass 31 bits.)
+__device__ __forceinline__ int block_index(const PlanArgs& a, unsigned x) {
+  return static_cast<int>(a.shift >= 0 ? x >> a.shift : x / static_cast<unsigned>(a.bs));
 }
 __device__ __forceinline__ int blocks_of(const PlanArgs& a, int x) {
   const unsigned up = static_cast<unsigned>(x) + static_cast<unsigned>(a.bs) - 1u;
@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
   int* cu_new = plan_sm;                 // [B + 1]
   int* cu_total = cu_new + a.B + 1;      // [B + 1]
   int* off = cu_total + a.B + 1;         // [B] blocks taken before, -1: refused
+  int* cached = off + a.B;               // [B] context (the sums above may be cut off)
   const int tid = threadIdx.x, lane = tid & 31;
   if (tid == 0) {
     s_invalid = s_short = s_end = 0;
@@ -170,6 +171,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
       cu_new[r + 1] = saturated(carry[0] + v[0]);
       cu_total[r + 1] = saturated(carry[1] + v[1]);
       off[r] = l.refused || short_of ? -1 : saturated(end - l.take);
+      cached[r] = l.context;
       if (l.take > 0 && !short_of) atomicMax(&s_end, saturated(end));
       if (l.invalid) s_invalid = 1;
       if (l.refused || short_of) s_short = 1;
@@ -190,10 +192,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
     return a.free_blocks + at;
   };
   // where the cache block of a row is found (nullptr: the row has none)
-  auto block_at = [&](int r, int context, int pos) -> const int32_t* {
+  auto block_at = [&](int r, int context, unsigned pos) -> const int32_t* {
     const int blk = block_index(a, pos), o = off[r];
     // a refused request's new rows have no slot, even inside its last block
-    if (o < 0 && pos >= context) return nullptr;
+    if (o < 0 && pos >= static_cast<unsigned>(context)) return nullptr;
     // without a ring every block is in the table, or nowhere: a context may
     // reach past its table row
     if (!ring || blk < blocks_of(a, context))
@@ -217,15 +219,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
         const int64_t last = min(c0 + chunk, min(rows, static_cast<int64_t>(used))) - 1;
         hi = find_request(cu, static_cast<int>(last), lo, a.B - 1);
       }
-      int pos[kEach], block[kEach];
+      unsigned pos[kEach];
+      int block[kEach];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         const int64_t t = c0 + lane + 32 * i;
-        pos[i] = block[i] = -1;
+        pos[i] = ~0u;
+        block[i] = -1;
         if (i < each && t < rows && t < used) {
           const int r = find_request(cu, static_cast<int>(t), lo, hi);
-          const int context = (cu_total[r + 1] - cu_total[r]) - (cu_new[r + 1] - cu_new[r]);
-          pos[i] = static_cast<int>(t) - cu[r] + (all_rows ? 0 : context);
+          const int context = cached[r];
+          pos[i] = static_cast<unsigned>(static_cast<int>(t) - cu[r]) +
+              (all_rows ? 0u : static_cast<unsigned>(context));
           const int32_t* at = block_at(r, context, pos[i]);
           if (at != nullptr) block[i] = *at;
         }
@@ -235,11 +240,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kv_blocks_kernel(PlanArgs a
         const int64_t t = c0 + lane + 32 * i;
         if (i >= each || t >= rows) continue;
         const int64_t slot = block[i] < 0 ? -1
-            : static_cast<int64_t>(block[i]) * a.bs + (pos[i] - block_index(a, pos[i]) * a.bs);
+            : static_cast<int64_t>(block[i]) * a.bs +
+                (pos[i] - static_cast<unsigned>(block_index(a, pos[i])) * static_cast<unsigned>(a.bs));
         if (all_rows) {
           a.kv_slots[t] = slot;
         } else {
-          a.positions[t] = pos[i];
+          a.positions[t] = pos[i] == ~0u ? -1 : static_cast<int64_t>(pos[i]);
           a.slots[t] = slot;
         }
       }
@@ -523,11 +529,11 @@ extern "C" int sl_plan_kv_blocks(const int32_t* context_lens, const int32_t* new
   grid = grid < 1 ? 1 : (grid > most ? most : grid);
   const bool in_place = ring && free_range_out == free_range;
   a.write_range = !(in_place && grid > 1);
-  const size_t smem = sizeof(int) * (3 * static_cast<size_t>(B) + 2);
+  const size_t smem = sizeof(int) * (4 * static_cast<size_t>(B) + 2);
   static std::atomic<uint64_t> smem_set{0};
   if (smem > 40 * 1024)
     SL_CUDA_TRY(sl::ensure_smem_limit(plan_kv_blocks_kernel,
-                                      sizeof(int) * (3 * kPlanMaxRequests + 2), smem_set));
+                                      sizeof(int) * (4 * kPlanMaxRequests + 2), smem_set));
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   SL_CUDA_TRY(sl::launch(plan_kv_blocks_kernel, dim3(static_cast<unsigned>(grid)),
                          dim3(threads), smem, st, a));

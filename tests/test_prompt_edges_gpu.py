@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from oracle import prompt as oprompt
 from sluice_b200 import _lib, prompt
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,90 @@ def test_plan_of_a_context_past_its_row_among_many():
         want_kv += rows
         want.append(rows[-1])
     assert p.slots.tolist() == want and p.kv_slots.tolist() == want_kv
+
+
+@pytest.mark.parametrize("bs", [16, 96, 1])
+@pytest.mark.parametrize("ring", [True, False])
+@pytest.mark.parametrize("huge", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 5), (2 ** 31 - 40, 7)])
+def test_plan_of_requests_behind_a_huge_one(bs, ring, huge):
+    """A request whose lengths pass its table row, and with it the sums pass
+    2^31 - 1, is reported; the ones behind it get their own positions and
+    blocks."""
+    context, new = [huge[0], 10, 3, 0], [huge[1], 5, 30, 2]
+    width, rest = 40, 3
+    held = [-(-c // bs) for c in context]
+    need = [-(-(c + n) // bs) for c, n in zip(context, new)]
+    ids = torch.randperm(400, generator=torch.Generator().manual_seed(bs)).tolist()
+    rows, at = [ids[:width]], width
+    for r in (1, 2, 3):
+        n = held[r] if ring else need[r]
+        rows.append(ids[at:at + n] + [-1] * (width - n))
+        at += n
+    table = torch.tensor(rows, **I32)
+    free, rng = (torch.tensor(ids[300:364], **I32), torch.tensor([60, 124], device="cuda")) \
+        if ring else (None, None)
+    T, Tk = sum(new) + rest, 100
+    p = prompt.plan_kv_blocks(torch.tensor(context, **I32), torch.tensor(new, **I32), table, free,
+                              rng, bs, T, num_kv_tokens=Tk)
+    taken = 0
+    for r in (1, 2, 3):
+        for i in range(held[r], need[r] if ring else held[r]):
+            rows[r][i] = ids[300 + (60 + taken) % 64]
+            taken += 1
+    assert p.status.tolist() == [_lib.KV_PLAN_BAD_INPUT, taken]
+    assert table.tolist() == rows
+    positions = [c + i for c, n in zip(context, new) for i in range(n)]
+    slots = [-1] * new[0] + [rows[r][q // bs] * bs + q % bs for r in (1, 2, 3)
+                             for q in range(context[r], context[r] + new[r])]
+    assert p.positions.tolist() == positions + [-1] * rest
+    assert p.slots.tolist() == slots + [-1] * rest
+    assert p.cu_new.tolist() == [0, new[0], new[0] + 5, new[0] + 35, new[0] + 37]
+    assert p.cu_total.tolist() == [0] + 4 * [Tk]
+    assert p.kv_slots.tolist() == [rows[0][q // bs] * bs + q % bs if q < width * bs else -1
+                                   for q in range(Tk)]
+
+
+def test_plan_of_sums_that_end_inside_a_request():
+    """The sum of all rows passes 2^31 - 1 within a request that fits its row,
+    behind one that found no blocks."""
+    bs, width = 1 << 20, 2048
+    context, new = [2 ** 31 - 6000, 0, 1023], [0, 5 * bs, 1]
+    table = torch.full((3, width), -1, **I32)
+    table[0] = torch.arange(width)
+    table[2, 0] = 77
+    T = 16
+    p = prompt.plan_kv_blocks(torch.tensor(context, **I32), torch.tensor(new, **I32), table,
+                              torch.tensor([9], **I32), torch.tensor([0, 1], device="cuda"), bs, T)
+    assert p.status.tolist() == [_lib.KV_PLAN_BAD_INPUT, 0]
+    assert p.slots.eq(-1).all() and p.positions.tolist() == list(range(T))
+    T = sum(new) + 1
+    p = prompt.plan_kv_blocks(torch.tensor(context, **I32), torch.tensor(new, **I32), table,
+                              torch.tensor([9], **I32), torch.tensor([0, 1], device="cuda"), bs, T)
+    assert p.slots[:5 * bs].eq(-1).all()
+    assert p.slots[5 * bs:].tolist() == [77 * bs + 1023, -1]
+    assert p.positions[5 * bs:].tolist() == [1023, -1]
+    assert torch.equal(p.positions[:5 * bs], torch.arange(5 * bs, device="cuda"))
+
+
+def test_plan_of_the_most_requests():
+    """8192 requests, the most that a plan takes, against the oracle."""
+    B, bs, width = 8192, 16, 3
+    g = torch.Generator().manual_seed(8)
+    context = torch.randint(0, 20, (B,), generator=g)
+    new = torch.randint(0, 20, (B,), generator=g)
+    held = (context + bs - 1) // bs
+    table = torch.where(torch.arange(width) < held[:, None],
+                        torch.arange(B * width).view(B, width), -1).int()
+    free = (torch.randperm(2 * B, generator=g) + B * width).int()
+    T, Tk = int(new.sum()), int((context + new).sum())
+    tab = table.cuda()
+    rng = torch.tensor([7, 7 + len(free)], device="cuda")
+    p = prompt.plan_kv_blocks(context.int().cuda(), new.int().cuda(), tab, free.cuda(), rng, bs, T,
+                              num_kv_tokens=Tk)
+    ref = oprompt.plan(context.tolist(), new.tolist(), table.tolist(), free.tolist(), 7,
+                       7 + len(free), bs, T, Tk)
+    assert p.cu_new.tolist() == ref[0] and p.cu_total.tolist() == ref[1]
+    assert p.positions.tolist() == ref[2] and p.slots.tolist() == ref[3]
+    assert p.kv_slots.tolist() == ref[4] and tab.tolist() == ref[5]
+    assert rng.tolist() == [ref[6], 7 + len(free)] and not ref[7]
+    p.check()
