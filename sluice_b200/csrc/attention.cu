@@ -54,7 +54,7 @@ constexpr int kThreads = 384;
 constexpr int kTile = 128;           // rows of a half and keys of a tile
 constexpr int kSlotBytes = 16384;
 constexpr int kCoarse = 256;         // entries of the work table
-constexpr int kBars = 16;            // barriers of tiles in flight
+constexpr int kBars = 16;            // barriers of tiles in flight; even ones keys, odd ones values
 // How far (in powers of 2) a row's maximum may lag behind its scores: bf16
 // weights have the exponents of the 32-bit sums, fp16 ones end at 2^16.
 constexpr float kLagBf16 = 32.f, kLagF16 = 12.f;
@@ -609,7 +609,8 @@ static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 // A role's place in the sequence of tiles (keys, values, keys, ...): the
 // tile's number, which names its barriers and their parity, and its first slot.
-// At most kSlots tiles are in flight, fewer than there are barriers.
+// At most kSlots tiles are in flight, fewer than there are barriers, and each is
+// let go by all that wait for it before its slots are filled again.
 struct Tiles {
   uint32_t n = 0;
   int slot = 0;
@@ -685,7 +686,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
   if (tid == 0) {
     for (int i = 0; i < kBars; ++i) {
       sl::mbar_init(&sy.full[i], 1);
-      sl::mbar_init(&sy.empty[i], 2);
+      // both halves' MMAs, and of a value tile the guard, which may be late: it
+      // tells the uses of a barrier apart by their parity, so none may pass it by
+      sl::mbar_init(&sy.empty[i], i % 2 ? 3 : 2);
       sl::mbar_init(&sy.clean[i], 1);
     }
     for (int h = 0; h < 2; ++h) {
@@ -1199,8 +1202,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       const int mark = n_item++;
       for (int j = g.j0; j < g.j1; ++j) {
         at.step<C::kSlots>(C::kChunks);
-        // every value tile is waited for, cleaned or not: a wait names a use
-        // of its barrier by the parity alone
+        // every value tile is waited for and let go, cleaned or not: a wait
+        // names a use of its barrier by the parity alone
         if (!out.wait(&sy.full[at.bar()], at.phase())) break;
         if ((j + 1) * kTile > g.lim0) {
           bool found = false;
@@ -1220,6 +1223,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
           __syncwarp();
           if (lane == 0) sl::mbar_arrive(&sy.clean[at.bar()]);
         }
+        if (lane == 0) sl::mbar_arrive(&sy.empty[at.bar()]);
         at.step<C::kSlots>(C::kVSlots);
       }
     }

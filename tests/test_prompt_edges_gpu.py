@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import prompt as oprompt
-from sluice_b200 import _lib, prompt
+from sluice_b200 import _lib, ops, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,59 @@ def test_plan_of_the_most_requests():
     assert p.kv_slots.tolist() == ref[4] and tab.tolist() == ref[5]
     assert rng.tolist() == [ref[6], 7 + len(free)] and not ref[7]
     p.check()
+
+
+# ---------------------------------------------------------------- attention
+def _attend(q_lens, k_lens, heads, kv_heads, dim, seed, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    q, k, v = (torch.randn(n, h, dim, device="cuda", generator=g).to(dtype)
+               for n, h in ((sum(q_lens), heads), (sum(k_lens), kv_heads), (sum(k_lens), kv_heads)))
+    cu_q, cu_k = (torch.tensor([0] + list(n), device="cuda").cumsum(0).int()
+                  for n in (q_lens, k_lens))
+    out = prompt.prompt_attention(q, k, v, cu_q, cu_k)
+    assert ops.workspace_status(prompt.prompt_attention.last_workspace) == 0
+    return out, q, k, v
+
+
+def _close(out, ref, mag, dtype=torch.bfloat16, more=0.0):
+    """Half a step on the output, half a step on each weight as it is fed to the
+    second product (hence on mag = sum p |v|), and 2^-11 of mag for the 32-bit
+    scores, exponentials and sums."""
+    u = torch.finfo(dtype).eps / 2
+    err = (out.double() - ref).abs()
+    tol = u * ref.abs() + (u + 2.0 ** -11) * mag + more
+    assert out.isfinite().all() and (err <= tol).all(), (err - tol).max().item()
+
+
+def _shared_out(q_lens, k_lens, heads, kv_heads, v_dim):
+    """Whether the key tiles are shared out (only then the workspace is more
+    than its header)."""
+    return _lib.lib().sl_prompt_attention_workspace_bytes(
+        len(q_lens), sum(q_lens), sum(k_lens), heads, kv_heads, v_dim) > 256
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [
+    ([700] + [1] * 256, [3700] + [1300] * 256),                  # a work table entry of several
+    ([1] * 200 + [900] + [1] * 99, [1600 + r % 7 for r in range(200)] + [4900] + [1600] * 99)])
+def test_attention_of_a_long_prompt_among_many_in_shares(q_lens, k_lens):
+    """Looking up a stretch takes long (hundreds of items of one sequence, added
+    up by one lane) while the tiles of the one before pass by."""
+    assert _shared_out(q_lens, k_lens, 128, 1, 128)
+    out, q, k, v = _attend(q_lens, k_lens, 128, 1, 128, seed=len(q_lens))
+    ref, mag = oprompt.attention(q, k, v, q_lens, k_lens, 128 ** -0.5)
+    _close(out, ref, mag)
+
+
+@pytest.mark.parametrize("heads,dim,q_len,k_len", [(128, 128, 4000, 12000), (128, 64, 4000, 12000),
+                                                   (64, 128, 16001, 56003)])
+def test_attention_of_thousands_of_items_in_shares(heads, dim, q_len, k_len):
+    """Thousands of items of one sequence and many key tiles that no row is
+    masked in; every 97th query is compared."""
+    assert _shared_out([q_len], [k_len], heads, 1, dim)
+    out, q, k, v = _attend([q_len], [k_len], heads, 1, dim, seed=q_len)
+    kk, vv = k[:, 0].double(), v[:, 0].double()
+    for i in list(range(0, q_len, 97)) + [q_len - 1]:
+        n = i + 1 + k_len - q_len
+        p = torch.softmax(q[i].double() @ kk[:n].T * dim ** -0.5, dim=-1)
+        _close(out[i], p @ vv[:n], p @ vv[:n].abs())
