@@ -573,7 +573,10 @@ int sl_rotary(const int64_t* positions, const double* turns, int T, int rot, int
  * 16-byte aligned. bf16 or fp16; (dim, v_dim) one of (64, 64), (128, 128),
  * (192, 128); shared_dim 0 or, at dim 192, 64; at most 128 heads per key
  * head. The workspace (sl_prompt_attention_workspace_bytes, 32-byte aligned)
- * starts with a status word: SL_OK, or SL_ERR_TIMEOUT when a bounded wait ran out. */
+ * starts with a status word: SL_OK, or SL_ERR_TIMEOUT when a bounded wait ran
+ * out and the output is not to be used. sl_prompt_attention_ex raises *failed
+ * (a device i32 of the caller's, or NULL) to that status too, and never lowers
+ * it, so that many calls, or replays of a graph, can share one. */
 typedef struct {
   const void *q, *k, *v, *k_shared;
   void* out;
@@ -587,6 +590,8 @@ size_t sl_prompt_attention_workspace_bytes(int B, int64_t Tq, int64_t Tk, int he
                                            int v_dim);
 int sl_prompt_attention(const sl_attention_args* args, void* workspace, size_t workspace_bytes,
                         sl_stream_t stream);
+int sl_prompt_attention_ex(const sl_attention_args* args, void* workspace, size_t workspace_bytes,
+                           int32_t* failed, sl_stream_t stream);
 
 #ifdef __cplusplus
 }

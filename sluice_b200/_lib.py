@@ -134,6 +134,7 @@ _SIGNATURES = {
                        _c.POINTER(RotaryPart), _vp]),
     "sl_prompt_attention_workspace_bytes": (_sz, [_i, _i64, _i64, _i, _i, _i]),
     "sl_prompt_attention": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp]),
+    "sl_prompt_attention_ex": (_i, [_c.POINTER(AttentionArgs), _vp, _sz, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -104,7 +104,8 @@ struct Params {
   float* part;                       // [2 * grid][rows_cap][v_dim]
   float2* part_ml;                   // [2 * grid][rows_cap] (maximum, sum)
   Later* later;                      // [grid]
-  int32_t* status;
+  int32_t* status;                   // of this call
+  int32_t* failed;                   // of many calls: only ever raised (nullptr: not asked for)
 };
 
 // ------------------------------------------------------------------ helpers
@@ -238,6 +239,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
+}
+
+__device__ __forceinline__ void report(const Params& p, int status) {
+  atomicMax(p.status, status);
+  if (p.failed != nullptr) atomicMax(p.failed, status);
 }
 
 // A role's outlook: once a bounded wait has run out, it waits for nothing more
@@ -680,7 +686,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
 
   if (sl::smem_u32(buf) & 1023) {
     // (the swizzled tiles want it; there is no static shared memory before it)
-    if (tid == 0) *p.status = SL_ERR_UNSUPPORTED;
+    if (tid == 0) {
+      *p.status = SL_OK;
+      report(p, SL_ERR_UNSUPPORTED);
+    }
     return;
   }
   if (tid == 0) {
@@ -1228,7 +1237,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
       }
     }
   }
-  if (!out.ok && lane == 0) atomicMax(p.status, SL_ERR_TIMEOUT);
+  if (!out.ok && lane == 0) report(p, SL_ERR_TIMEOUT);
   sl::tc_fence_before();
   __syncthreads();
   sl::tc_fence_after();
@@ -1433,6 +1442,12 @@ extern "C" size_t sl_prompt_attention_workspace_bytes(int B, int64_t Tq, int64_t
 
 extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspace,
                                    size_t workspace_bytes, sl_stream_t stream) {
+  return sl_prompt_attention_ex(args, workspace, workspace_bytes, nullptr, stream);
+}
+
+extern "C" int sl_prompt_attention_ex(const sl_attention_args* args, void* workspace,
+                                      size_t workspace_bytes, int32_t* failed,
+                                      sl_stream_t stream) {
   if (!args) return SL_ERR_INVALID;
   const sl_attention_args& a = *args;
   if (a.B <= 0 || a.Tq < 0 || a.Tk < 0 || a.heads <= 0 || a.kv_heads <= 0 ||
@@ -1509,6 +1524,7 @@ extern "C" int sl_prompt_attention(const sl_attention_args* args, void* workspac
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.lag = (bf16 ? kLagBf16 : kLagF16) / p.scale_log2;
   p.status = static_cast<int32_t*>(workspace);
+  p.failed = failed;
   p.later = reinterpret_cast<Later*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
   p.part = reinterpret_cast<float*>(p.later + r.grid);
   p.part_ml = reinterpret_cast<float2*>(p.part + 2 * r.grid * r.rows_cap * a.v_dim);

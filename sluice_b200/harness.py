@@ -315,10 +315,12 @@ class DecoderHarness:
         self.pos.add_(1)
         return logits.argmax(dim=-1)
 
-    def _prompt_attention(self, li: int, x: torch.Tensor, plan, has_context: bool) -> torch.Tensor:
+    def _prompt_attention(self, li: int, x: torch.Tensor, plan, has_context: bool,
+                          status: torch.Tensor) -> torch.Tensor:
         """The attention of packed prompt rows x [T, H]: their latents and
         rotated keys go to the cache, keys and values are expanded from the
-        latents of the whole sequences (the cached beginnings included)."""
+        latents of the whole sequences (the cached beginnings included).
+        ``status`` is raised where a wait of the kernel ran out."""
         from .prompt import prompt_attention
         cfg, lw = self.cfg, self.layers[li]
         nh, R = cfg.num_heads, cfg.kv_lora_rank
@@ -338,7 +340,8 @@ class DecoderHarness:
             lw["w_ukv"] = torch.cat([lw["w_uk"], lw["w_uv"]], dim=1).flatten(0, 1)
         kv = F.linear(rows[:, :R], lw["w_ukv"]).view(-1, nh, cfg.qk_nope + cfg.v_head)
         o = prompt_attention(q, kv[..., :cfg.qk_nope], kv[..., cfg.qk_nope:], plan.cu_new,
-                             plan.cu_total, k_shared=rows[:, R:], scale=self.scale)
+                             plan.cu_total, k_shared=rows[:, R:], scale=self.scale,
+                             status=status)
         return F.linear(o.flatten(1), lw["wo"])
 
     def prefill(self, ids: torch.Tensor, lengths: list[int],
@@ -351,11 +354,12 @@ class DecoderHarness:
         tokens). ``context`` are the positions, where the caller knows them;
         otherwise they are read back. Raises ``KvPlanError``, with nothing
         changed, where the pool has too few blocks left or a position before
-        the new tokens has none. CUDA with the fused attention only; the
+        the new tokens has none, and ``SluiceError``, with no position moved
+        and no block taken, where a layer's attention gave up on a wait. CUDA with the fused attention only; the
         MoE layers take the pass as one step of T rows."""
         if not self.fused_attention:
             raise ValueError("prefill runs on a CUDA device with the fused attention")
-        from ._lib import KV_PLAN_BAD_INPUT
+        from ._lib import KV_PLAN_BAD_INPUT, check
         from .prompt import KvPlanError
         cfg, dev = self.cfg, self.device
         if len(lengths) != self.batch or any(n < 0 for n in lengths):
@@ -394,11 +398,12 @@ class DecoderHarness:
         except RuntimeError:
             self.restore_blocks(blocks0)
             raise
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
         h = self.embed[ids]
         x = self._add_norm(h, None, self.layers[0]["in_norm"])
         for li in range(cfg.num_layers):
             lw = self.layers[li]
-            x = self._add_norm(h, self._prompt_attention(li, x, plan, has_context),
+            x = self._add_norm(h, self._prompt_attention(li, x, plan, has_context, status),
                                lw["post_norm"])
             f = self._dense_ffn(li, x) if li < cfg.first_dense else \
                 self.moe(li - cfg.first_dense, x)
@@ -407,6 +412,11 @@ class DecoderHarness:
         live = [b for b, n in enumerate(lengths) if n]
         ends = plan.cu_new[1:].long()[live] - 1
         nxt[live] = F.linear(x[ends], self.head).argmax(dim=-1)
+        try:
+            check(int(status), "prompt_attention")
+        except RuntimeError:
+            self.restore_blocks(blocks0)
+            raise
         self.pos.add_(new)
         return nxt
 

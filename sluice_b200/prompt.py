@@ -459,10 +459,39 @@ def _workspace_bytes(B: int, Tq: int, Tk: int, heads: int, kv_heads: int, v_dim:
                                                                   v_dim))
 
 
+# a status word per device, which its calls raise and ``check_attention`` reads
+# and clears; kept for good, as captured calls hold its address
+_failed: dict[int, torch.Tensor] = {}
+
+
+def _failed_word(dev: int) -> torch.Tensor | None:
+    word = _failed.get(dev)
+    if word is None:
+        with torch.cuda.device(dev):
+            # (what a capture allocates belongs to its graph: the word of a
+            # process whose first call is captured comes with a later call)
+            if not torch.cuda.is_current_stream_capturing():
+                word = _failed[dev] = torch.zeros(1, dtype=torch.int32, device="cuda")
+    return word
+
+
+def check_attention(device="cuda") -> None:
+    """Raise if a bounded wait ran out in a ``prompt_attention`` call without
+    a ``status`` of its own, on this device since the last check, so that its
+    output is not to be used (synchronises)."""
+    device = torch.device(device)
+    word = _failed.get(torch.cuda.current_device() if device.index is None else device.index)
+    if word is None:
+        return
+    status = int(word.item())
+    word.zero_()
+    check(status, "prompt_attention")
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: torch.Tensor, *, k_shared: torch.Tensor | None = None,
-                     scale: float | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     scale: float | None = None, out: torch.Tensor | None = None,
+                     status: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention over packed sequences: ``out`` [Tq, heads, v_dim].
 
     ``q`` [Tq, heads, dim], ``k`` [Tk, kv_heads, dim], ``v`` [Tk, kv_heads,
@@ -476,6 +505,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     last 64 are one row for all heads. ``scale`` (positive) defaults to dim^-0.5. A query
     that sees no key gets zeros; rows of ``q`` outside every sequence leave
     ``out`` as it was there (a new ``out`` is not initialised).
+
+    ``status`` (int32 [1]; default: a word of the device's, which
+    ``check_attention`` reads) is raised to the code of the error, and never
+    lowered, when a bounded wait of the device ran out.
     """
     for name, t in (("k", k), ("v", v), ("k_shared", k_shared), ("out", out)):
         if t is not None and t.dtype != q.dtype:
@@ -483,6 +516,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     _no_gradient(q, k, v, k_shared, out)
     _vector("cu_q", cu_q, torch.int32)
     _vector("cu_k", cu_k, torch.int32)
+    if status is not None:
+        _vector("status", status, torch.int32, 1)
     for copied in (False, True):
         layout, shape, tiled = _attention_layout(
             (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),
@@ -503,7 +538,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         raise ValueError("out needs a 16-byte aligned address")
     elif any(_ranges_meet(out, t) for t in (q, k, v, k_shared) if t is not None):
         raise ValueError("out overlaps an input")
-    dev = _device_index(q, k, v, cu_q, cu_k, k_shared, out)
+    dev = _device_index(q, k, v, cu_q, cu_k, k_shared, out, status)
     if a.B == 0 or a.Tq == 0:
         return out
     a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
@@ -512,8 +547,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         a.k_shared = k_shared.data_ptr()
     n = _workspace_bytes(a.B, a.Tq, a.Tk, a.heads, a.kv_heads, a.v_dim, dev)
     workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-    _call(dev, "sl_prompt_attention", ctypes.byref(a), workspace.data_ptr(), n)
-    prompt_attention.last_workspace = workspace
+    if status is None:
+        status = _failed_word(dev)
+    _call(dev, "sl_prompt_attention_ex", ctypes.byref(a), workspace.data_ptr(), n, ptr(status))
+    # (as other operators name the tensor that starts with their status)
+    prompt_attention.last_workspace = status
     return out
 
 

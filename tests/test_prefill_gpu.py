@@ -209,3 +209,30 @@ def test_offloaded_decoder_from_prompts_to_captured_steps():
         d.release()
     # the experts' slots differ in order only, so the tokens are the same
     assert runs[0][0] == runs[1][0] and runs[0][1] == runs[1][1]
+
+
+@pytest.mark.parametrize("kw", [{}, dict(cache_blocks=24, block_size=32)])
+def test_prefill_reports_a_wait_that_ran_out(kw, monkeypatch):
+    """One layer's attention gives up (its status says so): no position moves,
+    no block is taken, and the same prompts can be taken again."""
+    h, calls = _harness(**kw), []
+    real = prompt.prompt_attention
+
+    def gives_up(*args, status=None, **rest):
+        out = real(*args, status=status, **rest)
+        calls.append(status)
+        if len(calls) == 2:
+            status.fill_(5)   # SL_ERR_TIMEOUT
+        return out
+
+    tokens = _tokens([30, 1, 50])
+    monkeypatch.setattr(prompt, "prompt_attention", gives_up)
+    before = h.save_blocks()
+    with pytest.raises(RuntimeError, match="wait ran out"):
+        h.prefill(torch.cat(tokens).cuda(), [30, 1, 50])
+    assert len(calls) == 3 and h.pos.tolist() == [0, 0, 0]
+    assert all(torch.equal(v, before[n]) for n, v in h.save_blocks().items())
+    monkeypatch.undo()
+    again = h.prefill(torch.cat(tokens).cuda(), [30, 1, 50])
+    assert torch.equal(again, _harness(**kw).prefill(torch.cat(tokens).cuda(), [30, 1, 50]))
+    h.check_blocks()

@@ -192,3 +192,40 @@ def test_attention_of_thousands_of_items_in_shares(heads, dim, q_len, k_len):
         n = i + 1 + k_len - q_len
         p = torch.softmax(q[i].double() @ kk[:n].T * dim ** -0.5, dim=-1)
         _close(out[i], p @ vv[:n], p @ vv[:n].abs())
+
+
+def test_attention_raises_a_status_and_never_lowers_it():
+    """A call that ran through leaves the caller's word, and the device's, as
+    they were, whatever they hold; what the device's holds is raised once."""
+    def call(**kw):
+        return prompt.prompt_attention(q, q, q, cu, cu, **kw)
+
+    q = torch.randn(40, 2, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 40], **I32)
+    want = call()
+    prompt.check_attention()
+    word = torch.zeros(1, **I32)
+    assert torch.equal(call(status=word), want) and word.item() == 0
+    word.fill_(_lib.SL_ERR_TIMEOUT)
+    call(status=word)
+    assert word.item() == _lib.SL_ERR_TIMEOUT
+    prompt.check_attention()            # (the call had a word of its own)
+    call()
+    shared = prompt.prompt_attention.last_workspace
+    shared.fill_(_lib.SL_ERR_TIMEOUT)   # as a wait that ran out does
+    call()
+    with pytest.raises(_lib.SluiceError, match="wait ran out"):
+        prompt.check_attention(torch.device("cuda", 0))
+    prompt.check_attention("cuda")
+    with pytest.raises(ValueError, match="status"):
+        call(status=torch.zeros(2, **I32))
+    with pytest.raises(ValueError):
+        call(status=torch.zeros(1, dtype=torch.int32))
+
+
+def test_attention_keeps_no_workspace():
+    """Key tiles in shares take tens of MB while the call runs, none after."""
+    assert _shared_out([1, 1], [30000, 30000], 8, 2, 128)
+    out, *rest = _attend([1, 1], [30000, 30000], 8, 2, 128, seed=1)
+    del out, rest
+    assert prompt.prompt_attention.last_workspace.untyped_storage().nbytes() <= 512
