@@ -229,3 +229,31 @@ def test_attention_keeps_no_workspace():
     out, *rest = _attend([1, 1], [30000, 30000], 8, 2, 128, seed=1)
     del out, rest
     assert prompt.prompt_attention.last_workspace.untyped_storage().nbytes() <= 512
+
+
+@pytest.mark.parametrize("size", [3.3e38, 1e-20])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim", [
+    ([300, 1], [300, 700], 2, 1, 128), ([1, 2], [40001, 30], 8, 2, 128), ([130], [1500], 4, 4, 64)])
+def test_attention_of_the_largest_and_of_small_values(size, q_lens, k_lens, heads, kv_heads, dim):
+    """No weighted sum passes the largest value, for scores at random, all alike
+    and growing from key to key."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    tq, tk = sum(q_lens), sum(k_lens)
+    v = size * (1 - 0.9 * torch.rand(tk, kv_heads, dim, device="cuda", generator=g))
+    v = (v * torch.randint(0, 2, (tk, 1, 1), device="cuda", generator=g).sub(0.5).sign()).bfloat16()
+    cu_q, cu_k = (torch.tensor([0] + n, device="cuda").cumsum(0).int() for n in (q_lens, k_lens))
+    for step in (None, 0.0, 0.05, 0.7):
+        if step is None:
+            q, k = (torch.randn(n, h, dim, device="cuda", generator=g).bfloat16()
+                    for n, h in ((tq, heads), (tk, kv_heads)))
+        else:
+            # (steps of 1/16 in the last column: exact in bf16 up to 256 of them)
+            q = torch.zeros(tq, heads, dim, device="cuda", dtype=torch.bfloat16)
+            q[..., -1] = 16 * step * dim ** 0.5
+            k = torch.zeros(tk, kv_heads, dim, device="cuda", dtype=torch.bfloat16)
+            k[..., -1] = ((torch.arange(tk, device="cuda") % 256) / 16)[:, None].bfloat16()
+        out = prompt.prompt_attention(q, k, v, cu_q, cu_k)
+        ref, mag = oprompt.attention(q, k, v, q_lens, k_lens, dim ** -0.5)
+        # scores reach 256 * step, rounded at 2^-24 of that
+        _close(out, ref, mag, more=(256 * (step or 0.0) * 2.0 ** -22) * mag)
