@@ -257,3 +257,25 @@ def test_attention_of_the_largest_and_of_small_values(size, q_lens, k_lens, head
         ref, mag = oprompt.attention(q, k, v, q_lens, k_lens, dim ** -0.5)
         # scores reach 256 * step, rounded at 2^-24 of that
         _close(out, ref, mag, more=(256 * (step or 0.0) * 2.0 ** -22) * mag)
+
+
+@pytest.mark.parametrize("strong", [0, 30000, -1])
+@pytest.mark.parametrize("q_len,n,heads", [(1, 60001, 2), (130, 60001, 2), (1, 30101, 148)])
+def test_attention_of_a_flat_tail_behind_one_strong_key_in_fp16(strong, q_len, n, heads):
+    """Weights of 2^-26.3 of the strong key's, tens of thousands of them, make a
+    difference together; in shares (few heads) and in whole items."""
+    q = torch.zeros(q_len, heads, 64, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1.0
+    at = strong if strong >= 0 else n - q_len   # (every query sees it)
+    k = torch.zeros(n, heads, 64, device="cuda", dtype=torch.float16)
+    k[at, :, 0] = 18.25
+    v = torch.ones(n, heads, 64, device="cuda", dtype=torch.float16)
+    v[at, :, :32] = 0.0
+    cu_q, cu_k = torch.tensor([0, q_len], **I32), torch.tensor([0, n], **I32)
+    out = prompt.prompt_attention(q, k, v, cu_q, cu_k, scale=1.0)
+    ref, mag = oprompt.attention(q, k, v, [q_len], [n], 1.0)
+    assert ref[..., :32].min() > 3e-4
+    # a weight of 2^7 w in fp16 is off by half of 2^-24 at most where it has no
+    # bits below that, against a sum of at least 2^7; and the output by half of
+    # its own last bit
+    _close(out, ref, mag, torch.float16, more=2.0 ** -32 * n + 2.0 ** -25)
