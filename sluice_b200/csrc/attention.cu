@@ -99,8 +99,9 @@ struct Params {
   int64_t out_token, out_head;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  const void* vraw;                  // values, for the rare repair of a column
-  int64_t v_token, v_head;
+  // inputs as they are, for the rare repair of a column
+  const void *vraw, *qraw, *kraw, *ksraw;
+  int64_t v_token, v_head, q_token, q_head, k_token, k_head, ks_token;
   int B, Tq, Tk, heads, kv_heads, group, half_tokens;  // tokens of a half: 128 / group
   int shared;                        // the last 64 key columns come from ks
   int wide;                          // the output's rows are 32-byte aligned: stores of 32 bytes
@@ -684,6 +685,29 @@ __device__ __forceinline__ bool clean_rows(uint8_t* base, int lo, int hi, int ro
   return found;
 }
 
+// Whether the weight of a key is zero as the second product takes it, against a
+// row's maximum m. One thread.
+template <int kDim, bool kBf16>
+__device__ __noinline__ bool no_weight(const Params& p, float m, int row, int head, int key_row,
+                                       int key_head) {
+  auto f = [](uint16_t b) {
+    return kBf16 ? __uint_as_float(static_cast<uint32_t>(b) << 16)
+                 : __half2float(__ushort_as_half(b));
+  };
+  const uint16_t* q = static_cast<const uint16_t*>(p.qraw) + row * p.q_token + head * p.q_head;
+  const uint16_t* k = static_cast<const uint16_t*>(p.kraw) + key_row * p.k_token +
+      key_head * p.k_head;
+  const int own = p.shared ? kDim - 64 : kDim;
+  float s = 0.f;
+  for (int c = 0; c < own; ++c) s = fmaf(f(q[c]), f(k[c]), s);
+  const uint16_t* ks = static_cast<const uint16_t*>(p.ksraw) + key_row * p.ks_token;
+  for (int c = own; c < kDim; ++c) s = fmaf(f(q[c]), f(ks[c - own]), s);
+  const float top = kBf16 ? kTopBf16 : kTopF16;
+  const float w = m == -INFINITY ? 0.f
+                                 : ex2(fmaf(s, p.scale_log2, __fadd_rn(__fmul_rn(-m, p.scale_log2), top)));
+  return pack2<kBf16>(w, w) == 0;
+}
+
 template <int kDim, int kVDim, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
     const __grid_constant__ Params p) {
@@ -950,20 +974,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(
         }
         if (repair && live) {
           // values that are not finite were taken out of the tiles that not
-          // all rows see; a row that does see one gets it back: its weight
-          // is positive, so only its sign and kind count
+          // all rows see; a row that does see one gets it back: of its weight
+          // it only counts whether it is zero
           const int ja = max(g.lim0, g.j0 * kTile), jb = min(lim, g.j1 * kTile);
           for (int j = ja; j < jb; ++j) {
             const uint16_t* v = static_cast<const uint16_t*>(p.vraw) +
                 static_cast<int64_t>(g.k0 + j) * p.v_token + static_cast<int64_t>(g.head) * p.v_head +
                 c;
             constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u, kFrac = kBf16 ? 0x7fu : 0x3ffu;
+            uint32_t bad_ones = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) bad_ones |= static_cast<uint32_t>((v[i] & kExp) == kExp) << i;
+            if (bad_ones == 0) continue;
+            const bool none = no_weight<kDim, kBf16>(p, m, out_row, out_head, g.k0 + j, g.head);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const uint32_t b = v[i];
-              if ((b & kExp) == kExp) {
-                const float bad = b & kFrac ? __int_as_float(0x7fffffff)
-                                            : (b & 0x8000u) ? -INFINITY : INFINITY;
+              if (bad_ones >> i & 1u) {
+                const uint32_t b = v[i];
+                const float bad = none || (b & kFrac) ? __int_as_float(0x7fffffff)
+                                  : (b & 0x8000u)     ? -INFINITY
+                                                      : INFINITY;
                 o[i] = __float_as_uint(__uint_as_float(o[i]) + bad);
               }
             }
@@ -1516,6 +1546,14 @@ extern "C" int sl_prompt_attention_ex(const sl_attention_args* args, void* works
   p.vraw = a.v;
   p.v_token = a.v_token;
   p.v_head = a.v_head;
+  p.qraw = a.q;
+  p.q_token = a.q_token;
+  p.q_head = a.q_head;
+  p.kraw = a.k;
+  p.k_token = a.k_token;
+  p.k_head = a.k_head;
+  p.ksraw = a.shared_dim ? a.k_shared : nullptr;
+  p.ks_token = a.k_shared_token;
   p.B = a.B;
   p.Tq = static_cast<int>(a.Tq);
   p.Tk = static_cast<int>(a.Tk);

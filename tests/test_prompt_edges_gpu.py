@@ -279,3 +279,47 @@ def test_attention_of_a_flat_tail_behind_one_strong_key_in_fp16(strong, q_len, n
     # bits below that, against a sum of at least 2^7; and the output by half of
     # its own last bit
     _close(out, ref, mag, torch.float16, more=2.0 ** -32 * n + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,dim,v_dim,shared", [(2, 2, 64, 64, 0), (4, 2, 128, 128, 0),
+                                                             (2, 2, 192, 128, 64)])
+@pytest.mark.parametrize("q_len,k_len", [(150, 150), (2, 3000), (40, 700)])
+def test_attention_of_an_infinite_value_at_a_weight_of_zero(dtype, heads, kv_heads, dim, v_dim,
+                                                            shared, q_len, k_len):
+    """0 times inf: a key that scores -inf, or too low for a weight, makes NaN
+    of its value's infinite columns, as the formula does, wherever it lies; a
+    key with a weight makes inf of them."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    q = (torch.rand(q_len, heads, dim, device="cuda", generator=g) + 0.1).to(dtype)
+    k = torch.randn(k_len, kv_heads, dim - shared, device="cuda", generator=g).to(dtype)
+    v = torch.randn(k_len, kv_heads, v_dim, device="cuda", generator=g).to(dtype)
+    ks = torch.randn(k_len, shared, device="cuda", generator=g).to(dtype) if shared else None
+    cu_q, cu_k = torch.tensor([0, q_len], **I32), torch.tensor([0, k_len], **I32)
+    clean = prompt.prompt_attention(q, k, v, cu_q, cu_k, k_shared=ks)
+    for at in (k_len - q_len, k_len - q_len // 2 - 1, k_len - 1):
+        first = max(0, at - (k_len - q_len))   # the first query that sees it
+        for low in (float("-inf"), -30000.0, None):
+            k2, v2, s2 = k.clone(), v.clone(), None if ks is None else ks.clone()
+            if low is not None:
+                (k2[at, :, 3] if s2 is None else s2[at, 3:4])[:] = low
+            v2[at, :, 5] = float("inf")
+            v2[at, :, 40] = float("-inf")
+            o = prompt.prompt_attention(q, k2, v2, cu_q, cu_k, k_shared=s2)
+            assert torch.equal(o[:first], clean[:first])
+            seen = o[first:]
+            if at == 0 and low == float("-inf"):
+                assert seen[0].isnan().all()   # it is all that this query sees
+                seen = seen[1:]
+            if at == 0 and low == -30000.0:
+                # ... with all the weight there is
+                assert seen[0, :, 5].eq(float("inf")).all() and seen[0, :, 40].eq(-float("inf")).all()
+                seen = seen[1:]
+            if low is None:
+                assert seen[..., 5].eq(float("inf")).all()
+                assert seen[..., 40].eq(-float("inf")).all()
+            else:
+                assert seen[..., [5, 40]].isnan().all()
+            rest = [c for c in range(v_dim) if c not in (5, 40)]
+            assert seen[..., rest].isfinite().all()
