@@ -163,9 +163,10 @@ class DecoderHarness:
         self.cache = torch.zeros(L, *rows, cfg.kv_lora_rank + cfg.qk_rope, dtype=bf, device=dev)
         self.kv_status = torch.zeros((), dtype=torch.int32, device=dev)
         self._ones = torch.ones(batch, dtype=torch.int32, device=dev)
-        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.qk_rope, 2).float() / cfg.qk_rope))
-        ang = torch.arange(max_len).float()[:, None] * inv[None, :]
-        self.freqs = torch.polar(torch.ones_like(ang), ang).to(dev)   # complex64
+        # angles in 64 bits, as the prompt pass forms them: both write one cache
+        inv = cfg.rope_theta ** (torch.arange(0, cfg.qk_rope, 2).double() / -cfg.qk_rope)
+        ang = torch.arange(max_len).double()[:, None] * inv[None, :]
+        self.freqs = torch.polar(torch.ones_like(ang), ang).to(torch.complex64).to(dev)
         self.rope_cs = torch.view_as_real(self.freqs).contiguous()    # [max_len, r/2, 2]
         self.fused_attention = (self.device.type == "cuda") if fused_attention is None \
             else bool(fused_attention)

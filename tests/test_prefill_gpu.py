@@ -236,3 +236,25 @@ def test_prefill_reports_a_wait_that_ran_out(kw, monkeypatch):
     again = h.prefill(torch.cat(tokens).cuda(), [30, 1, 50])
     assert torch.equal(again, _harness(**kw).prefill(torch.cat(tokens).cuda(), [30, 1, 50]))
     h.check_blocks()
+
+
+def test_far_positions_have_the_same_keys_from_steps_and_prompts():
+    """A million positions on, the first layer's rotated keys of two tokens as
+    single steps and as a prompt's chunk write them."""
+    P, rope = 10 ** 6, V2_LITE_DECODER.qk_rope
+    ids = torch.tensor([7, 1999], device="cuda")
+    rows = []
+    for chunk in (False, True):
+        h = _harness(batch=1, max_len=P + 8, layers=1)
+        h.pos.fill_(P)
+        if chunk:
+            h.prefill(ids, [2], context=[P])
+        else:
+            for i in range(2):
+                h.step(ids[i:i + 1])
+        assert h.pos.tolist() == [P + 2]
+        rows.append(h.cache[0, 0, P:P + 2, -rope:].float())
+    a, b = (r.view(2, rope // 2, 2) for r in rows)
+    # a step of the projection's rounding between them, half a step of each
+    # result's: four half steps of a pair's length
+    assert ((a - b).abs().amax(-1) <= 4 * 2.0 ** -8 * a.norm(dim=-1)).all()

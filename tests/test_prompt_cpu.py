@@ -310,3 +310,21 @@ def test_outputs_whose_rows_share_memory_are_refused():
 def test_attention_of_columns_that_no_copy_aligns_ends_in_a_refusal():
     with pytest.raises(ValueError, match="CUDA"):
         prompt.prompt_attention(**_qkv(dim=67, v_dim=67))
+
+
+def test_decoder_angles_of_far_positions():
+    """The decode step's table of angles has the phase of the prompt pass's
+    64-bit ones, as far as the cache reaches."""
+    from dataclasses import replace
+
+    from sluice_b200.harness import V2_LITE_DECODER, DecoderHarness
+    cfg = replace(V2_LITE_DECODER, num_layers=1, vocab=16)
+    n = 70001
+    h = DecoderHarness(cfg, None, batch=1, max_len=n, device="cpu")
+    freqs, _ = prompt.rotary_frequencies(cfg.qk_rope, cfg.rope_theta)
+    for p in (0, 1, 4095, 65537, n - 1):
+        angle = p * freqs
+        want = torch.stack([angle.cos(), angle.sin()], dim=-1)
+        # one rounding to 32 bits of values up to one
+        assert (h.rope_cs[p].double() - want).abs().max() <= 2.0 ** -24
+        assert torch.equal(torch.view_as_real(h.freqs[p]), h.rope_cs[p])
