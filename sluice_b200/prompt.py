@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from typing import NamedTuple
 
 import torch
@@ -249,6 +250,7 @@ class Rotary:
     def _part(self, name: str, x: torch.Tensor, out: torch.Tensor | None, offset: int, T: int):
         """(the call's description of one tensor, its output, its input)."""
         in_place = out is x
+        offset = operator.index(offset)   # (layouts are kept by value)
         copied, x_strides, new = _rotary_input(name, x.shape, x.stride(), offset, T,
                                                self.rotary_dim)
         if out is None and new is not None:
@@ -446,7 +448,7 @@ def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
     a.Tq, a.Tk, a.B = Tq, Tk, nq - 1
     a.heads, a.kv_heads, a.dim, a.v_dim, a.shared_dim = heads, kv_heads, dim, v_dim, shared
     a.dtype = _DTYPES[dtype]
-    a.scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    a.scale = 1.0 / math.sqrt(dim) if scale is None else scale
     tiled = all(t is None or _tile_strides(*t) for t in (q, k, v, k_shared))
     return a, (Tq, heads, v_dim), tiled
 
@@ -518,6 +520,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     _vector("cu_k", cu_k, torch.int32)
     if status is not None:
         _vector("status", status, torch.int32, 1)
+    if scale is not None:
+        scale = float(scale)   # (layouts are kept by value)
     for copied in (False, True):
         layout, shape, tiled = _attention_layout(
             (q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()),

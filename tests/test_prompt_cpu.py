@@ -328,3 +328,15 @@ def test_decoder_angles_of_far_positions():
         # one rounding to 32 bits of values up to one
         assert (h.rope_cs[p].double() - want).abs().max() <= 2.0 ** -24
         assert torch.equal(torch.view_as_real(h.freqs[p]), h.rope_cs[p])
+
+
+def test_rotary_offsets_count_by_value():
+    """An offset that is a tensor, changed between two calls."""
+    r, x, at = prompt.Rotary(64, device="cpu"), torch.zeros(4, 2, 128), torch.tensor(64)
+    with pytest.raises(ValueError, match="CUDA"):
+        r(torch.arange(4), x, q_offset=at)
+    at.fill_(65)
+    with pytest.raises(ValueError, match="columns"):
+        r(torch.arange(4), x, q_offset=at)
+    with pytest.raises(TypeError):
+        r(torch.arange(4), x, q_offset=1.5)

@@ -323,3 +323,13 @@ def test_attention_of_an_infinite_value_at_a_weight_of_zero(dtype, heads, kv_hea
                 assert seen[..., [5, 40]].isnan().all()
             rest = [c for c in range(v_dim) if c not in (5, 40)]
             assert seen[..., rest].isfinite().all()
+
+
+def test_attention_scales_count_by_value():
+    """A scale that is a tensor, changed between two calls."""
+    q = torch.randn(40, 2, 64, device="cuda").bfloat16()
+    cu, scale = torch.tensor([0, 40], **I32), torch.tensor(0.05)
+    for value in (0.05, 2.0):
+        scale.fill_(value)
+        assert torch.equal(prompt.prompt_attention(q, q, q, cu, cu, scale=scale),
+                           prompt.prompt_attention(q, q, q, cu, cu, scale=value))
