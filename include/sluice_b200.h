@@ -552,7 +552,7 @@ typedef struct {
  * angle reduced in 64 bits. interleaved: pairs (2j, 2j + 1); otherwise
  * (j, j + rot / 2). Columns outside the rotated ones are copied. A row at a
  * negative position (padding) is copied whole; in place it is left as it was.
- * k may be NULL. rot even, at most 512; dim at most 4096. */
+ * k may be NULL. rot even, at most 512; dim at most 4096; T below 2^31 - 64. */
 int sl_rotary(const int64_t* positions, const double* turns, int T, int rot, int interleaved,
               float factor, int dtype, const sl_rotary_part* q, const sl_rotary_part* k,
               sl_stream_t stream);

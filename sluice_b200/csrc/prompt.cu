@@ -548,7 +548,8 @@ extern "C" int sl_rotary(const int64_t* positions, const double* turns, int T, i
                          const sl_rotary_part* k, sl_stream_t stream) {
   if (T < 0 || rot <= 0 || rot % 2 || !q || dtype < SL_DTYPE_BF16 || dtype > SL_DTYPE_FP32)
     return SL_ERR_INVALID;
-  if (rot > 2 * kRotMaxPairs) return SL_ERR_UNSUPPORTED;
+  // (rows rounded up to a CTA's, of 32 at most, are still counted in 32 bits)
+  if (rot > 2 * kRotMaxPairs || T > 0x7fffffff - 64) return SL_ERR_UNSUPPORTED;
   const sl_rotary_part none = {};
   const sl_rotary_part* parts[2] = {q, k ? k : &none};
   if (q->heads <= 0) return SL_ERR_INVALID;

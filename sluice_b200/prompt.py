@@ -34,6 +34,10 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16,
            torch.float32: _lib.DTYPE_FP32}
 
 
+_INT_MAX = 0x7fffffff
+_ROTARY_ROWS = _INT_MAX - 64   # of one call
+
+
 def _device_index(first: torch.Tensor, *others) -> int:
     """The index of the CUDA device of ``first``, which every other tensor is
     on too."""
@@ -151,6 +155,10 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
             raise ValueError("free_range_out overlaps half of free_range")
     if num_tokens < 0 or num_kv_tokens < 0:
         raise ValueError("num_tokens and num_kv_tokens are counts")
+    block_size = operator.index(block_size)
+    ring = 0 if free_blocks is None else free_blocks.numel()
+    if max(block_size, width, ring) > _INT_MAX:
+        raise ValueError("block_size, the table's width and the ring's size are 32-bit numbers")
     dev = _device_index(context_lens, new_lens, block_table, free_blocks, free_range,
                         free_range_out)
     # one allocation: the 64-bit outputs, then the 32-bit ones
@@ -159,8 +167,8 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     r = buf.data_ptr()
     c = r + 8 * n64
     _call(dev, "sl_plan_kv_blocks", context_lens.data_ptr(), new_lens.data_ptr(), B,
-          int(block_size), block_table.data_ptr(), ld, width, ptr(free_blocks),
-          0 if free_blocks is None else free_blocks.numel(), ptr(free_range),
+          block_size, block_table.data_ptr(), ld, width, ptr(free_blocks),
+          ring, ptr(free_range),
           ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
           r + 8 * num_tokens, r + 16 * num_tokens if num_kv_tokens else None, c + 8 * (B + 1))
     # (views; "unsafe" to autograd only, which has no part in this)
@@ -292,7 +300,8 @@ class Rotary:
         without ``k``), new tensors or ``out_q`` / ``out_k``; passing ``q``
         itself as ``out_q`` rotates in place. Rows at negative positions
         (padding) keep their values. Up to 512 rotated columns of up to 4096,
-        and fewer than 2^20 columns in all heads of a token."""
+        fewer than 2^20 columns in all heads of a token, and fewer than
+        2^31 - 64 rows."""
         dtype = _DTYPES.get(q.dtype)
         if dtype is None or (k is not None and k.dtype != q.dtype):
             raise ValueError("q and k must share one of bfloat16, float16, float32")
@@ -323,6 +332,8 @@ def _rotary_input(name: str, shape, strides, offset: int, T: int, rot: int):
     without the addresses), by its layout."""
     if len(shape) != 3 or shape[0] != T:
         raise ValueError(f"{name} must be [{T}, heads, dim], got {tuple(shape)}")
+    if T > _ROTARY_ROWS:
+        raise ValueError(f"{T} rows in one call, at most {_ROTARY_ROWS}")
     if not 0 <= offset <= shape[2] - rot:
         raise ValueError(f"{name}'s columns [{offset}, {offset + rot}) are not within its "
                          f"{shape[2]}")
@@ -427,6 +438,8 @@ def _attention_layout(q, k, v, k_shared, out, dtype, nq: int, nk: int, scale):
         raise ValueError(f"q has {dim} columns per head, k {own} + {shared}")
     if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
+    if nq > _INT_MAX:
+        raise ValueError(f"{nq - 1} sequences in one call")
     if nq < 1 or nk != nq:
         raise ValueError(f"cu_q has {nq} entries and cu_k {nk}: both have one per sequence and "
                          "one more")

@@ -340,3 +340,24 @@ def test_rotary_offsets_count_by_value():
         r(torch.arange(4), x, q_offset=at)
     with pytest.raises(TypeError):
         r(torch.arange(4), x, q_offset=1.5)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Not taken modulo 2^32, which is what a C int would keep of them."""
+    meta = dict(device="meta")
+    big = 2 ** 32 + 16
+    for change in (dict(block_size=big), dict(block_table=torch.empty(2, big, dtype=torch.int32, **meta)),
+                   dict(free_blocks=torch.empty(big, dtype=torch.int32, **meta))):
+        with pytest.raises(ValueError, match="32-bit"):
+            prompt.plan_kv_blocks(**{**_plan_args(), **change})
+    r = prompt.Rotary(2, device="cpu")
+    for T in (big, 2 ** 31 - 1):
+        x = torch.empty(T, 1, 2, dtype=torch.bfloat16, **meta)
+        with pytest.raises(ValueError, match="rows"):
+            r(torch.empty(T, dtype=torch.long, **meta), x)
+    cu = torch.empty(big, dtype=torch.int32, **meta)
+    with pytest.raises(ValueError, match="sequences"):
+        prompt.prompt_attention(**{**_qkv(), "cu_q": cu, "cu_k": cu})
+    p = _lib.RotaryPart(16, 16, 2, 2, 2, 2, 1, 2, 0)
+    assert _lib.lib().sl_rotary(256, 256, 2 ** 31 - 1, 2, 1, 1.0, 0, ctypes.byref(p), None, None) == \
+        _lib.SL_ERR_UNSUPPORTED
