@@ -355,12 +355,13 @@ class DecoderHarness:
         tokens). ``context`` are the positions, where the caller knows them;
         otherwise they are read back. Raises ``KvPlanError``, with nothing
         changed, where the pool has too few blocks left or a position before
-        the new tokens has none, and ``SluiceError``, with no position moved
-        and no block taken, where a layer's attention gave up on a wait. CUDA with the fused attention only; the
-        MoE layers take the pass as one step of T rows."""
+        the new tokens has none, and ``SluiceError`` where a layer's attention
+        gave up on a wait; an error, of the MoE layers too, moves no position
+        and takes no block. CUDA with the fused attention only; the MoE layers
+        take the pass as one step of T rows."""
         if not self.fused_attention:
             raise ValueError("prefill runs on a CUDA device with the fused attention")
-        from ._lib import KV_PLAN_BAD_INPUT, check
+        from ._lib import KV_PLAN_BAD_INPUT
         from .prompt import KvPlanError
         cfg, dev = self.cfg, self.device
         if len(lengths) != self.batch or any(n < 0 for n in lengths):
@@ -374,9 +375,8 @@ class DecoderHarness:
             raise ValueError(f"context must be {self.batch} positions")
         if any(c + n > self.max_len for c, n in zip(context, lengths)):
             raise ValueError(f"a sequence would pass max_len {self.max_len}")
-        nxt = torch.full((self.batch,), -1, dtype=torch.long, device=dev)
         if T == 0:
-            return nxt
+            return torch.full((self.batch,), -1, dtype=torch.long, device=dev)
         if self._rotary is None:
             from .prompt import Rotary
             self._rotary = Rotary(cfg.qk_rope, base=cfg.rope_theta, interleaved=True, device=dev)
@@ -396,10 +396,19 @@ class DecoderHarness:
             rows = plan.slots if plan.kv_slots is None else torch.cat([plan.slots, plan.kv_slots])
             if int(rows.min()) < 0:
                 raise KvPlanError(KV_PLAN_BAD_INPUT)
-        except RuntimeError:
+            nxt = self._prompt_pass(ids, lengths, plan, has_context)
+        except BaseException:
             self.restore_blocks(blocks0)
             raise
-        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.pos.add_(new)
+        return nxt
+
+    def _prompt_pass(self, ids: torch.Tensor, lengths: list[int], plan,
+                     has_context: bool) -> torch.Tensor:
+        """The layers over the packed rows of a plan that holds."""
+        from ._lib import check
+        cfg = self.cfg
+        status = torch.zeros(1, dtype=torch.int32, device=self.device)
         h = self.embed[ids]
         x = self._add_norm(h, None, self.layers[0]["in_norm"])
         for li in range(cfg.num_layers):
@@ -412,13 +421,9 @@ class DecoderHarness:
             x = self._add_norm(h, f, last)
         live = [b for b, n in enumerate(lengths) if n]
         ends = plan.cu_new[1:].long()[live] - 1
+        nxt = torch.full((self.batch,), -1, dtype=torch.long, device=self.device)
         nxt[live] = F.linear(x[ends], self.head).argmax(dim=-1)
-        try:
-            check(int(status), "prompt_attention")
-        except RuntimeError:
-            self.restore_blocks(blocks0)
-            raise
-        self.pos.add_(new)
+        check(int(status), "prompt_attention")
         return nxt
 
 

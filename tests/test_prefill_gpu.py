@@ -258,3 +258,25 @@ def test_far_positions_have_the_same_keys_from_steps_and_prompts():
     # a step of the projection's rounding between them, half a step of each
     # result's: four half steps of a pair's length
     assert ((a - b).abs().amax(-1) <= 4 * 2.0 ** -8 * a.norm(dim=-1)).all()
+
+
+def test_prefill_that_fails_in_a_layer_takes_no_blocks():
+    h = _harness(cache_blocks=8, block_size=32)
+    h.prefill(torch.cat(_tokens([20, 40, 1])).cuda(), [20, 40, 1])
+    before, pos, moe = h.save_blocks(), h.pos.tolist(), h.moe
+
+    def fails(li, x):
+        raise OSError("no experts")
+
+    h.moe = fails
+    more = torch.cat(_tokens([60, 0, 31], seed=6)).cuda()
+    for _ in range(3):
+        with pytest.raises(OSError):
+            h.prefill(more, [60, 0, 31])
+        assert h.pos.tolist() == pos
+        assert all(torch.equal(v, before[n]) for n, v in h.save_blocks().items())
+    h.moe = moe
+    nxt = h.prefill(more, [60, 0, 31])
+    assert nxt.tolist()[1] == -1 and h.pos.tolist() == [80, 40, 32]
+    assert h.free_range.tolist() == [6, 8]   # ceil(80 / 32) + ceil(40 / 32) + ceil(32 / 32)
+    h.check_blocks()
