@@ -512,10 +512,12 @@ class OffloadedDecoder:
 
     def restore(self, saved: dict) -> None:
         m = self.model
+        if m.paged and "blocks" not in saved:
+            raise ValueError("the state of a paged cache holds its blocks")
         m.cache.copy_(saved["cache"])
         m.pos.copy_(saved["pos"])
         self._ids.copy_(saved["ids"])
-        m.restore_blocks(saved["blocks"])
+        m.restore_blocks(saved.get("blocks", {}))
 
     def check(self) -> None:
         self.stack.check()

@@ -361,3 +361,20 @@ def test_sizes_past_32_bits_are_refused():
     p = _lib.RotaryPart(16, 16, 2, 2, 2, 2, 1, 2, 0)
     assert _lib.lib().sl_rotary(256, 256, 2 ** 31 - 1, 2, 1, 1.0, 0, ctypes.byref(p), None, None) == \
         _lib.SL_ERR_UNSUPPORTED
+
+
+def test_restore_of_a_state_without_blocks():
+    """A state that holds caches, positions and ids only, as a contiguous cache
+    needs them."""
+    from dataclasses import replace
+
+    from sluice_b200.harness import V2_LITE_DECODER, DecoderHarness, OffloadedDecoder
+    d = OffloadedDecoder.__new__(OffloadedDecoder)
+    d.model = DecoderHarness(replace(V2_LITE_DECODER, num_layers=1, vocab=16), None, batch=2,
+                             max_len=8, device="cpu")
+    d._ids = torch.tensor([3, 4])
+    saved = {n: t for n, t in d.save().items() if n != "blocks"}
+    d.model.pos.add_(5)
+    d._ids.zero_()
+    d.restore(saved)
+    assert d.model.pos.tolist() == [0, 0] and d._ids.tolist() == [3, 4]
