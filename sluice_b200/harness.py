@@ -216,8 +216,8 @@ class DecoderHarness:
         if status:
             raise KvPlanError(status)
 
-    def _attention(self, li: int, x: torch.Tensor, mask_bias: torch.Tensor,
-                   freqs: torch.Tensor) -> torch.Tensor:
+    def _attention(self, li: int, x: torch.Tensor, mask_bias: torch.Tensor | None,
+                   freqs: torch.Tensor | None) -> torch.Tensor:
         cfg, lw = self.cfg, self.layers[li]
         B, nh, R = x.shape[0], cfg.num_heads, cfg.kv_lora_rank
         dq = cfg.qk_nope + cfg.qk_rope
@@ -298,12 +298,17 @@ class DecoderHarness:
         h = self.embed[ids]
         if self.paged:
             self._plan(self.pos.to(torch.int32), self._ones, self.batch)
-        # per step: the positions' rotations and the causal mask as an additive
-        # bias over the cache (0 up to each sequence's position, -inf after)
-        freqs = self.freqs[self.pos]
-        mask_bias = torch.zeros(h.shape[0], 1, self.max_len, dtype=h.dtype, device=h.device)
-        mask_bias.masked_fill_((self._ar[None, :] > self.pos[:, None])[:, None, :],
-                               float("-inf"))
+        freqs = mask_bias = None
+        if self.fused_attention:
+            # (KV_PLAN_NO_BLOCKS is 1; the kernel stays within max_len)
+            torch.maximum(self.kv_status, (self.pos >= self.max_len).any(), out=self.kv_status)
+        else:
+            # per step: the positions' rotations and the causal mask as an additive
+            # bias over the cache (0 up to each sequence's position, -inf after)
+            freqs = self.freqs[self.pos]
+            mask_bias = torch.zeros(h.shape[0], 1, self.max_len, dtype=h.dtype, device=h.device)
+            mask_bias.masked_fill_((self._ar[None, :] > self.pos[:, None])[:, None, :],
+                                   float("-inf"))
         x = self._add_norm(h, None, self.layers[0]["in_norm"])
         for li in range(cfg.num_layers):
             lw = self.layers[li]

@@ -280,3 +280,21 @@ def test_prefill_that_fails_in_a_layer_takes_no_blocks():
     assert nxt.tolist()[1] == -1 and h.pos.tolist() == [80, 40, 32]
     assert h.free_range.tolist() == [6, 8]   # ceil(80 / 32) + ceil(40 / 32) + ceil(32 / 32)
     h.check_blocks()
+
+
+@pytest.mark.parametrize("kw", [{}, dict(cache_blocks=8, block_size=32),
+                                dict(cache_blocks=8, block_size=96)])
+def test_steps_past_the_last_position_are_reported(kw):
+    h = _harness(batch=2, max_len=96 if kw.get("block_size") == 32 else 80, **kw)
+    n = h.max_len - 1
+    ids = h.prefill(torch.cat(_tokens([n, 20])).cuda(), [n, 20])
+    other = _rows(h, 0, 1, 20)
+    ids = h.step(ids)   # the last position
+    h.check_blocks()
+    for _ in range(2):
+        ids = h.step(ids)
+        with pytest.raises(prompt.KvPlanError):
+            h.check_blocks()
+    assert torch.equal(_rows(h, 0, 1, 20), other)
+    h.reset()
+    h.check_blocks()
