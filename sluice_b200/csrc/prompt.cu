@@ -391,45 +391,41 @@ __global__ void __launch_bounds__(kRotThreads, V * sizeof(E) == 32   ? 8
   const int t0 = blockIdx.x * a.per_cta;
   const int nt = min(a.per_cta, a.T - t0);
   const int nq = a.t[0].heads * a.t[0].units, n = nq + a.t[1].heads * a.t[1].units;
-  constexpr int U = 1;  // items in flight per thread
-  Vec lo[U], hi[U];
-  E* dst[U];
-  int pair[U];   // first pair's place in cs, -1: not rotated
-  int to[U];     // from the first vector to the second, 0: there is none
-  int token[U];  // -1: no item
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kRotThreads;
-      token[u] = -1;
-      if (i >= nt * n) continue;
-      // i / n (exact: a CTA of several tokens has at most 2^12 items)
-      const int t = a.per_cta == 1 ? 0 : static_cast<int>((i + 0.5f) * a.inv_items);
-      const int w = i - t * n;
-      const RotTensor& x = w < nq ? a.t[0] : a.t[1];
-      const int idx = w < nq ? w : w - nq;
-      const int head = x.units == 1 ? idx
-                                    : static_cast<int>(__umulhi(static_cast<uint32_t>(idx), x.units_mul));
-      const int unit = idx - head * x.units;
-      int col;
-      if (unit < a.rot_units) {
-        col = x.offset + unit * (kInterleaved && V == 1 ? 2 : V);
-        pair[u] = t * half + unit;
-        to[u] = to_hi;
-      } else {
-        // columns that are not rotated, two vectors a unit: those before the
-        // rotated ones, then those behind them
-        const int c = (unit - a.rot_units) * (2 * V);
-        col = c < x.offset ? c : c + a.rot;
-        pair[u] = -1;
-        to[u] = c + V >= x.copied ? 0 : c + V == x.offset ? V + a.rot : V;
-      }
-      token[u] = t;
-      const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
-      dst[u] = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
-      lo[u] = *reinterpret_cast<const Vec*>(src);
-      if (to[u] != 0) hi[u] = *reinterpret_cast<const Vec*>(src + to[u]);
+  // the unit of a thread's turn
+  Vec lo, hi;
+  E* dst;
+  int pair;   // first pair's place in cs, -1: not rotated
+  int to;     // from the first vector to the second, 0: there is none
+  int token;  // -1: no unit
+  auto load = [&](int i) {
+    token = -1;
+    if (i >= nt * n) return;
+    // i / n (exact: a CTA of several tokens has at most 2^12 items)
+    const int t = a.per_cta == 1 ? 0 : static_cast<int>((i + 0.5f) * a.inv_items);
+    const int w = i - t * n;
+    const RotTensor& x = w < nq ? a.t[0] : a.t[1];
+    const int idx = w < nq ? w : w - nq;
+    const int head = x.units == 1 ? idx
+                                  : static_cast<int>(__umulhi(static_cast<uint32_t>(idx), x.units_mul));
+    const int unit = idx - head * x.units;
+    int col;
+    if (unit < a.rot_units) {
+      col = x.offset + unit * (kInterleaved && V == 1 ? 2 : V);
+      pair = t * half + unit;
+      to = to_hi;
+    } else {
+      // columns that are not rotated, two vectors a unit: those before the
+      // rotated ones, then those behind them
+      const int c = (unit - a.rot_units) * (2 * V);
+      col = c < x.offset ? c : c + a.rot;
+      pair = -1;
+      to = c + V >= x.copied ? 0 : c + V == x.offset ? V + a.rot : V;
     }
+    token = t;
+    const E* src = static_cast<const E*>(x.x) + (t0 + t) * x.xs + head * x.xh + col;
+    dst = static_cast<E*>(x.y) + (t0 + t) * x.ys + head * x.yh + col;
+    lo = *reinterpret_cast<const Vec*>(src);
+    if (to != 0) hi = *reinterpret_cast<const Vec*>(src + to);
   };
   // the first rows are on their way while the angles are formed
   load(threadIdx.x);
@@ -448,29 +444,26 @@ __global__ void __launch_bounds__(kRotThreads, V * sizeof(E) == 32   ? 8
     if (j == 0) s_skip[t] = p < 0;
   }
   __syncthreads();
-  for (int i0 = threadIdx.x;;) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (token[u] < 0) continue;
-      if (pair[u] >= 0 && !s_skip[token[u]]) {
+  for (int i = threadIdx.x;;) {
+    if (token >= 0) {
+      if (pair >= 0 && !s_skip[token]) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float2 c = cs[pair[u] + k * a.rot_units];
+          const float2 c = cs[pair + k * a.rot_units];
           constexpr int kIn = V > 1 ? V / 2 : 1;  // pairs of one vector
-          E& e0 = !kWithin ? lo[u].e[k] : k < kIn ? lo[u].e[2 * k % V] : hi[u].e[2 * k % V];
-          E& e1 = !kWithin ? hi[u].e[k]
-                           : k < kIn ? lo[u].e[(2 * k + 1) % V] : hi[u].e[(2 * k + 1) % V];
+          E& e0 = !kWithin ? lo.e[k] : k < kIn ? lo.e[2 * k % V] : hi.e[2 * k % V];
+          E& e1 = !kWithin ? hi.e[k] : k < kIn ? lo.e[(2 * k + 1) % V] : hi.e[(2 * k + 1) % V];
           const float x0 = to_f(e0), x1 = to_f(e1);
           e0 = from_f<E>(fmaf(x0, c.x, -__fmul_rn(x1, c.y)));
           e1 = from_f<E>(fmaf(x1, c.x, __fmul_rn(x0, c.y)));
         }
       }
-      *reinterpret_cast<Vec*>(dst[u]) = lo[u];
-      if (to[u] != 0) *reinterpret_cast<Vec*>(dst[u] + to[u]) = hi[u];
+      *reinterpret_cast<Vec*>(dst) = lo;
+      if (to != 0) *reinterpret_cast<Vec*>(dst + to) = hi;
     }
-    i0 += U * kRotThreads;
-    if (i0 >= nt * n) break;
-    load(i0);
+    i += kRotThreads;
+    if (i >= nt * n) break;
+    load(i);
   }
 }
 
