@@ -1,5 +1,7 @@
 """The prompt pass's operators at the edges of what their calls allow."""
 
+import math
+
 import pytest
 import torch
 
@@ -333,3 +335,66 @@ def test_attention_scales_count_by_value():
         scale.fill_(value)
         assert torch.equal(prompt.prompt_attention(q, q, q, cu, cu, scale=scale),
                            prompt.prompt_attention(q, q, q, cu, cu, scale=value))
+
+
+@pytest.mark.parametrize("cq,ck,q_len,k_len,rows", [
+    ([0, 1000], [0, 64], 64, 64, (0, 64)), ([0, 64], [0, 5000], 64, 64, (0, 64)),
+    ([-50, 64], [-9, 64], 64, 64, (0, 64)), ([0, 64], [60, 10], 64, 0, (0, 64)),
+    ([0, 64], [2000000000, 2000000100], 64, 0, (0, 64)),
+    # (rows 20 to 39 belong to two sequences; those behind see no keys)
+    ([0, 40, 20, 64], [0, 64, 64, 64], 40, 64, (0, 20)), ([0, 40, 20, 64], [0, 64, 64, 64], 64, 0, (40, 64))])
+def test_attention_of_offsets_cut_to_the_tensors(cq, ck, q_len, k_len, rows):
+    """Offsets past the tensors count as their ends, and a sequence that runs
+    backwards is empty; no wait runs out."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    q, k, v = (torch.randn(64, 2, 64, device="cuda", generator=g).bfloat16() for _ in range(3))
+    word = torch.zeros(1, **I32)
+    out = prompt.prompt_attention(q, k, v, torch.tensor(cq, **I32), torch.tensor(ck, **I32),
+                                  status=word)
+    assert word.item() == 0
+    ref, mag = oprompt.attention(q, k, v, [q_len], [k_len], 64 ** -0.5)
+    a, b = rows
+    _close(out[a:b], ref[a:b], mag[a:b])
+
+
+# ------------------------------------------------------------------- rotary
+def _frequencies(kind, rot, base=10000.0):
+    f = [base ** (-2.0 * i / rot) for i in range(rot // 2)]
+    if kind == "linear":
+        return [x / 4.0 for x in f], {"type": kind, "factor": 4.0}
+    if kind == "ntk":
+        b = base * 3.0 ** (rot / (rot - 2))
+        return [b ** (-2.0 * i / rot) for i in range(rot // 2)], {"type": kind, "factor": 3.0}
+
+    def llama3(x):
+        wave = 2 * math.pi / x
+        if wave < 8192 / 4.0:
+            return x
+        if wave > 8192 / 1.0:
+            return x / 8.0
+        smooth = (8192 / wave - 1.0) / (4.0 - 1.0)
+        return (1 - smooth) * x / 8.0 + smooth * x
+
+    return [llama3(x) for x in f], {"type": kind, "factor": 8.0, "original_max": 8192,
+                                    "low_freq_factor": 1.0, "high_freq_factor": 4.0}
+
+
+@pytest.mark.parametrize("kind", ["linear", "ntk", "llama3"])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotary_of_scaled_frequencies(kind, interleaved, dtype):
+    T, rot = 37, 64
+    freqs, scaling = _frequencies(kind, rot)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    x = torch.randn(T, 3, 96, device="cuda", generator=g).to(dtype)
+    pos = torch.randint(0, 1 << 20, (T,), device="cuda", generator=g)
+    y = prompt.Rotary(rot, scaling=scaling, interleaved=interleaved)(pos, x, q_offset=8)
+    ref = oprompt.rotary(x, pos, torch.tensor(freqs, dtype=torch.float64), 1.0, 8, interleaved)
+    # half a step of the result; 8 half steps of 32 bits of a pair's magnitude for
+    # the angle, the sine and the products; and the frequencies' own powers, 4 steps
+    # of 2^-52 relative to an angle of 2^20 at most
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + \
+        (8 * 2.0 ** -24 + 2.0 ** 20 * 2.0 ** -50) * 2 * x.double().abs().amax() + 2.0 ** -25
+    assert ((y.double() - ref).abs() <= tol).all()
