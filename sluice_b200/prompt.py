@@ -482,11 +482,11 @@ _failed: dict[int, torch.Tensor] = {}
 def _failed_word(dev: int) -> torch.Tensor | None:
     word = _failed.get(dev)
     if word is None:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(dev), torch.inference_mode(False):
             # (what a capture allocates belongs to its graph: the word of a
             # process whose first call is captured comes with a later call)
             if not torch.cuda.is_current_stream_capturing():
-                word = _failed[dev] = torch.zeros(1, dtype=torch.int32, device="cuda")
+                word = _failed.setdefault(dev, torch.zeros(1, dtype=torch.int32, device="cuda"))
     return word
 
 
