@@ -298,6 +298,17 @@ cudaError_t ensure_smem_limit(Kernel kernel, int bytes, std::atomic<uint64_t>& d
   return e;
 }
 
+// A tensor map's encoding needs a current context, and a host thread has none
+// before its first runtime call that makes one (the caching allocator's and the
+// stream's lookups are none): `encode` is called again with the current device's.
+template <typename Encode>
+bool encode_in_context(Encode encode) {
+  if (encode() == CUDA_SUCCESS) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess &&
+         encode() == CUDA_SUCCESS;
+}
+
 // Launch with programmatic stream serialisation (PDL) when enabled.
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

@@ -1,6 +1,7 @@
 """The prompt pass's operators at the edges of what their calls allow."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -398,3 +399,42 @@ def test_rotary_of_scaled_frequencies(kind, interleaved, dtype):
     tol = torch.finfo(dtype).eps / 2 * ref.abs() + \
         (8 * 2.0 ** -24 + 2.0 ** 20 * 2.0 ** -50) * 2 * x.double().abs().amax() + 2.0 ** -25
     assert ((y.double() - ref).abs() <= tol).all()
+
+
+def test_the_devices_status_word_of_two_threads_and_inference_mode(monkeypatch):
+    """First calls at the same time, in inference mode: one word, which is read
+    and cleared outside of it."""
+    monkeypatch.setattr(prompt, "_failed", {})
+    q = torch.randn(9, 2, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 9], **I32)
+    gate, words = threading.Barrier(4), []
+
+    def work():
+        with torch.inference_mode():
+            gate.wait()
+            prompt.prompt_attention(q, q, q, cu, cu)
+            words.append(prompt._failed_word(0).data_ptr())
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(words) == 4 and len(set(words)) == 1
+    prompt._failed[0].fill_(_lib.SL_ERR_TIMEOUT)
+    with pytest.raises(_lib.SluiceError):
+        prompt.check_attention()
+    prompt.check_attention()
+
+
+def test_attention_as_the_first_call_of_a_thread():
+    """A host thread that has called nothing of the device yet."""
+    q = torch.randn(50, 4, 64, device="cuda").bfloat16()
+    cu = torch.tensor([0, 50], **I32)
+    outs = [prompt.prompt_attention(q, q, q, cu, cu) for _ in range(2)]
+    want = outs.pop().clone()
+    outs.clear()   # (the thread's allocations come from the cache)
+    t = threading.Thread(target=lambda: outs.append(prompt.prompt_attention(q, q, q, cu, cu)))
+    t.start()
+    t.join()
+    assert outs and torch.equal(outs[0], want)
