@@ -320,3 +320,24 @@ def test_four_part_split_on_two_streams(fp8, T):
                               **kw)
     torch.cuda.synchronize()
     assert torch.equal(whole, out)
+
+
+def test_fused_experts_as_the_first_call_of_a_thread():
+    """A host thread that has called nothing of the device yet."""
+    import threading
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    hs = torch.randn(4, 256, device="cuda", generator=g).bfloat16()
+    w1, w2 = (torch.randn(4, n, 256, device="cuda", generator=g).mul(0.02).bfloat16()
+              for n in (512, 256))
+    tw = torch.rand(4, 2, device="cuda", generator=g)
+    ti = torch.tensor([[0, 1], [1, 2], [2, 3], [3, 0]], dtype=torch.int32, device="cuda")
+    outs = [ops.fused_experts(hs, w1, w2, tw, ti) for _ in range(2)]
+    want = outs.pop().clone()
+    outs.clear()   # (the thread's allocations come from the cache)
+    ops.fused_experts.last_workspace = None
+    t = threading.Thread(target=lambda: outs.append(ops.fused_experts(hs, w1, w2, tw, ti)))
+    t.start()
+    t.join()
+    assert outs and torch.equal(outs[0], want)
