@@ -568,7 +568,8 @@ int sl_rotary(const int64_t* positions, const double* turns, int T, int rot, int
  * out = softmax(scale * q k^T) v per head, head h reading key head
  * h / (heads / kv_heads). A query that sees no key gets zeros; rows of q that
  * belong to no sequence leave their output rows as they were; keys and
- * values that no query may see do not reach the output, whatever they hold.
+ * values that no query may see do not reach the output, whatever they hold; a
+ * value that is not finite makes NaN of its column where the weight is zero.
  * Strides in elements, last dimension contiguous, multiples of 8; addresses
  * 16-byte aligned. bf16 or fp16; (dim, v_dim) one of (64, 64), (128, 128),
  * (192, 128); shared_dim 0 or, at dim 192, 64; at most 128 heads per key

@@ -31,10 +31,10 @@
 // Then the hand-overs count: named barriers instead of mbarriers between warps,
 // waits without a suspend hint or a vote (82 -> 74 us), the maximum taken outside
 // the turn (16384 tokens on 32 / 4 heads of 128: 1.93 -> 1.77 ms). Now, device time:
-//   4096 tokens, 16 heads of 192 / 128        72 us, 1194 TFLOP/s, 0.73 of cuBLAS's burst
-//   16384 tokens, 32 / 4 heads of 128       1.80 ms, 1220 TFLOP/s, 0.89 of cuBLAS's
-//                                             sustained rate (the power cap; 1.62 ms before)
-//   8 single tokens over 60 000 keys, 32 / 4  33 us, 19 of them the bytes; 8 until the first
+//   4096 tokens, 16 heads of 192 / 128        73 us, 1180 TFLOP/s, 0.72 of cuBLAS's burst
+//   16384 tokens, 32 / 4 heads of 128       1.88 ms, 1172 TFLOP/s, 0.86 of cuBLAS's
+//                                             sustained rate (the power cap; 1.64 ms before)
+//   8 single tokens over 60 000 keys, 32 / 4  34 us, 19 of them the bytes; 8 until the first
 //                                             scores are there, 5 for the join
 // Measured and not kept: part of the exponentials as a cubic on the FMA pipes
 // (73.5 us with a quarter against 72.5), 16 softmax warps with a row in two

@@ -87,7 +87,10 @@ __device__ __forceinline__ int col16(int lane, int i) {
 // Where a sequence's cached rows are: one run of max_len rows (kPaged false),
 // or blocks of block_size rows (a multiple of kRingRows, so that a chunk lies in
 // one block) listed in the sequence's block table row. A block id outside the
-// pool reads block 0 and writes nothing (the planner has reported it).
+// pool reads block 0 and writes nothing (the planner has reported it). The table
+// entry is loaded when a chunk's copy is issued, one load before it: 8 sequences
+// behind 1000 positions, 16 heads, 53.6 us in blocks of 64 and 56.8 in blocks of 32
+// (one run of rows 47.7); behind 8000 353 and 373 (308).
 struct Pages {
   const int32_t* table;
   int64_t ld;

@@ -20,8 +20,8 @@ namespace {
 // CTAs that updates it in place (plan_range_kernel then writes it).
 //
 // Bound by latency: the lengths, the scan, a search and a table entry follow one
-// another. Eight single tokens take 3.5 us, 256 take 4.1, 72 000 rows 6.2, 2.2
-// million (17 MB, 2.6 us at copy bandwidth) 16; with a row a lane at a time and
+// another. Eight single tokens take 3.8 to 4.4 us, 256 take 4.5, 72 000 rows 6.5,
+// 2.2 million (17 MB, 2.6 us at copy bandwidth) 16; with a row a lane at a time and
 // one warp for the table the last two took 35 and 40 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxRequests = 8192;

@@ -210,7 +210,7 @@ class DecoderHarness:
 
     def check_blocks(self) -> None:
         """Raise if a step since ``reset`` found no block for a position, or
-        no room below ``max_len`` (synchronises)."""
+        no room below ``max_len``, on either cache (synchronises)."""
         from .prompt import KvPlanError
         status = int(self.kv_status.item())
         if status:
