@@ -61,11 +61,11 @@ constexpr int kBars = 16;            // barriers of tiles in flight; even ones k
 // that no sum of weighted values passes the largest value (weights below 2^-86 of
 // the maximum's become zero). fp16 ones end at 2^16 and, below 2^-14, lose bits: of
 // weights of 2^-21 of the maximum's and less, 2^-33 of its, so that 2^21 keys lose
-// half an output's rounding at most (a lag of 4 would keep 2^4 more of them, but
-// scores that spread by 3 then move the maximum often: 8192 tokens on 16 / 4 heads
-// 276 us instead of 245; of 12 228). bf16: (16384 tokens, 8 / 2 heads of
-// 128, scores that spread by 1, 3 and 6: 409, 413 and 415 us; with a lag of 8 410,
-// 443 and 492, of 32 410, 412 and 410.)
+// half an output's rounding at most. A smaller lag moves the maximum more often:
+// bf16, 16384 tokens on 8 / 2 heads of 128, scores that spread by 1, 3 and 6, 409,
+// 413 and 415 us; with a lag of 8 410, 443 and 492, of 32 410, 412 and 410. fp16,
+// 8192 tokens on 16 / 4 heads, scores that spread by 3, 245; with 4, which would
+// keep weights 2^4 smaller, 276, with 12 228.
 constexpr float kLagBf16 = 24.f, kLagF16 = 8.f;
 constexpr float kTopBf16 = -40.f, kTopF16 = 7.f;
 // registers a thread: 168 at launch, then shared out between the softmax warps

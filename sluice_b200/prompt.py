@@ -155,7 +155,7 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
             raise ValueError("free_range_out overlaps half of free_range")
     if num_tokens < 0 or num_kv_tokens < 0:
         raise ValueError("num_tokens and num_kv_tokens are counts")
-    block_size = operator.index(block_size)
+    block_size = int(block_size)
     ring = 0 if free_blocks is None else free_blocks.numel()
     if max(block_size, width, ring) > _INT_MAX:
         raise ValueError("block_size, the table's width and the ring's size are 32-bit numbers")
@@ -167,8 +167,7 @@ def plan_kv_blocks(context_lens: torch.Tensor, new_lens: torch.Tensor,
     r = buf.data_ptr()
     c = r + 8 * n64
     _call(dev, "sl_plan_kv_blocks", context_lens.data_ptr(), new_lens.data_ptr(), B,
-          block_size, block_table.data_ptr(), ld, width, ptr(free_blocks),
-          ring, ptr(free_range),
+          block_size, block_table.data_ptr(), ld, width, ptr(free_blocks), ring, ptr(free_range),
           ptr(free_range_out), num_tokens, num_kv_tokens, c, c + 4 * (B + 1), r,
           r + 8 * num_tokens, r + 16 * num_tokens if num_kv_tokens else None, c + 8 * (B + 1))
     # (views; "unsafe" to autograd only, which has no part in this)
